@@ -1,8 +1,10 @@
 /*
  * B200 additions to the aclsparse API.  The reference library drives one
  * device through one stream and has no multi-device code, so the entry points
- * in this header have no counterpart there; they carry the one piece of the
- * multi-GPU path that has to run where the matrix lives.
+ * in this header have no counterpart there; they carry the pieces of the
+ * multi-GPU path that have to run where the matrix lives, a product that needs
+ * no buffer, and the dense products of ragged row groups (experts) that stand
+ * between the sparse operators of a mixture-of-experts layer.
  */
 #ifndef ACLSPARSE_B200_EXT_H_
 #define ACLSPARSE_B200_EXT_H_
@@ -98,6 +100,73 @@ aclsparseStatus_t aclsparseB200DnVecSetClosingBarrier(aclsparseDnVecDescr_t vec,
 aclsparseStatus_t aclsparseB200DnMatSetClosingBarrier(aclsparseDnMatDescr_t mat, void* localState,
                                                       void* const* peerStates, int world, int rank,
                                                       unsigned spinLimit);
+
+/* Grouped matrix product: the product of a block-diagonal matrix of ragged dense row blocks with one dense
+ * matrix per block, as a mixture-of-experts layer computes it once its rows are sorted by expert:
+ *     C[r, :] = alpha * rowScales[r] * (A[r, :] * op(B_g)) .* colScales[g, :] + beta * C[r, :]
+ * for the rows r of group g, groupOffsets[g] <= r < groupOffsets[g + 1].
+ *   matA  rows x k, row-major.  matC  rows x n, row-major.  matB  one batch entry per group
+ *         (aclsparseDnMatSetStridedBatch), op(B_g) is k x n, row- or column-major, op N / T (H is T).
+ *   groupOffsets  DEVICE array of groups + 1 int32, ascending; NULL with a single group: all rows.  Its content is
+ *         never trusted with an address: values are clamped to [0, rows], and to the largest one before them.
+ *   rowScales (rows floats) and colScales (groups x n floats), DEVICE arrays, may be NULL: ones.
+ *   types  A, B fp16 or bf16 with C of that type or fp32: fp32 sums; A, B int8 with C fp32, fp16 or bf16: exact
+ *         int32 sums, k <= 131071.  The compute type is ACL_FLOAT.  The result is formed in fp32 and rounded once
+ *         to the type of C.  Others, also mirrors and closing barriers on C: NOT_SUPPORTED.
+ * Rows of C outside [groupOffsets[0], groupOffsets[groups]) are left as they are; beta == 0 does not read C; an
+ * empty group costs nothing; k == 0 gives beta * C.  C must not overlap A or B.  Results do not depend on
+ * scheduling.  The buffer holds partial sums of products split along k: 64-byte aligned, one call at a time.
+ * Preprocess clears its counters; it is optional: a product that finds no Preprocess of its matC for this buffer
+ * on this stream clears them itself, with one more launch.  Asynchronous on the handle's stream.
+ * No counterpart in the reference. */
+aclsparseStatus_t aclsparseB200GroupedMMGetBufferSize(aclsparseHandle_t handle, aclsparseOperation_t opB,
+                                                      const void* alpha, aclsparseConstDnMatDescr_t matA,
+                                                      const int32_t* groupOffsets, aclsparseConstDnMatDescr_t matB,
+                                                      const float* rowScales, const float* colScales, const void* beta,
+                                                      aclsparseDnMatDescr_t matC, aclDataType computeType,
+                                                      size_t* bufferSize);
+aclsparseStatus_t aclsparseB200GroupedMMPreprocess(aclsparseHandle_t handle, aclsparseOperation_t opB,
+                                                   const void* alpha, aclsparseConstDnMatDescr_t matA,
+                                                   const int32_t* groupOffsets, aclsparseConstDnMatDescr_t matB,
+                                                   const float* rowScales, const float* colScales, const void* beta,
+                                                   aclsparseDnMatDescr_t matC, aclDataType computeType,
+                                                   void* externalBuffer);
+aclsparseStatus_t aclsparseB200GroupedMM(aclsparseHandle_t handle, aclsparseOperation_t opB, const void* alpha,
+                                         aclsparseConstDnMatDescr_t matA, const int32_t* groupOffsets,
+                                         aclsparseConstDnMatDescr_t matB, const float* rowScales,
+                                         const float* colScales, const void* beta, aclsparseDnMatDescr_t matC,
+                                         aclDataType computeType, void* externalBuffer);
+
+/* The gradient of the grouped product with respect to its weights:
+ *     C_g = alpha * A_g^T * B_g + beta * C_g,
+ * A_g and B_g being the rows groupOffsets[g] .. groupOffsets[g + 1] of matA (rows x m, row-major) and matB
+ * (rows x n, row-major), C_g batch entry g of matC (m x n, row- or column-major).  With y = x * W_g^T the gradient of
+ * W_g is the product of A = dy and B = x.  fp16 or bf16 with C of that type or fp32 (beta = 1 accumulates);
+ * an empty group gives beta * C_g.  groupOffsets, the buffer, Preprocess and everything else as above. */
+aclsparseStatus_t aclsparseB200GroupedMMWeightGradGetBufferSize(
+    aclsparseHandle_t handle, const void* alpha, aclsparseConstDnMatDescr_t matA, aclsparseConstDnMatDescr_t matB,
+    const int32_t* groupOffsets, const void* beta, aclsparseDnMatDescr_t matC, aclDataType computeType,
+    size_t* bufferSize);
+aclsparseStatus_t aclsparseB200GroupedMMWeightGradPreprocess(
+    aclsparseHandle_t handle, const void* alpha, aclsparseConstDnMatDescr_t matA, aclsparseConstDnMatDescr_t matB,
+    const int32_t* groupOffsets, const void* beta, aclsparseDnMatDescr_t matC, aclDataType computeType,
+    void* externalBuffer);
+aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t handle, const void* alpha,
+                                                   aclsparseConstDnMatDescr_t matA, aclsparseConstDnMatDescr_t matB,
+                                                   const int32_t* groupOffsets, const void* beta,
+                                                   aclsparseDnMatDescr_t matC, aclDataType computeType,
+                                                   void* externalBuffer);
+
+/* Rows of a matrix in 8 bits with one scale each, the operand of the int8 product above:
+ *     scales[r] = max_k |X[r, k]| / 127   (fp32, correctly rounded),
+ *     Q[r, k]   = X[r, k] / scales[r], the exact quotient rounded to the nearest integer, ties to even
+ * (and held to +-127, which only matters where the scale is subnormal).
+ * matX fp32, fp16 or bf16, matQ int8, both rows x cols, row-major with any leading dimension; scales: DEVICE array of
+ * rows floats.  A row of zeros, and one so small that its scale rounds to zero, gives zeros with the scale 0.  A row
+ * that holds an infinity or a NaN gives zeros with that scale, infinite or NaN: a product with it is then NaN
+ * throughout, never silently finite.  Asynchronous on the handle's stream.  No counterpart in the reference. */
+aclsparseStatus_t aclsparseB200QuantizeRows(aclsparseHandle_t handle, aclsparseConstDnMatDescr_t matX,
+                                            aclsparseDnMatDescr_t matQ, float* scales);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

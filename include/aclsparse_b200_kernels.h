@@ -216,6 +216,48 @@ typedef struct AclspNodeBarrierState {
 void aclsp_b200_node_barrier_kernel_do(void* localState, void* const* peerStates, uint32_t world, uint32_t rank,
                                        uint32_t spinLimit, void* stream);
 
+/* Per-launch parameters of the grouped matrix products.  Two forms share the block:
+ *   forward   C[r, n] = alpha * rowScales[r] * colScales[g * n + ..] * sum_k A[r, k] * op(B_g)[k, n] + beta * C[r, n]
+ *   gradient  C_g[m, n] = alpha * sum_r A[r, m] * B[r, n] + beta * C_g[m, n]     (weightGrad != 0)
+ * Strides are in elements.  An operand's element (i, k) lies at i * strideOuter + k * strideInner, i being its row or
+ * column in the result and k the summed index; one of the two strides is 1. */
+typedef struct AclspGroupedParams {
+    uint32_t rows;            /* rows of A (and of B in the gradient) */
+    uint32_t groups;
+    uint32_t m;               /* gradient: rows of C_g */
+    uint32_t n;               /* columns of C */
+    uint32_t k;               /* forward: the summed index */
+    uint32_t weightGrad;
+    uint32_t inType;          /* ACLSP_TYPE_F16, _BF16 or _I8 */
+    uint32_t outType;         /* ACLSP_TYPE_F32, _F16 or _BF16 */
+    int64_t aOuter, aInner;
+    int64_t bOuter, bInner;
+    int64_t bBatchStride;     /* forward: from B_g to B_(g+1) */
+    int64_t ldc;
+    int64_t cBatchStride;     /* gradient: from C_g to C_(g+1) */
+    float alpha;              /* used when alphaPtr == NULL (host pointer mode) */
+    float beta;
+    const float* alphaPtr;
+    const float* betaPtr;
+    const int32_t* offsets;   /* groups + 1 values, or NULL: one group of all rows */
+    const float* rowScales;
+    const float* colScales;
+} AclspGroupedParams;
+
+/* Bytes of buffer that the launcher below wants for these parameters (a host computation). */
+uint64_t aclsp_b200_grouped_buffer_bytes(const AclspGroupedParams* params);
+
+/* Clears the counters in the buffer of a grouped product: one small launch. */
+void aclsp_b200_grouped_preprocess_kernel_do(void* buffer, void* stream);
+
+/* The grouped product, or its weight gradient, over a buffer whose counters are clear; it leaves them clear. */
+void aclsp_b200_grouped_mm_kernel_do(const void* a, const void* b, void* c, void* buffer,
+                                     const AclspGroupedParams* params, void* stream);
+
+/* Rows in 8 bits with one fp32 scale each; xType is ACLSP_TYPE_F32, _F16 or _BF16, strides in elements. */
+void aclsp_b200_quantize_rows_kernel_do(const void* x, void* q, float* scales, uint32_t rows, uint32_t cols,
+                                        int64_t ldx, int64_t ldq, uint32_t xType, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -88,6 +88,16 @@ class SpmmParams(ctypes.Structure):
                 ("alphaInt", ctypes.c_int32), ("betaInt", ctypes.c_int32), ("barrier", BarrierLink)]
 
 
+class GroupedParams(ctypes.Structure):
+    """AclspGroupedParams of include/aclsparse_b200_kernels.h."""
+    _fields_ = [("rows", c_uint32), ("groups", c_uint32), ("m", c_uint32), ("n", c_uint32), ("k", c_uint32),
+                ("weightGrad", c_uint32), ("inType", c_uint32), ("outType", c_uint32),
+                ("aOuter", c_int64), ("aInner", c_int64), ("bOuter", c_int64), ("bInner", c_int64),
+                ("bBatchStride", c_int64), ("ldc", c_int64), ("cBatchStride", c_int64),
+                ("alpha", c_float), ("beta", c_float), ("alphaPtr", c_void_p), ("betaPtr", c_void_p),
+                ("offsets", c_void_p), ("rowScales", c_void_p), ("colScales", c_void_p)]
+
+
 _P = c_void_p
 _PP = POINTER(c_void_p)
 _I64P = POINTER(c_int64)
@@ -184,6 +194,13 @@ SIGNATURES = {
     "aclsparseB200SpMVWaitFailures": [_P, _P, POINTER(c_uint32)],
     "aclsparseB200DnVecSetClosingBarrier": [_P, _P, POINTER(c_void_p), c_int, c_int, c_uint32],
     "aclsparseB200DnMatSetClosingBarrier": [_P, _P, POINTER(c_void_p), c_int, c_int, c_uint32],
+    "aclsparseB200GroupedMMGetBufferSize": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, POINTER(c_size_t)],
+    "aclsparseB200GroupedMMPreprocess": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, _P],
+    "aclsparseB200GroupedMM": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, _P],
+    "aclsparseB200GroupedMMWeightGradGetBufferSize": [_P, _P, _P, _P, _P, _P, _P, c_int, POINTER(c_size_t)],
+    "aclsparseB200GroupedMMWeightGradPreprocess": [_P, _P, _P, _P, _P, _P, _P, c_int, _P],
+    "aclsparseB200GroupedMMWeightGrad": [_P, _P, _P, _P, _P, _P, _P, c_int, _P],
+    "aclsparseB200QuantizeRows": [_P, _P, _P, _P],
     # include/aclsparse_b200_kernels.h
     "spmv_b200_preprocess_kernel_do": [_P, _P, c_uint32, c_uint32, c_uint32, c_int32, c_int64, _P],
     "spmv_b200_kernel_do": [_P, _P, _P, _P, _P, POINTER(SpmvParams), _P],
@@ -193,14 +210,21 @@ SIGNATURES = {
     "aclsp_b200_push_slice_kernel_do": [_P, POINTER(c_void_p), c_uint32, c_int64, c_int64, _P],
     "aclsp_b200_node_barrier_kernel_do": [_P, POINTER(c_void_p), c_uint32, c_uint32, c_uint32, _P],
     "aclsp_b200_kernel_launches": [],
+    "aclsp_b200_grouped_buffer_bytes": [POINTER(GroupedParams)],
+    "aclsp_b200_grouped_preprocess_kernel_do": [_P, _P],
+    "aclsp_b200_grouped_mm_kernel_do": [_P, _P, _P, _P, POINTER(GroupedParams), _P],
+    "aclsp_b200_quantize_rows_kernel_do": [_P, _P, _P, c_uint32, c_uint32, c_int64, c_int64, c_uint32, _P],
     "aclsp_b200_transpose_build_kernel_do": [_P, _P, c_uint32, c_uint32, c_uint32, c_int32, c_int64, c_int64, _P, _P, _P],
     "aclsp_b200_transpose_values_kernel_do": [_P, c_int64, c_uint32, c_uint32, _P, _P, c_uint32, _P],
 }
 _VOID = {"spmv_b200_preprocess_kernel_do", "spmv_b200_kernel_do", "spmm_b200_preprocess_kernel_do",
          "spmm_b200_kernel_do", "aclsp_b200_row_block_bounds_kernel_do", "aclsp_b200_push_slice_kernel_do",
          "aclsp_b200_node_barrier_kernel_do", "aclsp_b200_transpose_build_kernel_do",
-         "aclsp_b200_transpose_values_kernel_do", "aclsparseSetMatType", "aclsparseSetMatIndexBase",
+         "aclsp_b200_transpose_values_kernel_do", "aclsp_b200_grouped_preprocess_kernel_do",
+         "aclsp_b200_grouped_mm_kernel_do", "aclsp_b200_quantize_rows_kernel_do", "aclsparseSetMatType", "aclsparseSetMatIndexBase",
          "aclsparseSetMatDiagType", "aclsparseSetMatFillMode"}
+
+_U64 = {"aclsp_b200_kernel_launches", "aclsp_b200_grouped_buffer_bytes"}
 
 _lib = None
 
@@ -217,6 +241,6 @@ def lib() -> ctypes.CDLL:
         for name, args in SIGNATURES.items():
             fn = getattr(handle, name)
             fn.argtypes = args
-            fn.restype = None if name in _VOID else (ctypes.c_uint64 if name == "aclsp_b200_kernel_launches" else c_int)
+            fn.restype = None if name in _VOID else (ctypes.c_uint64 if name in _U64 else c_int)
         _lib = handle
     return _lib

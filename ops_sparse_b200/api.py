@@ -157,11 +157,22 @@ class DnVec:
 
 
 class DnMat:
-    def __init__(self, rows: int, cols: int, ld: int, values, order: int = L.ORDER_ROW):
+    """Dense matrix descriptor; ``batch_count`` matrices, ``batch_stride`` elements apart, for the operators that
+    take one matrix per group."""
+
+    def __init__(self, rows: int, cols: int, ld: int, values, order: int = L.ORDER_ROW, batch_count: int = 1,
+                 batch_stride: int = 0):
         self.rows, self.cols, self.ld, self.values, self.order = rows, cols, ld, values, order
         self._d = c_void_p(None)
         check("aclsparseCreateDnMat", L.lib().aclsparseCreateDnMat(byref(self._d), rows, cols, ld, _ptr(values),
                                                                   acl_type(values), order))
+        self.batch_count, self.batch_stride = 1, 0
+        if batch_count != 1 or batch_stride != 0:
+            self.set_strided_batch(batch_count, batch_stride)
+
+    def set_strided_batch(self, count: int, stride: int) -> None:
+        check("aclsparseDnMatSetStridedBatch", L.lib().aclsparseDnMatSetStridedBatch(self._d, count, stride))
+        self.batch_count, self.batch_stride = count, stride
 
     @property
     def raw(self) -> c_void_p:
@@ -288,6 +299,99 @@ class SpMM:
         check("aclsparseSpMM", L.lib().aclsparseSpMM(
             self.handle.raw, self.op_a, self.op_b, pa, self.mat.raw, self.b.raw, pb, self.c.raw, self.compute_type,
             self.alg, _ptr(self.buffer)))
+
+
+def _device_array(name: str, t, dtype, count: int):
+    """A contiguous CUDA tensor of ``count`` elements that a C function takes as a plain array; None passes."""
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor on a CUDA device")
+    if t.numel() != count:
+        raise ValueError(f"{name} must have {count} elements, but has {t.numel()}")
+
+
+class _Grouped:
+    """The three phases of a grouped product; the subclasses supply the C functions' names and operands."""
+
+    name = ""
+
+    def _args(self, pa, pb):
+        raise NotImplementedError
+
+    def _call(self, phase: str, alpha, beta, last) -> None:
+        pa, pb, _keep = _scalars(alpha, beta)
+        check(self.name + phase, getattr(L.lib(), self.name + phase)(*self._args(pa, pb), last))
+
+    def buffer_size(self, alpha=1.0, beta=0.0) -> int:
+        size = c_size_t(0)
+        self._call("GetBufferSize", alpha, beta, byref(size))
+        return int(size.value)
+
+    def allocate(self, alpha=1.0, beta=0.0):
+        n = self.buffer_size(alpha, beta)
+        self.buffer = torch.empty(max(n, 64), dtype=torch.uint8, device=self.c.values.device)
+        return self.buffer
+
+    def preprocess(self, alpha=1.0, beta=0.0) -> None:
+        if self.buffer is None:
+            self.allocate(alpha, beta)
+        self._call("Preprocess", alpha, beta, _ptr(self.buffer))
+
+    def __call__(self, alpha=1.0, beta=0.0) -> None:
+        if self.buffer is None:
+            self.allocate(alpha, beta)
+        self._call("", alpha, beta, _ptr(self.buffer))
+
+
+class GroupedMM(_Grouped):
+    """C[r] = alpha * row_scales[r] * (A[r] @ op(B_g)) * col_scales[g] + beta * C[r] for the rows r of group g.
+
+    ``b`` holds one matrix per group (``DnMat(..., batch_count=groups, batch_stride=...)``); ``offsets`` is an int32
+    CUDA tensor of groups + 1 row numbers, or None with a single group.  The scales are optional fp32 CUDA tensors of
+    ``rows`` and ``groups x n`` elements.
+    """
+
+    name = "aclsparseB200GroupedMM"
+
+    def __init__(self, handle: Handle, a: DnMat, b: DnMat, c: DnMat, offsets=None, op_b: int = L.OP_N,
+                 row_scales=None, col_scales=None):
+        _device_array("offsets", offsets, torch.int32, b.batch_count + 1)
+        _device_array("row_scales", row_scales, torch.float32, c.rows)
+        _device_array("col_scales", col_scales, torch.float32, b.batch_count * c.cols)
+        self.handle, self.a, self.b, self.c, self.op_b = handle, a, b, c, op_b
+        self.offsets, self.row_scales, self.col_scales = offsets, row_scales, col_scales
+        self.buffer = None
+
+    def _args(self, pa, pb):
+        return (self.handle.raw, self.op_b, pa, self.a.raw, _ptr(self.offsets), self.b.raw, _ptr(self.row_scales),
+                _ptr(self.col_scales), pb, self.c.raw, L.ACL_FLOAT)
+
+
+class GroupedMMWeightGrad(_Grouped):
+    """C_g = alpha * A_g^T @ B_g + beta * C_g, A_g and B_g being the rows of group g; ``c`` holds one matrix per group."""
+
+    name = "aclsparseB200GroupedMMWeightGrad"
+
+    def __init__(self, handle: Handle, a: DnMat, b: DnMat, c: DnMat, offsets=None):
+        _device_array("offsets", offsets, torch.int32, c.batch_count + 1)
+        self.handle, self.a, self.b, self.c, self.offsets = handle, a, b, c, offsets
+        self.buffer = None
+
+    def _args(self, pa, pb):
+        return (self.handle.raw, pa, self.a.raw, self.b.raw, _ptr(self.offsets), pb, self.c.raw, L.ACL_FLOAT)
+
+
+class QuantizeRows:
+    """scales[r] = max|X[r]| / 127 and Q[r] = X[r] / scales[r] in int8, rounded to the nearest integer, ties to even."""
+
+    def __init__(self, handle: Handle, x: DnMat, q: DnMat, scales):
+        _device_array("scales", scales, torch.float32, x.rows)
+        self.handle, self.x, self.q, self.scales = handle, x, q, scales
+
+    def __call__(self) -> None:
+        check("aclsparseB200QuantizeRows", L.lib().aclsparseB200QuantizeRows(self.handle.raw, self.x.raw, self.q.raw,
+                                                                             _ptr(self.scales)))
 
 
 def kernel_launches() -> int:

@@ -1,0 +1,148 @@
+/*
+ * How a kernel finds its tile of a grouped product.  The sizes of the groups are
+ * known on the device only, so the tiles are numbered there: group after group,
+ * a group of `size` rows being cut into ceil(size / tileRows) pieces of nearly
+ * equal length (a multiple of 16 rows, so that no piece pays for a much larger
+ * neighbour), each piece with `across` tiles along the other dimension.
+ *
+ * A warp walks the groups 32 at a time: each lane loads two offsets, a running
+ * maximum makes them ascending whatever the array holds (every row is in one
+ * group at most, so the number of tiles stays bounded), a prefix sum numbers the
+ * tiles.  Tiles are asked for in ascending order, so the walk only goes forward.
+ */
+#ifndef ACLSPARSE_B200_GROUP_WALK_CUH_
+#define ACLSPARSE_B200_GROUP_WALK_CUH_
+
+#include <cstdint>
+
+namespace aclsp {
+
+// One tile: `count` rows from row `row0` on, of group `group`; `across` is its place along the other dimension.
+struct GroupTile {
+    uint32_t group;
+    uint32_t row0;
+    uint32_t count;
+    uint32_t across;
+};
+
+class GroupWalk {
+public:
+    __device__ __forceinline__ GroupWalk(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t tileRows,
+                                         uint32_t across)
+        : offsets_(offsets), groups_(groups), rows_(rows), tileRows_(tileRows), across_(across)
+    {
+        Load();
+    }
+
+    // Tile `t`; false when there are fewer.  Called by a whole warp, with ascending t.
+    __device__ __forceinline__ bool Find(uint32_t t, GroupTile* tile)
+    {
+        while (t >= end_) {
+            if (base_ + 32u >= groups_) {
+                return false;
+            }
+            base_ += 32u;
+            Load();
+        }
+        // the lane whose tiles include t: the first one whose inclusive prefix is beyond it
+        const uint32_t ballot = __ballot_sync(0xFFFFFFFFu, t < inclusive_);
+        const int lane = __ffs(static_cast<int>(ballot)) - 1;
+        const uint32_t begin = __shfl_sync(0xFFFFFFFFu, begin_, lane);
+        const uint32_t size = __shfl_sync(0xFFFFFFFFu, size_, lane);
+        const uint32_t pieces = (size + tileRows_ - 1u) / tileRows_;
+        const uint32_t local = t - (__shfl_sync(0xFFFFFFFFu, inclusive_, lane) - pieces * across_);
+        const uint32_t piece = local % pieces;
+        const uint32_t length = ((size + pieces - 1u) / pieces + 15u) / 16u * 16u;
+        const uint32_t from = piece * length < size ? piece * length : size;
+        tile->group = base_ + static_cast<uint32_t>(lane);
+        tile->across = local / pieces;
+        tile->row0 = begin + from;
+        tile->count = size - from < length ? size - from : length;
+        return true;
+    }
+
+    // Number of tiles in all groups; walks to the end.
+    __device__ __forceinline__ uint32_t Count()
+    {
+        while (base_ + 32u < groups_) {
+            base_ += 32u;
+            Load();
+        }
+        return end_;
+    }
+
+private:
+    __device__ __forceinline__ uint32_t Clamp(int32_t v) const
+    {
+        return v < 0 ? 0u : (static_cast<uint32_t>(v) > rows_ ? rows_ : static_cast<uint32_t>(v));
+    }
+
+    __device__ __forceinline__ void Load()
+    {
+        const uint32_t lane = threadIdx.x % 32u;
+        const uint32_t g = base_ + lane;
+        uint32_t first = 0;
+        uint32_t last = 0;
+        if (offsets_ == nullptr) {
+            last = g == 0 ? rows_ : 0u;
+        } else if (g < groups_) {
+            first = Clamp(__ldg(offsets_ + g));
+            last = Clamp(__ldg(offsets_ + g + 1));
+        }
+        // ascending ends: the largest offset up to and including this group's end
+        uint32_t top = first > last ? first : last;
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, top, d);
+            top = static_cast<int>(lane) >= d && up > top ? up : top;
+        }
+        uint32_t before = __shfl_up_sync(0xFFFFFFFFu, top, 1);
+        before = lane == 0 ? 0u : before;
+        before = before > reached_ ? before : reached_;
+        begin_ = first > before ? first : before;
+        const uint32_t until = last > begin_ ? last : begin_;
+        size_ = g < groups_ ? until - begin_ : 0u;
+        uint32_t sum = (size_ + tileRows_ - 1u) / tileRows_ * across_;
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+            sum += static_cast<int>(lane) >= d ? up : 0u;
+        }
+        inclusive_ = sum + end_;
+        end_ = __shfl_sync(0xFFFFFFFFu, inclusive_, 31);
+        const uint32_t chunkTop = __shfl_sync(0xFFFFFFFFu, top, 31);
+        reached_ = chunkTop > reached_ ? chunkTop : reached_;
+    }
+
+    const int32_t* offsets_;
+    uint32_t groups_;
+    uint32_t rows_;
+    uint32_t tileRows_;
+    uint32_t across_;
+    uint32_t base_ = 0;       // first group of the 32 that the lanes hold
+    uint32_t end_ = 0;        // tiles of all groups up to the last of them
+    uint32_t reached_ = 0;    // largest offset before them
+    uint32_t begin_ = 0;      // this lane's group: first row, rows, tiles up to its end
+    uint32_t size_ = 0;
+    uint32_t inclusive_ = 0;
+};
+
+// Rows of group g for a kernel that looks at one group only: clamped, never negative in number.
+__device__ __forceinline__ void GroupRows(const int32_t* offsets, uint32_t g, uint32_t rows, uint32_t* first,
+                                          uint32_t* last)
+{
+    if (offsets == nullptr) {
+        *first = 0;
+        *last = rows;
+        return;
+    }
+    const int64_t a = __ldg(offsets + g);
+    const int64_t b = __ldg(offsets + g + 1);
+    const int64_t top = rows;
+    const int64_t lo = a < 0 ? 0 : (a > top ? top : a);
+    const int64_t hi = b < lo ? lo : (b > top ? top : b);
+    *first = static_cast<uint32_t>(lo);
+    *last = static_cast<uint32_t>(hi);
+}
+
+}  // namespace aclsp
+
+#endif  // ACLSPARSE_B200_GROUP_WALK_CUH_

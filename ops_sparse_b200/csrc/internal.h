@@ -144,6 +144,15 @@ struct aclsparseDnVecDescr {
     AclspBarrierLink barrier = {};
 };
 
+// The last Preprocess of a grouped product into a matrix: its buffer's counters are clear for products on this
+// stream while the serial is still the last one published for the buffer.
+struct GroupedPlanRecord {
+    const void* buffer = nullptr;
+    const void* stream = nullptr;
+    uint64_t streamEpoch = 0;
+    uint64_t serial = 0;
+};
+
 struct aclsparseDnMatDescr {
     uint32_t signature = 0;
     int64_t rows = 0;
@@ -160,6 +169,7 @@ struct aclsparseDnMatDescr {
     void* mirrors[7] = {};
     // aclsparseB200DnMatSetClosingBarrier: the node barrier that ends a product into this matrix.
     AclspBarrierLink barrier = {};
+    GroupedPlanRecord grouped;
 };
 
 uint64_t AclspNextWorkspaceOwnerId();

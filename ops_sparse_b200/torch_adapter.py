@@ -10,12 +10,21 @@ arrays directly.  Same entry names and argument meaning here:
     spmv_csr(row_ptr, col_ind, values, x, y, alpha, beta, base=0, trans="N", cols=None)   in place on y
     spmv_workspace(...)                                   bytes aclsparseSpMVGetBufferSize asks for
 
+The products between the sparse steps of a mixture-of-experts layer have no counterpart in the reference:
+
+    grouped_mm(x, weight, offsets)                        y[r] = x[r] @ weight[g].T for the rows r of group g, with gradients
+    int8_mm(x, weight, x_scales, w_scales, offsets)       the same on int8 with one scale per row and per output column
+    quantize_rows(x)                                      int8 rows and their scales
+
 Argument errors are raised as ``ValueError`` / ``TypeError`` before anything is launched, in the order the reference
 checks them; the product itself runs through the C API on the current CUDA stream.  Like the reference's adapter,
 every call builds its descriptors and preprocesses (the plan build is tens of microseconds on the device and needs
 no host round trip).  ``install()`` additionally registers ``mv`` as the ``aten::mv`` kernel of CSR CUDA tensors.
 """
 from __future__ import annotations
+
+import contextlib
+import threading
 
 import torch
 
@@ -189,6 +198,177 @@ def spmv_workspace(row_ptr, col_ind, values, x, y, alpha: float = 1.0, beta: flo
         return _spmv_op(row_ptr, col_ind, values, x, y, base, trans, cols, sizes).buffer_size(alpha, beta)
 
 
+_local = threading.local()
+
+
+@contextlib.contextmanager
+def _stream_handle():
+    """This thread's kept handle on the current stream.
+
+    Destroying a handle waits for its stream, which a capture forbids and a training step should not pay for; between
+    calls the kept one is on no stream, so that nothing waits for a stream that is gone.
+    """
+    from . import api
+    handle = getattr(_local, "handle", None)
+    if handle is None:
+        handle = _local.handle = api.Handle(set_stream=False)
+    handle.set_stream(torch.cuda.current_stream().cuda_stream)
+    try:
+        yield handle
+    finally:
+        L.lib().aclsparseSetStream(handle.raw, None)
+
+
+def _dense_operand(name: str, t, dim: int, dtypes) -> None:
+    if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.device.type != "cuda":
+        raise ValueError(f"{name} must be a dense CUDA tensor")
+    if t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions, but has {t.dim()}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}, but is {t.dtype}")
+
+
+def _check_grouped(x, weight, offsets, dtypes, names=("x", "weight")) -> None:
+    _dense_operand(names[0], x, 2, dtypes)
+    _dense_operand(names[1], weight, 3, dtypes)
+    if weight.dtype != x.dtype:
+        raise TypeError(f"{names[0]} and {names[1]} must have the same dtype, but got {x.dtype} and {weight.dtype}")
+    if x.size(1) != weight.size(2):
+        raise ValueError(f"size mismatch: {names[0]} is {tuple(x.shape)}, {names[1]} is {tuple(weight.shape)}")
+    if weight.size(0) < 1 or weight.size(0) > 65535:
+        raise ValueError(f"between 1 and 65535 groups are supported, but got {weight.size(0)}")
+    _check_offsets(offsets, weight.size(0), x.device)
+    if weight.device != x.device:
+        raise ValueError(f"{names[0]} and {names[1]} must be on the same device")
+
+
+def _check_offsets(offsets, groups: int, device) -> None:
+    if offsets is None:
+        if groups != 1:
+            raise ValueError(f"offsets are needed with {groups} groups")
+        return
+    if not isinstance(offsets, torch.Tensor) or offsets.device != device or offsets.dtype != torch.int32:
+        raise TypeError("offsets must be an int32 tensor on the device of the operands")
+    if offsets.dim() != 1 or offsets.numel() != groups + 1:
+        raise ValueError(f"offsets must hold {groups + 1} row numbers, but has shape {tuple(offsets.shape)}")
+
+
+def _rows_descr(t: torch.Tensor):
+    """Row-major descriptor of a 2-D tensor; a copy is made where a row is not contiguous or rows overlap."""
+    from . import api
+    if t.size(1) > 1 and t.stride(1) != 1 or t.size(0) > 1 and t.stride(0) < t.size(1):
+        t = t.contiguous()
+    return api.DnMat(t.size(0), t.size(1), t.stride(0) if t.size(0) > 1 else t.size(1), t)
+
+
+def _batch_descr(w: torch.Tensor):
+    """Descriptor of a 3-D tensor, one matrix per group, rows or columns contiguous; else a copy is described."""
+    from . import api
+    groups, rows, cols = w.shape
+
+    def fits(outer, outer_stride, inner, inner_stride):
+        return ((inner_stride == 1 or inner == 1) and (outer == 1 or outer_stride >= inner) and
+                (groups == 1 or w.stride(0) >= (outer - 1) * outer_stride + inner))
+
+    if rows and cols and fits(cols, w.stride(2), rows, w.stride(1)) and not fits(rows, w.stride(1), cols, w.stride(2)):
+        order, ld = L.ORDER_COL, w.stride(2) if cols > 1 else rows
+    else:
+        if not fits(rows, w.stride(1), cols, w.stride(2)):
+            w = w.contiguous()
+        order, ld = L.ORDER_ROW, w.stride(1) if rows > 1 else cols
+    return api.DnMat(rows, cols, ld, w, order, groups, w.stride(0) if groups > 1 else 0)
+
+
+def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=None):
+    """x[r] @ op(weight[g]); rows in no group are zero."""
+    from . import api
+    n = weight.size(1) if op_b == L.OP_T else weight.size(2)
+    with torch.cuda.device(x.device):
+        y = torch.zeros(x.size(0), n, dtype=out_dtype, device=x.device)
+        if y.numel():
+            with _stream_handle() as handle:
+                api.GroupedMM(handle, _rows_descr(x), _batch_descr(weight), _rows_descr(y),
+                              None if offsets is None else offsets.contiguous(), op_b, row_scales, col_scales)()
+    return y
+
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, out_dtype):
+        ctx.save_for_backward(x, weight, offsets)
+        return _forward(x, weight, offsets, out_dtype, L.OP_T)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        from . import api
+        x, weight, offsets = ctx.saved_tensors
+        dy = dy.to(x.dtype)
+        dx = _forward(dy, weight, offsets, x.dtype, L.OP_N) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            with torch.cuda.device(x.device):
+                dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+                if dw.numel():
+                    with _stream_handle() as handle:
+                        api.GroupedMMWeightGrad(handle, _rows_descr(dy), _rows_descr(x), _batch_descr(dw),
+                                                None if offsets is None else offsets.contiguous())()
+        return dx, dw, None, None
+
+
+def grouped_mm(x: torch.Tensor, weight: torch.Tensor, offsets: "torch.Tensor | None" = None, *,
+               out_dtype: "torch.dtype | None" = None) -> torch.Tensor:
+    """``x[r] @ weight[g].T`` for the rows ``offsets[g] <= r < offsets[g + 1]`` of every group g.
+
+    x: rows x k, weight: groups x n x k, fp16 or bf16; offsets: groups + 1 ascending int32 values on the same device
+    (None with one group).  The result has ``out_dtype``: that type (default) or float32; rows in no group are zero.
+    Differentiable in x and weight; offsets carry no gradient.
+    """
+    _check_grouped(x, weight, offsets, (torch.float16, torch.bfloat16))
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, but got {out_dtype}")
+    return _GroupedMM.apply(x, weight, offsets, out_dtype)
+
+
+def int8_mm(x: torch.Tensor, weight: torch.Tensor, x_scales: torch.Tensor, w_scales: torch.Tensor,
+            offsets: "torch.Tensor | None" = None, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x_scales[r] * w_scales[g] * (x[r] @ weight[g].T)`` on int8 operands, exact inside the sum; no gradients.
+
+    x: rows x k and weight: groups x n x k (or n x k: one group), int8; x_scales: rows and w_scales: groups x n (or
+    n) float32 values.  The result is bfloat16, float16 or float32; rows in no group are zero.
+    """
+    if isinstance(weight, torch.Tensor) and weight.dim() == 2:
+        weight = weight.unsqueeze(0)
+    _check_grouped(x, weight, offsets, (torch.int8,))
+    if x.size(1) > 131071:
+        raise ValueError("sums of more than 131071 int8 products do not fit int32")
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"out_dtype must be a 16-bit floating type or torch.float32, but got {out_dtype}")
+    for name, t, count in (("x_scales", x_scales, x.size(0)), ("w_scales", w_scales, weight.size(0) * weight.size(1))):
+        if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32:
+            raise TypeError(f"{name} must be a float32 tensor on the device of the operands")
+        if t.numel() != count:
+            raise ValueError(f"{name} must have {count} elements, but has {t.numel()}")
+    return _forward(x.detach(), weight.detach(), offsets, out_dtype, L.OP_T, x_scales.detach().contiguous(),
+                    w_scales.detach().contiguous())
+
+
+def quantize_rows(x: torch.Tensor) -> "tuple[torch.Tensor, torch.Tensor]":
+    """int8 rows ``q`` and float32 ``scales`` with ``x[r]`` close to ``scales[r] * q[r]``: scales[r] = max|x[r]| / 127.
+
+    Rows are rounded to the nearest integer, ties to even; a row with an infinity or a NaN gets zeros and that scale.
+    """
+    _dense_operand("x", x, 2, (torch.float32, torch.float16, torch.bfloat16))
+    from . import api
+    with torch.cuda.device(x.device):
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scales = torch.empty(x.size(0), dtype=torch.float32, device=x.device)
+        with _stream_handle() as handle:
+            api.QuantizeRows(handle, _rows_descr(x.detach()), _rows_descr(q), scales)()
+    return q, scales
+
+
 _installed = []
 
 
@@ -201,4 +381,4 @@ def install() -> None:
     _installed.append(lib)  # the registration lives as long as the Library object
 
 
-__all__ = ["mv", "mm", "addmm", "spmv_csr", "spmv_workspace", "install"]
+__all__ = ["mv", "mm", "addmm", "spmv_csr", "spmv_workspace", "grouped_mm", "int8_mm", "quantize_rows", "install"]
