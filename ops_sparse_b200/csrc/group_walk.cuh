@@ -51,11 +51,16 @@ public:
         const uint32_t size = __shfl_sync(0xFFFFFFFFu, size_, lane);
         const uint32_t pieces = (size + tileRows_ - 1u) / tileRows_;
         const uint32_t local = t - (__shfl_sync(0xFFFFFFFFu, inclusive_, lane) - pieces * across_);
-        const uint32_t piece = local % pieces;
+        // Bands of eight pieces, all tiles across for each: the tiles that run at one time share their operands
+        // (a wave of 148 tiles reads about 8 + 19 different ones), also in a group far larger than the L2 cache.
+        const uint32_t band = local / (kBand * across_);
+        const uint32_t inBand = local - band * kBand * across_;
+        const uint32_t width = pieces - band * kBand < kBand ? pieces - band * kBand : kBand;
+        const uint32_t piece = band * kBand + inBand % width;
         const uint32_t length = ((size + pieces - 1u) / pieces + 15u) / 16u * 16u;
         const uint32_t from = piece * length < size ? piece * length : size;
         tile->group = base_ + static_cast<uint32_t>(lane);
-        tile->across = local / pieces;
+        tile->across = inBand / width;
         tile->row0 = begin + from;
         tile->count = size - from < length ? size - from : length;
         return true;
@@ -71,7 +76,20 @@ public:
         return end_;
     }
 
+    // Back to the first group; tiles may be asked for from the beginning again.
+    __device__ __forceinline__ void Restart()
+    {
+        if (base_ != 0u) {
+            base_ = 0;
+            end_ = 0;
+            reached_ = 0;
+            Load();
+        }
+    }
+
 private:
+    static constexpr uint32_t kBand = 8;
+
     __device__ __forceinline__ uint32_t Clamp(int32_t v) const
     {
         return v < 0 ? 0u : (static_cast<uint32_t>(v) > rows_ ? rows_ : static_cast<uint32_t>(v));

@@ -13,6 +13,8 @@
 #include "aclsparse_b200_kernels.h"
 #include "element_types.cuh"
 #include "group_walk.cuh"
+#include "grouped_schedule.cuh"
+#include "grouped_tc.h"
 #include "plan_kernels.h"
 
 namespace {
@@ -23,7 +25,8 @@ using aclsp::kBF16;
 using aclsp::kF16;
 using aclsp::kI8;
 
-constexpr uint32_t kHeaderBytes = 64;
+// The part of the buffer that Preprocess clears, and where partial sums begin.
+constexpr uint32_t kCountersEnd = 4u * (kGroupedHeaderWords + aclsp::kGroupedCounters);
 
 template <int kIn>
 struct Plain {
@@ -155,22 +158,24 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
 
 extern "C" uint64_t aclsp_b200_grouped_buffer_bytes(const AclspGroupedParams* params)
 {
-    (void)params;
-    return kHeaderBytes;
+    // two partial tiles per CTA at most
+    return kCountersEnd + 2ull * aclsp::kGroupedMaxCtas * aclsp::kTileLanes * AclspGroupedColumns(*params) * 4u;
 }
 
 extern "C" void aclsp_b200_grouped_preprocess_kernel_do(void* buffer, void* stream)
 {
     AclspCountLaunches(1);
-    cudaMemsetAsync(buffer, 0, kHeaderBytes, static_cast<cudaStream_t>(stream));
+    cudaMemsetAsync(buffer, 0, kCountersEnd, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" void aclsp_b200_grouped_mm_kernel_do(const void* a, const void* b, void* c, void* buffer,
                                                 const AclspGroupedParams* params, void* stream)
 {
-    (void)buffer;
     const AclspGroupedParams& p = *params;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (AclspGroupedTensorLaunch(a, b, c, buffer, p, s)) {
+        return;
+    }
     AclspCountLaunches(1);
     const uint32_t grid = 148u * 4u;
     if (p.inType == ACLSP_TYPE_F16) {

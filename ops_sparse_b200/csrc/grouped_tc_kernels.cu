@@ -1,0 +1,640 @@
+/*
+ * Grouped matrix products on the tensor cores (tcgen05), fed by TMA.
+ *
+ * A tile of the result is 128 lanes x up to kColumns columns of fp32 (int32) sums
+ * in tensor memory.  The DENSE matrix lies along the lanes and the ragged rows
+ * along the columns: N of tcgen05.mma is any multiple of 16, so a group of 5 rows
+ * costs an MMA of 16 columns and not one of 128 rows, and the same kernel serves a
+ * decoding batch (all time goes into reading weights) and a training batch.  For
+ * the weight gradient both operands are read with their summed index, the rows,
+ * along the outer dimension (MN-major), and the last rows of a group, which share
+ * a block with the next group's, are cut off in shared memory.
+ *
+ * One CTA per SM, persistent: warp 0 loads blocks of 128 bytes of the summed index
+ * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 7 read
+ * the finished sums and write results while the next tile computes in the other
+ * half of tensor memory.  Tiles that do not fill a wave are split along the summed
+ * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and the one
+ * that arrives last adds them in the CTAs' order, so that the result does not
+ * depend on who that is.
+ *
+ * Every wait is bounded.  One that runs out makes the CTA leave: the loads in
+ * flight are waited for (bounded again), tensor memory is freed, and the buffer's
+ * first word counts it.
+ */
+#include <cstdint>
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "aclsparse_b200_kernels.h"
+#include "element_types.cuh"
+#include "grouped_schedule.cuh"
+#include "grouped_tc.h"
+#include "plan_kernels.h"
+#include "tcgen05.cuh"
+
+namespace {
+
+using namespace aclsp;
+
+constexpr int kThreads = 256;
+constexpr uint32_t kLeftBytes = kTileLanes * 128u;
+constexpr uint32_t kGradientColumns = 256;
+
+template <uint32_t kColumns>
+struct Ring {
+    static constexpr uint32_t kStageBytes = kLeftBytes + kColumns * 128u;
+    static constexpr uint32_t kStages = 200u * 1024u / kStageBytes;
+    static constexpr uint32_t kBytes = kStageBytes * kStages + 1024u;  // stages start on multiples of 1024
+    static constexpr uint32_t kBox = kColumns < 64u ? kColumns : 64u;  // rows of one load of the right operand
+};
+
+// One result in the type of C; beta == 0 does not read C.
+template <typename T>
+__device__ __forceinline__ float ToFloat(T v);
+template <>
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+template <>
+__device__ __forceinline__ float ToFloat(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float ToFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T FromFloat(float v);
+template <>
+__device__ __forceinline__ float FromFloat(float v) { return v; }
+template <>
+__device__ __forceinline__ __half FromFloat(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 FromFloat(float v) { return __float2bfloat16_rn(v); }
+
+// Sixteen neighbouring results of one lane.
+struct Lane16 {
+    float v[16];
+};
+
+// Forward: the lane is a column of C, the sixteen values belong to sixteen rows.  A warp writes 32 neighbouring
+// columns of a row at a time.
+template <typename T>
+__device__ __forceinline__ void StoreForward(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t column,
+                                             uint32_t j0, const Lane16& sums, float laneScale, float beta)
+{
+    if (column >= p.n) {
+        return;
+    }
+    T* at = static_cast<T*>(c) + static_cast<int64_t>(s.row0 + j0) * p.ldc + column;
+    const uint32_t count = s.columns - j0 < 16u ? s.columns - j0 : 16u;
+    T old[16];
+    if (beta != 0.0f) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            old[j] = j < count ? at[static_cast<int64_t>(j) * p.ldc] : FromFloat<T>(0.0f);
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+        if (j < count) {
+            float r = sums.v[j] * laneScale;
+            if (p.rowScales != nullptr) {
+                r *= __ldg(p.rowScales + s.row0 + j0 + j);
+            }
+            if (beta != 0.0f) {
+                r = fmaf(beta, ToFloat(old[j]), r);
+            }
+            at[static_cast<int64_t>(j) * p.ldc] = FromFloat<T>(r);
+        }
+    }
+}
+
+// Gradient: the lane is a row of C_g, the sixteen values are neighbours in it.
+template <typename T>
+__device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
+                                              uint32_t j0, const Lane16& sums, float laneScale, float beta)
+{
+    if (row >= p.m) {
+        return;
+    }
+    T* at = static_cast<T*>(c) + static_cast<int64_t>(s.group) * p.cBatchStride + static_cast<int64_t>(row) * p.ldc +
+            s.right + j0;
+    const uint32_t count = s.columns - j0 < 16u ? s.columns - j0 : 16u;
+    alignas(16) T out[16];
+    if (beta != 0.0f) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            const float old = j < count ? ToFloat(at[j]) : 0.0f;
+            out[j] = FromFloat<T>(fmaf(beta, old, sums.v[j] * laneScale));
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            out[j] = FromFloat<T>(sums.v[j] * laneScale);
+        }
+    }
+    if (count == 16u && reinterpret_cast<uintptr_t>(at) % 16u == 0u) {
+        const uint4* from = reinterpret_cast<const uint4*>(out);
+        uint4* to = reinterpret_cast<uint4*>(at);
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(out) / 16u; ++i) {
+            to[i] = from[i];
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            if (j < count) {
+                at[j] = out[j];
+            }
+        }
+    }
+}
+
+template <bool kGradient>
+__device__ __forceinline__ void StoreResults(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t lane,
+                                             uint32_t j0, const Lane16& sums, float laneScale, float beta)
+{
+    if constexpr (kGradient) {
+        if (p.outType == ACLSP_TYPE_F32) {
+            StoreGradient<float>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        } else if (p.outType == ACLSP_TYPE_F16) {
+            StoreGradient<__half>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        } else {
+            StoreGradient<__nv_bfloat16>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        }
+    } else {
+        if (p.outType == ACLSP_TYPE_F32) {
+            StoreForward<float>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        } else if (p.outType == ACLSP_TYPE_F16) {
+            StoreForward<__half>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        } else {
+            StoreForward<__nv_bfloat16>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+        }
+    }
+}
+
+template <bool kInt8>
+__device__ __forceinline__ float SumToFloat(uint32_t bits)
+{
+    return kInt8 ? __int2float_rn(static_cast<int32_t>(bits)) : __uint_as_float(bits);
+}
+
+template <bool kInt8>
+__device__ __forceinline__ uint32_t AddSums(uint32_t a, uint32_t b)
+{
+    return kInt8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+
+template <bool kGradient>
+struct ScheduleOf {
+    using Type = ForwardSchedule;
+};
+template <>
+struct ScheduleOf<true> {
+    using Type = GradientSchedule;
+};
+
+template <bool kInt8, uint32_t kColumns, bool kGradient>
+__global__ void __launch_bounds__(kThreads, 1)
+    GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
+                        void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
+                        const uint32_t leftMn, const uint32_t joinBlocks)
+{
+    using R = Ring<kColumns>;
+    constexpr uint32_t kBlock = kInt8 ? 128u : 64u;  // elements of the summed index in a block
+    extern __shared__ unsigned char dynamic[];
+    __shared__ uint64_t full[R::kStages];
+    __shared__ uint64_t empty[R::kStages];
+    __shared__ uint64_t sumsFull[2];
+    __shared__ uint64_t sumsEmpty[2];
+    __shared__ uint64_t joined;   // the four result warps meet here
+    __shared__ uint64_t drained;
+    __shared__ uint32_t tmemAddress;
+    __shared__ uint32_t gaveUp;
+    __shared__ uint32_t isLast;
+
+    const uint32_t warp = threadIdx.x / 32u;
+    const uint32_t lane = threadIdx.x % 32u;
+    const uint32_t ring = (SmemAddress(dynamic) + 1023u) & ~1023u;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < R::kStages; ++i) {
+            BarInit(SmemAddress(full + i), 1);
+            BarInit(SmemAddress(empty + i), 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            BarInit(SmemAddress(sumsFull + i), 1);
+            BarInit(SmemAddress(sumsEmpty + i), 4);
+        }
+        BarInit(SmemAddress(&joined), 4);
+        BarInit(SmemAddress(&drained), 1);
+        gaveUp = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        FenceProxyAsync();
+        TmaPrefetch(&leftMap);
+        TmaPrefetch(&rightMap);
+    }
+    if (warp == 2) {
+        TmemAlloc(SmemAddress(&tmemAddress), 2u * kColumns);
+        TmemFenceBefore();
+    }
+    __syncthreads();
+    TmemFenceAfter();
+    const uint32_t tmem = tmemAddress;
+    volatile uint32_t* const stop = &gaveUp;
+
+    auto makeSchedule = [&]() {
+        if constexpr (kGradient) {
+            return GradientSchedule(p, kColumns, kBlock);
+        } else {
+            return ForwardSchedule(p, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
+        }
+    };
+
+    if (warp == 0) {
+        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
+        Segment s;
+        uint32_t stage = 0;
+        uint32_t parity = 0;
+        uint32_t loads = 0;
+        bool good = true;
+        while (good && schedule.Next(&s)) {
+            const uint32_t boxes = kGradient ? (s.columns + kBlock - 1u) / kBlock : (s.columns + R::kBox - 1u) / R::kBox;
+            const uint32_t leftBoxes = !kGradient && leftMn == 0u          ? 1u
+                                       : kInt8                              ? 1u
+                                       : (kGradient ? p.m : p.n) - s.left > 64u ? 2u
+                                                                            : 1u;
+            const uint32_t leftBoxBytes = kGradient || (leftMn != 0u && !kInt8) ? 8192u : kLeftBytes;
+            const uint32_t bytes = leftBoxes * leftBoxBytes + boxes * (kGradient ? 8192u : R::kBox * 128u);
+            if (lane == 0) {
+                for (uint32_t b = s.block0; b < s.block1; ++b) {
+                    if (!BarWait(SmemAddress(empty + stage), parity ^ 1u, stop)) {
+                        good = false;
+                        break;
+                    }
+                    const uint32_t bar = SmemAddress(full + stage);
+                    const uint32_t left = ring + stage * R::kStageBytes;
+                    const uint32_t right = left + kLeftBytes;
+                    BarExpect(bar, bytes);
+                    const int32_t at = static_cast<int32_t>(b * kBlock);
+                    if constexpr (kGradient) {
+                        const int32_t row = static_cast<int32_t>(s.row0) + at;
+                        for (uint32_t i = 0; i < leftBoxes; ++i) {
+                            TmaLoad2(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(s.left + i * 64u), row);
+                        }
+                        for (uint32_t i = 0; i < boxes; ++i) {
+                            TmaLoad2(right + i * 8192u, &rightMap, bar, static_cast<int32_t>(s.right + i * 64u), row);
+                        }
+                    } else {
+                        if (leftMn == 0u) {
+                            TmaLoad3(left, &leftMap, bar, at, static_cast<int32_t>(s.left), static_cast<int32_t>(s.group));
+                        } else {
+                            for (uint32_t i = 0; i < leftBoxes; ++i) {
+                                TmaLoad3(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(s.left + i * 64u), at,
+                                         static_cast<int32_t>(s.group));
+                            }
+                        }
+                        for (uint32_t i = 0; i < boxes; ++i) {
+                            TmaLoad2(right + i * R::kBox * 128u, &rightMap, bar, at,
+                                     static_cast<int32_t>(s.row0 + i * R::kBox));
+                        }
+                    }
+                    ++loads;
+                    stage = stage + 1u == R::kStages ? 0u : stage + 1u;
+                    parity ^= stage == 0u ? 1u : 0u;
+                }
+            }
+            good = __shfl_sync(0xFFFFFFFFu, good ? 1 : 0, 0) != 0;
+        }
+        // A CTA that gives up must not end under its copies: the last load of each stage has landed when the stage's
+        // barrier has passed the phase that the load belongs to.
+        if (lane == 0 && !good) {
+            const uint32_t last = loads < R::kStages ? loads : R::kStages;
+            uint32_t never = 0;
+            for (uint32_t i = 0; i < last; ++i) {
+                stage = stage == 0u ? R::kStages - 1u : stage - 1u;
+                parity ^= stage == R::kStages - 1u ? 1u : 0u;
+                (void)BarWait(SmemAddress(full + stage), parity, &never);
+            }
+        }
+    } else if (warp == 1) {
+        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
+        const bool leftT = kGradient || leftMn != 0u;
+        const uint32_t shape = MmaShape(kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
+        // 32 bytes of the summed index per instruction: inside a 128-byte row, or as many rows as it has elements
+        constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;
+        const uint32_t leftStep = (leftT ? kStepElements * 128u : 32u) >> 4;
+        const uint32_t rightStep = (kGradient ? kStepElements * 128u : 32u) >> 4;
+        Segment s;
+        uint32_t stage = 0;
+        uint32_t parity = 0;
+        uint32_t tile = 0;
+        bool good = true;
+        while (good && schedule.Next(&s)) {
+            const uint32_t half = tile & 1u;
+            good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop)) != 0;
+            if (!good) {
+                break;
+            }
+            ++tile;
+            TmemFenceAfter();
+            const uint32_t d = tmem + half * kColumns;
+            const uint32_t instruction = shape | MmaColumns((s.columns + 15u) / 16u * 16u);
+            const uint32_t length = kGradient ? s.rows : p.k;
+            for (uint32_t b = s.block0; b < s.block1; ++b) {
+                good = BarWait(SmemAddress(full + stage), parity, stop);
+                good = __all_sync(0xFFFFFFFFu, good) != 0;
+                if (!good) {
+                    break;
+                }
+                TmemFenceAfter();
+                const uint32_t left = ring + stage * R::kStageBytes;
+                const uint32_t right = left + kLeftBytes;
+                const uint32_t valid = length - b * kBlock < kBlock ? length - b * kBlock : kBlock;
+                const uint32_t steps = (valid + kStepElements - 1u) / kStepElements;
+                if constexpr (kGradient) {
+                    // Rows behind the group's last one, up to the end of the last step, are somebody else's: zeros, in
+                    // both operands, so that no infinity or NaN of theirs gets in.
+                    const uint32_t cut = steps * kStepElements - valid;
+                    if (cut != 0u) {
+                        const uint32_t vectors = cut * 8u;
+                        constexpr uint32_t kSmemBlocks = 2u + kColumns / 64u;
+                        for (uint32_t i = lane; i < vectors * kSmemBlocks; i += 32u) {
+                            const uint32_t address = left + i / vectors * 8192u + valid * 128u + i % vectors * 16u;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(address), "r"(0) : "memory");
+                        }
+                        FenceProxyAsync();
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0) {
+                    const uint64_t a = OperandDescriptor(left, 8192u);
+                    const uint64_t w = OperandDescriptor(right, 8192u);
+                    for (uint32_t i = 0; i < steps; ++i) {
+                        Mma<kInt8>(d, a + i * leftStep, w + i * rightStep, instruction, b != s.block0 || i != 0u ? 1u : 0u);
+                    }
+                    MmaCommit(SmemAddress(empty + stage));
+                }
+                stage = stage + 1u == R::kStages ? 0u : stage + 1u;
+                parity ^= stage == 0u ? 1u : 0u;
+            }
+            if (good && lane == 0) {
+                MmaCommit(SmemAddress(sumsFull + half));
+            }
+            __syncwarp();
+        }
+        if (!good && lane == 0) {  // not under instructions that still read tensor memory
+            uint32_t never = 0;
+            MmaCommit(SmemAddress(&drained));
+            (void)BarWait(SmemAddress(&drained), 0, &never);
+        }
+    } else if (warp >= 4) {
+        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
+        const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
+        const float beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
+        const uint32_t row = threadIdx.x - 128u;  // lane of tensor memory
+        uint32_t* const counters = buffer + kGroupedHeaderWords;
+        uint32_t* const partials = counters + kGroupedCounters;
+        constexpr uint32_t kSlotWords = kTileLanes * kColumns;
+        Segment s;
+        uint32_t tile = 0;
+        uint32_t meetings = 0;
+        // The four warps meet; bounded like every wait.
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) {
+                BarArrive(SmemAddress(&joined));
+            }
+            return __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(&joined), meetings++ & 1u, stop)) != 0;
+        };
+        while (schedule.Next(&s)) {
+            const uint32_t half = tile & 1u;
+            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsFull + half), tile >> 1 & 1u, stop))) {
+                break;
+            }
+            ++tile;
+            TmemFenceAfter();
+            const uint32_t from = tmem + half * kColumns + (warp % 4u * 32u << 16);
+            const bool empty0 = s.block0 == s.block1;  // an empty group's gradient: nothing was summed
+            float laneScale = alpha;
+            if (!kGradient && p.colScales != nullptr && s.left + row < p.n) {
+                laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + s.left + row);
+            }
+            if (s.parts == 1u) {
+                for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+                    uint32_t bits[16];
+                    Lane16 sums;
+                    __syncwarp();
+                    TmemLoad16(from + j0, bits);
+                    TmemLoadWait();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) {
+                        sums.v[j] = empty0 ? 0.0f : SumToFloat<kInt8>(bits[j]);
+                    }
+                    StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta);
+                }
+                TmemFenceBefore();
+                __syncwarp();
+                if (lane == 0) {
+                    BarArrive(SmemAddress(sumsEmpty + half));
+                }
+                continue;
+            }
+            uint32_t* const mine = partials + static_cast<size_t>(s.slot) * kSlotWords + row;
+            for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+                uint32_t bits[16];
+                TmemLoad16(from + j0, bits);
+                TmemLoadWait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    __stcg(mine + (j0 + j) * kTileLanes, bits[j]);
+                }
+            }
+            TmemFenceBefore();
+            __syncwarp();
+            if (lane == 0) {
+                BarArrive(SmemAddress(sumsEmpty + half));
+            }
+            __threadfence();
+            if (!meet()) {
+                break;
+            }
+            if (row == 0) {
+                const uint32_t before = atomicAdd(counters + s.counter, 1u);
+                isLast = before + 1u == s.parts ? 1u : 0u;
+                if (before + 1u == s.parts) {
+                    counters[s.counter] = 0;  // clear for the next product
+                }
+                __threadfence();
+            }
+            if (!meet()) {
+                break;
+            }
+            if (isLast == 0u) {
+                continue;
+            }
+            __threadfence();
+            for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+                uint32_t total[16];
+                const uint32_t* first = partials + static_cast<size_t>(s.firstSlot) * kSlotWords + j0 * kTileLanes + row;
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    total[j] = __ldcg(first + j * kTileLanes);
+                }
+#pragma unroll 2
+                for (uint32_t part = 1; part < s.parts; ++part) {
+                    const uint32_t* next = partials + static_cast<size_t>(2u * (s.firstCta + part)) * kSlotWords +
+                                           j0 * kTileLanes + row;
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) {
+                        total[j] = AddSums<kInt8>(total[j], __ldcg(next + j * kTileLanes));
+                    }
+                }
+                Lane16 sums;
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    sums.v[j] = SumToFloat<kInt8>(total[j]);
+                }
+                StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta);
+            }
+        }
+    }
+
+    __syncthreads();
+    if (threadIdx.x == 0 && gaveUp != 0u) {
+        atomicAdd(buffer, 1u);
+    }
+    if (warp == 2) {
+        TmemFenceAfter();
+        TmemFree(tmem, 2u * kColumns);
+    }
+}
+
+// ---- host side ----
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn Encoder()
+{
+    static const EncodeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+// A map of `rank` dimensions (innermost first) whose boxes are 128 bytes wide and `boxRows` rows high.
+bool Encode(CUtensorMap* map, const AclspGroupedParams& p, const void* base, uint32_t rank, const uint64_t* sizes,
+            const uint64_t* strideElements, uint32_t boxRows)
+{
+    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    cuuint64_t dims[3];
+    cuuint64_t strides[2];
+    cuuint32_t box[3] = {static_cast<cuuint32_t>(128u / bytes), boxRows, 1};
+    cuuint32_t ones[3] = {1, 1, 1};
+    for (uint32_t i = 0; i < rank; ++i) {
+        dims[i] = sizes[i];
+        if (i > 0) {
+            strides[i - 1] = strideElements[i - 1] * bytes;
+        }
+    }
+    const CUtensorMapDataType type = p.inType == ACLSP_TYPE_I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : p.inType == ACLSP_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return Encoder()(map, type, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a tensor map asks of a matrix: 16-byte aligned, strides of multiples of 16 bytes below 2^40.
+bool Mappable(const void* base, int64_t ld, int64_t batchStride, uint64_t bytes)
+{
+    const uint64_t pitch = static_cast<uint64_t>(ld) * bytes;
+    const uint64_t batch = static_cast<uint64_t>(batchStride) * bytes;
+    return reinterpret_cast<uintptr_t>(base) % 16u == 0u && pitch % 16u == 0u && batch % 16u == 0u && pitch < 1ull << 40 &&
+           batch < 1ull << 40;
+}
+
+template <bool kInt8, uint32_t kColumns, bool kGradient>
+void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* buffer, const AclspGroupedParams& p,
+            uint32_t leftMn, uint32_t grid, cudaStream_t s)
+{
+    auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<kColumns>::kBytes));
+    AclspCountLaunches(1);
+    kernel<<<grid, kThreads, Ring<kColumns>::kBytes, s>>>(left, right, c, static_cast<uint32_t*>(buffer), p, leftMn,
+                                                          kJoinBlocks);
+}
+
+}  // namespace
+
+uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
+{
+    if (p.weightGrad != 0) {
+        return kGradientColumns;
+    }
+    // Rows per group on average: what the host knows.  Larger groups are cut into more pieces, which read the
+    // weights again (from L2); smaller ones only leave part of the stages unused.
+    const uint64_t average = p.rows / p.groups;
+    return average <= 24u ? 32u : average <= 96u ? 128u : 256u;
+}
+
+bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
+                              cudaStream_t s)
+{
+    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    CUtensorMap left;
+    CUtensorMap right;
+    constexpr uint32_t kLongest = 1u << 28;  // block numbers stay far inside 32 bits
+    if (p.rows > kLongest || p.k > kLongest || (p.weightGrad == 0 && p.k == 0) || p.rows == 0 || Encoder() == nullptr) {
+        return false;
+    }
+    uint32_t sms = AclspSmCount();
+    sms = sms == 0 || sms > kGroupedMaxCtas ? kGroupedMaxCtas : sms;
+    if (p.weightGrad != 0) {
+        const uint64_t tiles = static_cast<uint64_t>(p.groups) * ((p.m + kTileLanes - 1u) / kTileLanes) *
+                               ((p.n + kGradientColumns - 1u) / kGradientColumns);
+        if (!Mappable(a, p.aInner, 0, bytes) || !Mappable(b, p.bInner, 0, bytes) || tiles > 1u << 30) {
+            return false;
+        }
+        const uint64_t leftSizes[2] = {p.m, p.rows};
+        const uint64_t rightSizes[2] = {p.n, p.rows};
+        const uint64_t leftStride[1] = {static_cast<uint64_t>(p.aInner)};
+        const uint64_t rightStride[1] = {static_cast<uint64_t>(p.bInner)};
+        if (!Encode(&left, p, a, 2, leftSizes, leftStride, 64) || !Encode(&right, p, b, 2, rightSizes, rightStride, 64)) {
+            return false;
+        }
+        Launch<false, kGradientColumns, true>(left, right, c, buffer, p, 1u, sms, s);
+        return true;
+    }
+    const uint32_t leftMn = p.bInner == 1 ? 0u : 1u;
+    const int64_t ld = leftMn != 0 ? p.bInner : p.bOuter;
+    const int64_t batch = p.groups > 1 ? p.bBatchStride : ld;
+    const uint32_t columns = AclspGroupedColumns(p);
+    const uint64_t tiles = (static_cast<uint64_t>(p.rows) / columns + p.groups) * ((p.n + kTileLanes - 1u) / kTileLanes);
+    if (!Mappable(a, p.aOuter, 0, bytes) || !Mappable(b, ld, batch, bytes) || tiles > 1u << 30) {
+        return false;
+    }
+    const uint64_t leftSizes[3] = {leftMn != 0 ? p.n : p.k, leftMn != 0 ? p.k : p.n, p.groups};
+    const uint64_t leftStrides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(batch)};
+    const uint64_t rightSizes[2] = {p.k, p.rows};
+    const uint64_t rightStride[1] = {static_cast<uint64_t>(p.aOuter)};
+    const uint32_t leftBox = leftMn != 0 ? static_cast<uint32_t>(128u / bytes) : kTileLanes;
+    if (!Encode(&left, p, b, 3, leftSizes, leftStrides, leftBox) ||
+        !Encode(&right, p, a, 2, rightSizes, rightStride, columns < 64u ? columns : 64u)) {
+        return false;
+    }
+    const bool int8 = p.inType == ACLSP_TYPE_I8;
+    auto run = int8 ? (columns == 32u    ? Launch<true, 32, false>
+                       : columns == 128u ? Launch<true, 128, false>
+                                         : Launch<true, 256, false>)
+                    : (columns == 32u    ? Launch<false, 32, false>
+                       : columns == 128u ? Launch<false, 128, false>
+                                         : Launch<false, 256, false>);
+    run(left, right, c, buffer, p, leftMn, sms, s);
+    return true;
+}
