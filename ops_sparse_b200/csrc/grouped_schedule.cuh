@@ -1,10 +1,11 @@
 /*
- * Which part of which tile a CTA of the tensor-core kernel works on, in order.
- * Every warp of a CTA asks for itself and gets the same answers.
+ * Which part of which tile a worker - a CTA, or a pair of them - of the tensor-core
+ * kernel works on, in order.  Every warp of it asks for itself and gets the same
+ * answers.
  *
- * A tile is 128 x kTileColumns results; its summed index is cut into blocks of
- * 128 bytes.  Forward products run whole tiles in waves of one per CTA, and what
- * is left after the last full wave is split along the summed index over all CTAs
+ * A tile is (128 per CTA) x tileColumns results; its summed index is cut into blocks of
+ * 128 bytes.  Forward products run whole tiles in waves of one per worker, and what
+ * is left after the last full wave is split along the summed index over all of them
  * where that saves more time than joining the partial sums costs.  Weight
  * gradients, whose tiles differ in length with their groups, run whole tiles
  * round robin when there are many and are split into equal runs of blocks when
@@ -20,10 +21,10 @@
 
 namespace aclsp {
 
-constexpr uint32_t kTileLanes = 128;      // results along the first operand: lanes of tensor memory
+constexpr uint32_t kTileLanes = 128;      // results along the first operand per CTA: lanes of tensor memory
 constexpr uint32_t kGroupedMaxCtas = 148;
-constexpr uint32_t kMinSplitBlocks = 4;   // shortest run of blocks worth a CTA of its own
-constexpr uint32_t kWholeTileWaves = 4;   // gradient: with this many tiles per CTA nothing is split
+constexpr uint32_t kMinSplitBlocks = 4;   // shortest run of blocks worth a worker of its own
+constexpr uint32_t kWholeTileWaves = 4;   // gradient: with this many tiles per worker nothing is split
 constexpr uint32_t kGroupedCounters = kWholeTileWaves * kGroupedMaxCtas;
 
 struct Segment {
@@ -35,38 +36,45 @@ struct Segment {
     uint32_t columns;   // results along the other dimension
     uint32_t block0;    // blocks [block0, block1) of the summed index
     uint32_t block1;
-    uint32_t parts;     // CTAs that share the tile; 1: the result is complete here
+    uint32_t parts;     // workers that share the tile; 1: the result is complete here
     uint32_t counter;   // parts > 1: the tile's counter,
-    uint32_t firstCta;  // its first CTA, whose partial sums are in slot firstSlot; CTA c's after it in slot 2 * c
+    uint32_t firstWorker;  // its first worker, whose partial sums are in slot firstSlot; worker w's after it in slot 2 * w
     uint32_t firstSlot;
-    uint32_t slot;      // this CTA's slot
+    uint32_t slot;      // this worker's slot
 };
 
-// The CTAs that share units [start, start + length) of runs of `per` units each.
-__device__ __forceinline__ void SetParts(Segment* s, uint32_t start, uint32_t length, uint32_t per, uint32_t counter)
+struct Workers {
+    uint32_t index;
+    uint32_t count;
+};
+
+// The workers that share units [start, start + length) of runs of `per` units each.
+__device__ __forceinline__ void SetParts(Segment* s, const Workers& w, uint32_t start, uint32_t length, uint32_t per,
+                                         uint32_t counter)
 {
-    s->firstCta = start / per;
-    s->parts = (start + length - 1u) / per - s->firstCta + 1u;
-    // a CTA's run holds two partial tiles at most: one that it continues (slot 0) and one that it begins (slot 1)
-    s->firstSlot = 2u * s->firstCta + (s->firstCta * per < start ? 1u : 0u);
-    s->slot = blockIdx.x == s->firstCta ? s->firstSlot : 2u * blockIdx.x;
+    s->firstWorker = start / per;
+    s->parts = (start + length - 1u) / per - s->firstWorker + 1u;
+    // a worker's run holds two partial tiles at most: one that it continues (slot 0) and one that it begins (slot 1)
+    s->firstSlot = 2u * s->firstWorker + (s->firstWorker * per < start ? 1u : 0u);
+    s->slot = w.index == s->firstWorker ? s->firstSlot : 2u * w.index;
     s->counter = counter;
 }
 
 class ForwardSchedule {
 public:
-    __device__ __forceinline__ ForwardSchedule(const AclspGroupedParams& p, uint32_t tileRows, uint32_t blocks,
-                                               uint32_t joinBlocks)
-        : walk_(p.offsets, p.groups, p.rows, tileRows, (p.n + kTileLanes - 1u) / kTileLanes), blocks_(blocks)
+    __device__ __forceinline__ ForwardSchedule(const AclspGroupedParams& p, Workers workers, uint32_t tileLanes,
+                                               uint32_t tileRows, uint32_t blocks, uint32_t joinBlocks)
+        : walk_(p.offsets, p.groups, p.rows, tileRows, (p.n + tileLanes - 1u) / tileLanes), workers_(workers),
+          tileLanes_(tileLanes), blocks_(blocks)
     {
         const uint32_t tiles = walk_.Count();
         walk_.Restart();
-        waves_ = tiles / gridDim.x;
-        const uint32_t units = (tiles - waves_ * gridDim.x) * blocks;
-        per_ = (units + gridDim.x - 1u) / gridDim.x;
+        waves_ = tiles / workers_.count;
+        const uint32_t units = (tiles - waves_ * workers_.count) * blocks;
+        per_ = (units + workers_.count - 1u) / workers_.count;
         per_ = per_ > kMinSplitBlocks ? per_ : kMinSplitBlocks;
         per_ = per_ + joinBlocks < blocks ? per_ : blocks;
-        unit_ = blockIdx.x * per_ < units ? blockIdx.x * per_ : units;
+        unit_ = workers_.index * per_ < units ? workers_.index * per_ : units;
         unitEnd_ = unit_ + per_ < units ? unit_ + per_ : units;
     }
 
@@ -77,7 +85,7 @@ public:
         s->block1 = blocks_;
         s->parts = 1;
         if (wave_ < waves_) {
-            t = wave_ * gridDim.x + blockIdx.x;
+            t = wave_ * workers_.count + workers_.index;
             ++wave_;
         } else {
             if (unit_ >= unitEnd_) {
@@ -85,12 +93,12 @@ public:
             }
             const uint32_t local = unit_ / blocks_;
             const uint32_t start = local * blocks_;
-            t = waves_ * gridDim.x + local;
+            t = waves_ * workers_.count + local;
             s->block0 = unit_ - start;
             const uint32_t until = s->block0 + (unitEnd_ - unit_);
             s->block1 = until < blocks_ ? until : blocks_;
             unit_ += s->block1 - s->block0;
-            SetParts(s, start, blocks_, per_, local);
+            SetParts(s, workers_, start, blocks_, per_, local);
         }
         GroupTile tile;
         if (!walk_.Find(t, &tile)) {
@@ -99,7 +107,7 @@ public:
         s->group = tile.group;
         s->row0 = tile.row0;
         s->rows = tile.count;
-        s->left = tile.across * kTileLanes;
+        s->left = tile.across * tileLanes_;
         s->right = 0;
         s->columns = tile.count;
         return true;
@@ -107,6 +115,8 @@ public:
 
 private:
     GroupWalk walk_;
+    Workers workers_;
+    uint32_t tileLanes_;
     uint32_t blocks_;
     uint32_t waves_;
     uint32_t wave_ = 0;
@@ -117,13 +127,14 @@ private:
 
 class GradientSchedule {
 public:
-    __device__ __forceinline__ GradientSchedule(const AclspGroupedParams& p, uint32_t tileColumns, uint32_t blockRows)
-        : offsets_(p.offsets), groups_(p.groups), rows_(p.rows), n_(p.n), tileColumns_(tileColumns), blockRows_(blockRows),
-          across_((p.n + tileColumns - 1u) / tileColumns), perGroup_(across_ * ((p.m + kTileLanes - 1u) / kTileLanes))
+    __device__ __forceinline__ GradientSchedule(const AclspGroupedParams& p, Workers workers, uint32_t tileLanes,
+                                                uint32_t tileColumns, uint32_t blockRows)
+        : workers_(workers), tileLanes_(tileLanes), offsets_(p.offsets), groups_(p.groups), rows_(p.rows), n_(p.n), tileColumns_(tileColumns), blockRows_(blockRows),
+          across_((p.n + tileColumns - 1u) / tileColumns), perGroup_(across_ * ((p.m + tileLanes - 1u) / tileLanes))
     {
         total_ = groups_ * perGroup_;
-        split_ = total_ < kWholeTileWaves * gridDim.x;
-        tile_ = blockIdx.x;
+        split_ = total_ < kWholeTileWaves * workers_.count;
+        tile_ = workers_.index;
         if (split_) {
             Load();
             while (base_ + 32u < groups_) {
@@ -131,9 +142,9 @@ public:
                 Load();
             }
             const uint32_t units = end_;
-            per_ = (units + gridDim.x - 1u) / gridDim.x;
+            per_ = (units + workers_.count - 1u) / workers_.count;
             per_ = per_ > kMinSplitBlocks ? per_ : kMinSplitBlocks;
-            unit_ = blockIdx.x * per_ < units ? blockIdx.x * per_ : units;
+            unit_ = workers_.index * per_ < units ? workers_.index * per_ : units;
             unitEnd_ = unit_ + per_ < units ? unit_ + per_ : units;
             if (base_ != 0u) {
                 base_ = 0;
@@ -153,7 +164,7 @@ public:
             }
             s->group = tile_ / perGroup_;
             inGroup = tile_ % perGroup_;
-            tile_ += gridDim.x;
+            tile_ += workers_.count;
             uint32_t last;
             GroupRows(offsets_, s->group, rows_, &s->row0, &last);
             s->rows = last - s->row0;
@@ -184,10 +195,10 @@ public:
             if (blocks == 0u) {
                 s->block1 = 0;  // an empty group: beta * C
             } else {
-                SetParts(s, start, units, per_, s->group * perGroup_ + inGroup);
+                SetParts(s, workers_, start, units, per_, s->group * perGroup_ + inGroup);
             }
         }
-        s->left = inGroup / across_ * kTileLanes;
+        s->left = inGroup / across_ * tileLanes_;
         s->right = inGroup % across_ * tileColumns_;
         s->columns = n_ - s->right < tileColumns_ ? n_ - s->right : tileColumns_;
         return true;
@@ -217,6 +228,8 @@ private:
         end_ = __shfl_sync(0xFFFFFFFFu, inclusive_, 31);
     }
 
+    Workers workers_;
+    uint32_t tileLanes_;
     const int32_t* offsets_;
     uint32_t groups_;
     uint32_t rows_;

@@ -10,6 +10,11 @@
  * along the outer dimension (MN-major), and the last rows of a group, which share
  * a block with the next group's, are cut off in shared memory.
  *
+ * Wide tiles (256 columns) are computed by a pair of CTAs on neighbouring SMs, 256 x 256 results: each holds 128 rows
+ * of the dense matrix and half of the ragged rows, and one MMA reads both.  A single CTA would have to load 48 KB for
+ * 512 cycles of MMA, more than the 52 bytes per cycle that an SM was measured to get from L2 with all of them
+ * loading; the pair loads 32 KB each.
+ *
  * One CTA per SM, persistent: warp 0 loads blocks of 128 bytes of the summed index
  * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 7 read
  * the finished sums and write results while the next tile computes in the other
@@ -42,9 +47,10 @@ constexpr int kThreads = 256;
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kGradientColumns = 256;
 
-template <uint32_t kColumns>
+template <uint32_t kColumns, uint32_t kCtas>
 struct Ring {
-    static constexpr uint32_t kStageBytes = kLeftBytes + kColumns * 128u;
+    static constexpr uint32_t kRightRows = kColumns / kCtas;  // of the right operand in one CTA
+    static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
     static constexpr uint32_t kStages = 200u * 1024u / kStageBytes;
     static constexpr uint32_t kBytes = kStageBytes * kStages + 1024u;  // stages start on multiples of 1024
     static constexpr uint32_t kBox = kColumns < 64u ? kColumns : 64u;  // rows of one load of the right operand
@@ -74,34 +80,54 @@ struct Lane16 {
 };
 
 // Forward: the lane is a column of C, the sixteen values belong to sixteen rows.  A warp writes 32 neighbouring
-// columns of a row at a time.
+// columns of a row at a time.  Called by whole warps.
 template <typename T>
 __device__ __forceinline__ void StoreForward(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t column,
                                              uint32_t j0, const Lane16& sums, float laneScale, float beta)
 {
+    const uint32_t count = s.columns - j0 < 16u ? s.columns - j0 : 16u;
+    float r[16];
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+        r[j] = sums.v[j] * laneScale;
+    }
+    if (p.rowScales != nullptr) {
+        // one load for the sixteen rows, handed round: a load per row would wait for each store before it
+        const uint32_t mine = threadIdx.x % 16u;
+        const float scale = mine < count ? __ldg(p.rowScales + s.row0 + j0 + mine) : 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            r[j] *= __shfl_sync(0xFFFFFFFFu, scale, static_cast<int>(j));
+        }
+    }
     if (column >= p.n) {
         return;
     }
     T* at = static_cast<T*>(c) + static_cast<int64_t>(s.row0 + j0) * p.ldc + column;
-    const uint32_t count = s.columns - j0 < 16u ? s.columns - j0 : 16u;
-    T old[16];
     if (beta != 0.0f) {
+        T old[16];
 #pragma unroll
         for (uint32_t j = 0; j < 16; ++j) {
             old[j] = j < count ? at[static_cast<int64_t>(j) * p.ldc] : FromFloat<T>(0.0f);
         }
-    }
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) {
-        if (j < count) {
-            float r = sums.v[j] * laneScale;
-            if (p.rowScales != nullptr) {
-                r *= __ldg(p.rowScales + s.row0 + j0 + j);
+        for (uint32_t j = 0; j < 16; ++j) {
+            r[j] = fmaf(beta, ToFloat(old[j]), r[j]);
+        }
+    }
+    if (count == 16u) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            *at = FromFloat<T>(r[j]);
+            at += p.ldc;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            if (j < count) {
+                *at = FromFloat<T>(r[j]);
             }
-            if (beta != 0.0f) {
-                r = fmaf(beta, ToFloat(old[j]), r);
-            }
-            at[static_cast<int64_t>(j) * p.ldc] = FromFloat<T>(r);
+            at += p.ldc;
         }
     }
 }
@@ -148,24 +174,24 @@ __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void*
 }
 
 template <bool kGradient>
-__device__ __forceinline__ void StoreResults(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t lane,
+__device__ __forceinline__ void StoreResults(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
                                              uint32_t j0, const Lane16& sums, float laneScale, float beta)
 {
     if constexpr (kGradient) {
         if (p.outType == ACLSP_TYPE_F32) {
-            StoreGradient<float>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreGradient<float>(p, c, s, row, j0, sums, laneScale, beta);
         } else if (p.outType == ACLSP_TYPE_F16) {
-            StoreGradient<__half>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreGradient<__half>(p, c, s, row, j0, sums, laneScale, beta);
         } else {
-            StoreGradient<__nv_bfloat16>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreGradient<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta);
         }
     } else {
         if (p.outType == ACLSP_TYPE_F32) {
-            StoreForward<float>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreForward<float>(p, c, s, row, j0, sums, laneScale, beta);
         } else if (p.outType == ACLSP_TYPE_F16) {
-            StoreForward<__half>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreForward<__half>(p, c, s, row, j0, sums, laneScale, beta);
         } else {
-            StoreForward<__nv_bfloat16>(p, c, s, s.left + lane, j0, sums, laneScale, beta);
+            StoreForward<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta);
         }
     }
 }
@@ -191,36 +217,42 @@ struct ScheduleOf<true> {
     using Type = GradientSchedule;
 };
 
-template <bool kInt8, uint32_t kColumns, bool kGradient>
+template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
     GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
                         void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
                         const uint32_t leftMn, const uint32_t joinBlocks)
 {
-    using R = Ring<kColumns>;
-    constexpr uint32_t kBlock = kInt8 ? 128u : 64u;  // elements of the summed index in a block
+    using R = Ring<kColumns, kCtas>;
+    constexpr uint32_t kBlock = kInt8 ? 128u : 64u;         // elements of the summed index in a block
+    constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;   // and in one MMA
+    constexpr uint32_t kColumnStep = 16u * kCtas;           // N of the MMA is a multiple of this
     extern __shared__ unsigned char dynamic[];
     __shared__ uint64_t full[R::kStages];
     __shared__ uint64_t empty[R::kStages];
     __shared__ uint64_t sumsFull[2];
     __shared__ uint64_t sumsEmpty[2];
-    __shared__ uint64_t joined;   // the four result warps meet here
+    __shared__ uint64_t joined;     // the four result warps meet here
     __shared__ uint64_t drained;
+    __shared__ uint64_t tailReady[R::kStages];  // first CTA of a pair: the second one has cut a block's last rows off
     __shared__ uint32_t tmemAddress;
     __shared__ uint32_t gaveUp;
     __shared__ uint32_t isLast;
 
     const uint32_t warp = threadIdx.x / 32u;
     const uint32_t lane = threadIdx.x % 32u;
+    const uint32_t rank = kCtas == 2 ? blockIdx.x % 2u : 0u;  // in the pair; rank 0 issues the MMAs
+    const Workers workers{blockIdx.x / kCtas, gridDim.x / kCtas};
     const uint32_t ring = (SmemAddress(dynamic) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < R::kStages; ++i) {
             BarInit(SmemAddress(full + i), 1);
             BarInit(SmemAddress(empty + i), 1);
+            BarInit(SmemAddress(tailReady + i), 1);
         }
         for (uint32_t i = 0; i < 2; ++i) {
             BarInit(SmemAddress(sumsFull + i), 1);
-            BarInit(SmemAddress(sumsEmpty + i), 4);
+            BarInit(SmemAddress(sumsEmpty + i), 4u * kCtas);
         }
         BarInit(SmemAddress(&joined), 4);
         BarInit(SmemAddress(&drained), 1);
@@ -231,20 +263,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         TmaPrefetch(&rightMap);
     }
     if (warp == 2) {
-        TmemAlloc(SmemAddress(&tmemAddress), 2u * kColumns);
+        TmemAlloc<kCtas>(SmemAddress(&tmemAddress), 2u * kColumns);
         TmemFenceBefore();
     }
     __syncthreads();
+    if constexpr (kCtas == 2) {
+        ClusterSync();  // the other CTA's barriers are ready too
+    }
     TmemFenceAfter();
     const uint32_t tmem = tmemAddress;
     volatile uint32_t* const stop = &gaveUp;
 
     auto makeSchedule = [&]() {
         if constexpr (kGradient) {
-            return GradientSchedule(p, kColumns, kBlock);
+            return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock);
         } else {
-            return ForwardSchedule(p, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
+            return ForwardSchedule(p, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
         }
+    };
+    // Gradient: rows of block b that belong to the group.  The last block of a group may hold rows behind it; those of
+    // the last MMA's share are somebody else's and are overwritten with zeros, in both operands, so that no infinity or
+    // NaN of theirs gets in.
+    auto validRows = [&](const Segment& s, uint32_t b) {
+        return s.rows - b * kBlock < kBlock ? s.rows - b * kBlock : kBlock;
+    };
+    auto cutRows = [&](uint32_t valid, uint32_t left) {
+        const uint32_t vectors = (kStepElements - valid % kStepElements) % kStepElements * 8u;
+        constexpr uint32_t kSmemBlocks = 2u + R::kRightRows / 64u;
+        for (uint32_t i = lane; i < vectors * kSmemBlocks; i += 32u) {
+            const uint32_t address = left + i / vectors * 8192u + valid * 128u + i % vectors * 16u;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(address), "r"(0) : "memory");
+        }
+        FenceProxyAsync();
+        __syncwarp();
     };
 
     if (warp == 0) {
@@ -255,44 +306,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t loads = 0;
         bool good = true;
         while (good && schedule.Next(&s)) {
-            const uint32_t boxes = kGradient ? (s.columns + kBlock - 1u) / kBlock : (s.columns + R::kBox - 1u) / R::kBox;
-            const uint32_t leftBoxes = !kGradient && leftMn == 0u          ? 1u
-                                       : kInt8                              ? 1u
-                                       : (kGradient ? p.m : p.n) - s.left > 64u ? 2u
-                                                                            : 1u;
-            const uint32_t leftBoxBytes = kGradient || (leftMn != 0u && !kInt8) ? 8192u : kLeftBytes;
-            const uint32_t bytes = leftBoxes * leftBoxBytes + boxes * (kGradient ? 8192u : R::kBox * 128u);
+            const uint32_t share = (s.columns + kColumnStep - 1u) / kColumnStep * 16u;  // of the columns, in this CTA
+            const uint32_t boxes = (share + R::kBox - 1u) / R::kBox;
+            const uint32_t bytes = kLeftBytes + boxes * R::kBox * 128u;
+            const uint32_t leftAt = s.left + rank * kTileLanes;
+            const uint32_t rightAt = (kGradient ? s.right : s.row0) + rank * share;
             if (lane == 0) {
                 for (uint32_t b = s.block0; b < s.block1; ++b) {
                     if (!BarWait(SmemAddress(empty + stage), parity ^ 1u, stop)) {
                         good = false;
                         break;
                     }
-                    const uint32_t bar = SmemAddress(full + stage);
+                    // A pair's blocks are announced to the first CTA, except those whose last rows are cut off: the
+                    // second CTA has to see to its own share first.
+                    const uint32_t bar0 = SmemAddress(full + stage);
                     const uint32_t left = ring + stage * R::kStageBytes;
                     const uint32_t right = left + kLeftBytes;
-                    BarExpect(bar, bytes);
+                    const bool cut = kGradient && validRows(s, b) % kStepElements != 0u;
+                    const bool own = rank == 0u || cut;
+                    if (own) {
+                        BarExpect(bar0, kCtas == 2 && !cut ? 2u * bytes : bytes);
+                    }
+                    const uint32_t bar = own ? bar0 : PeerAddress(bar0, 0);
                     const int32_t at = static_cast<int32_t>(b * kBlock);
                     if constexpr (kGradient) {
                         const int32_t row = static_cast<int32_t>(s.row0) + at;
-                        for (uint32_t i = 0; i < leftBoxes; ++i) {
-                            TmaLoad2(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(s.left + i * 64u), row);
+                        for (uint32_t i = 0; i < 2; ++i) {
+                            TmaLoad2<kCtas>(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(leftAt + i * 64u), row);
                         }
                         for (uint32_t i = 0; i < boxes; ++i) {
-                            TmaLoad2(right + i * 8192u, &rightMap, bar, static_cast<int32_t>(s.right + i * 64u), row);
+                            TmaLoad2<kCtas>(right + i * 8192u, &rightMap, bar, static_cast<int32_t>(rightAt + i * 64u), row);
                         }
                     } else {
                         if (leftMn == 0u) {
-                            TmaLoad3(left, &leftMap, bar, at, static_cast<int32_t>(s.left), static_cast<int32_t>(s.group));
+                            TmaLoad3<kCtas>(left, &leftMap, bar, at, static_cast<int32_t>(leftAt), static_cast<int32_t>(s.group));
                         } else {
-                            for (uint32_t i = 0; i < leftBoxes; ++i) {
-                                TmaLoad3(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(s.left + i * 64u), at,
-                                         static_cast<int32_t>(s.group));
+                            for (uint32_t i = 0; i < (kInt8 ? 1u : 2u); ++i) {
+                                TmaLoad3<kCtas>(left + i * 8192u, &leftMap, bar, static_cast<int32_t>(leftAt + i * 64u), at,
+                                                static_cast<int32_t>(s.group));
                             }
                         }
                         for (uint32_t i = 0; i < boxes; ++i) {
-                            TmaLoad2(right + i * R::kBox * 128u, &rightMap, bar, at,
-                                     static_cast<int32_t>(s.row0 + i * R::kBox));
+                            TmaLoad2<kCtas>(right + i * R::kBox * 128u, &rightMap, bar, at,
+                                            static_cast<int32_t>(rightAt + i * R::kBox));
                         }
                     }
                     ++loads;
@@ -302,29 +358,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             good = __shfl_sync(0xFFFFFFFFu, good ? 1 : 0, 0) != 0;
         }
-        // A CTA that gives up must not end under its copies: the last load of each stage has landed when the stage's
-        // barrier has passed the phase that the load belongs to.
+        // A CTA that gives up must not end under its copies.  The first CTA's barriers know when they have landed; the
+        // second one of a pair, which has no barrier for them, gives them the limit of a wait.
         if (lane == 0 && !good) {
             const uint32_t last = loads < R::kStages ? loads : R::kStages;
             uint32_t never = 0;
             for (uint32_t i = 0; i < last; ++i) {
                 stage = stage == 0u ? R::kStages - 1u : stage - 1u;
                 parity ^= stage == R::kStages - 1u ? 1u : 0u;
-                (void)BarWait(SmemAddress(full + stage), parity, &never);
+                (void)BarWait(SmemAddress(full + stage), rank == 0u ? parity : 0u, &never);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0u) {
         typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         const bool leftT = kGradient || leftMn != 0u;
-        const uint32_t shape = MmaShape(kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
+        const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
         // 32 bytes of the summed index per instruction: inside a 128-byte row, or as many rows as it has elements
-        constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;
         const uint32_t leftStep = (leftT ? kStepElements * 128u : 32u) >> 4;
         const uint32_t rightStep = (kGradient ? kStepElements * 128u : 32u) >> 4;
         Segment s;
         uint32_t stage = 0;
         uint32_t parity = 0;
         uint32_t tile = 0;
+        uint32_t cuts = 0;  // a bit per stage: the parity of its next cut block
         bool good = true;
         while (good && schedule.Next(&s)) {
             const uint32_t half = tile & 1u;
@@ -335,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++tile;
             TmemFenceAfter();
             const uint32_t d = tmem + half * kColumns;
-            const uint32_t instruction = shape | MmaColumns((s.columns + 15u) / 16u * 16u);
+            const uint32_t instruction = shape | MmaColumns((s.columns + kColumnStep - 1u) / kColumnStep * kColumnStep);
             const uint32_t length = kGradient ? s.rows : p.k;
             for (uint32_t b = s.block0; b < s.block1; ++b) {
                 good = BarWait(SmemAddress(full + stage), parity, stop);
@@ -343,52 +399,73 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!good) {
                     break;
                 }
-                TmemFenceAfter();
                 const uint32_t left = ring + stage * R::kStageBytes;
                 const uint32_t right = left + kLeftBytes;
                 const uint32_t valid = length - b * kBlock < kBlock ? length - b * kBlock : kBlock;
                 const uint32_t steps = (valid + kStepElements - 1u) / kStepElements;
                 if constexpr (kGradient) {
-                    // Rows behind the group's last one, up to the end of the last step, are somebody else's: zeros, in
-                    // both operands, so that no infinity or NaN of theirs gets in.
-                    const uint32_t cut = steps * kStepElements - valid;
-                    if (cut != 0u) {
-                        const uint32_t vectors = cut * 8u;
-                        constexpr uint32_t kSmemBlocks = 2u + kColumns / 64u;
-                        for (uint32_t i = lane; i < vectors * kSmemBlocks; i += 32u) {
-                            const uint32_t address = left + i / vectors * 8192u + valid * 128u + i % vectors * 16u;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(address), "r"(0) : "memory");
+                    if (valid % kStepElements != 0u) {
+                        cutRows(valid, left);
+                        if constexpr (kCtas == 2) {
+                            good = __all_sync(0xFFFFFFFFu,
+                                              BarWait(SmemAddress(tailReady + stage), cuts >> stage & 1u, stop)) != 0;
+                            cuts ^= 1u << stage;
+                            if (!good) {
+                                break;
+                            }
                         }
-                        FenceProxyAsync();
-                        __syncwarp();
                     }
                 }
+                TmemFenceAfter();
                 if (lane == 0) {
                     const uint64_t a = OperandDescriptor(left, 8192u);
                     const uint64_t w = OperandDescriptor(right, 8192u);
                     for (uint32_t i = 0; i < steps; ++i) {
-                        Mma<kInt8>(d, a + i * leftStep, w + i * rightStep, instruction, b != s.block0 || i != 0u ? 1u : 0u);
+                        Mma<kInt8, kCtas>(d, a + i * leftStep, w + i * rightStep, instruction,
+                                          b != s.block0 || i != 0u ? 1u : 0u);
                     }
-                    MmaCommit(SmemAddress(empty + stage));
+                    MmaCommit<kCtas>(SmemAddress(empty + stage));
                 }
                 stage = stage + 1u == R::kStages ? 0u : stage + 1u;
                 parity ^= stage == 0u ? 1u : 0u;
             }
             if (good && lane == 0) {
-                MmaCommit(SmemAddress(sumsFull + half));
+                MmaCommit<kCtas>(SmemAddress(sumsFull + half));
             }
             __syncwarp();
         }
         if (!good && lane == 0) {  // not under instructions that still read tensor memory
             uint32_t never = 0;
-            MmaCommit(SmemAddress(&drained));
+            MmaCommit<kCtas>(SmemAddress(&drained));
             (void)BarWait(SmemAddress(&drained), 0, &never);
+        }
+    } else if (kGradient && kCtas == 2 && warp == 1) {
+        // second CTA of a pair: cuts the last rows of its share of a block off, then tells the first one
+        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
+        Segment s;
+        uint32_t block = 0;  // of all that this worker loads: the stage is block % kStages
+        uint32_t cuts = 0;
+        while (schedule.Next(&s)) {
+            const uint32_t count = s.block1 - s.block0;
+            const uint32_t valid = count != 0u ? validRows(s, s.block1 - 1u) : 0u;
+            if (valid % kStepElements != 0u) {
+                const uint32_t stage = (block + count - 1u) % R::kStages;
+                if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(full + stage), cuts >> stage & 1u, stop))) {
+                    break;
+                }
+                cuts ^= 1u << stage;
+                cutRows(valid, ring + stage * R::kStageBytes);
+                if (lane == 0) {
+                    BarArrivePeer(PeerAddress(SmemAddress(tailReady + stage), 0));
+                }
+            }
+            block += count;
         }
     } else if (warp >= 4) {
         typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
         const float beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
-        const uint32_t row = threadIdx.x - 128u;  // lane of tensor memory
+        const uint32_t tmemLane = threadIdx.x - 128u;
         uint32_t* const counters = buffer + kGroupedHeaderWords;
         uint32_t* const partials = counters + kGroupedCounters;
         constexpr uint32_t kSlotWords = kTileLanes * kColumns;
@@ -403,6 +480,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             return __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(&joined), meetings++ & 1u, stop)) != 0;
         };
+        // This warp has read its share of the sums: the tensor memory may be written again.
+        auto release = [&](uint32_t half) {
+            TmemFenceBefore();
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t bar = SmemAddress(sumsEmpty + half);
+                if (rank == 0u) {
+                    BarArrive(bar);
+                } else {
+                    BarArrivePeer(PeerAddress(bar, 0));
+                }
+            }
+        };
         while (schedule.Next(&s)) {
             const uint32_t half = tile & 1u;
             if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsFull + half), tile >> 1 & 1u, stop))) {
@@ -411,10 +501,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++tile;
             TmemFenceAfter();
             const uint32_t from = tmem + half * kColumns + (warp % 4u * 32u << 16);
-            const bool empty0 = s.block0 == s.block1;  // an empty group's gradient: nothing was summed
+            const uint32_t row = s.left + rank * kTileLanes + tmemLane;  // of the first operand
+            const bool nothing = s.block0 == s.block1;  // an empty group's gradient: no sums were made
             float laneScale = alpha;
-            if (!kGradient && p.colScales != nullptr && s.left + row < p.n) {
-                laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + s.left + row);
+            if (!kGradient && p.colScales != nullptr && row < p.n) {
+                laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + row);
             }
             if (s.parts == 1u) {
                 for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
@@ -425,18 +516,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     TmemLoadWait();
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) {
-                        sums.v[j] = empty0 ? 0.0f : SumToFloat<kInt8>(bits[j]);
+                        sums.v[j] = nothing ? 0.0f : SumToFloat<kInt8>(bits[j]);
                     }
                     StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta);
                 }
-                TmemFenceBefore();
-                __syncwarp();
-                if (lane == 0) {
-                    BarArrive(SmemAddress(sumsEmpty + half));
-                }
+                release(half);
                 continue;
             }
-            uint32_t* const mine = partials + static_cast<size_t>(s.slot) * kSlotWords + row;
+            uint32_t* const mine = partials + static_cast<size_t>(s.slot * kCtas + rank) * kSlotWords + tmemLane;
             for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
                 uint32_t bits[16];
                 TmemLoad16(from + j0, bits);
@@ -446,20 +533,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __stcg(mine + (j0 + j) * kTileLanes, bits[j]);
                 }
             }
-            TmemFenceBefore();
-            __syncwarp();
-            if (lane == 0) {
-                BarArrive(SmemAddress(sumsEmpty + half));
-            }
+            release(half);
             __threadfence();
             if (!meet()) {
                 break;
             }
-            if (row == 0) {
-                const uint32_t before = atomicAdd(counters + s.counter, 1u);
+            if (tmemLane == 0) {
+                uint32_t* const counter = counters + s.counter * kCtas + rank;
+                const uint32_t before = atomicAdd(counter, 1u);
                 isLast = before + 1u == s.parts ? 1u : 0u;
                 if (before + 1u == s.parts) {
-                    counters[s.counter] = 0;  // clear for the next product
+                    *counter = 0;  // clear for the next product
                 }
                 __threadfence();
             }
@@ -472,15 +556,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             __threadfence();
             for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
                 uint32_t total[16];
-                const uint32_t* first = partials + static_cast<size_t>(s.firstSlot) * kSlotWords + j0 * kTileLanes + row;
+                const uint32_t offset = j0 * kTileLanes + tmemLane;
+                const uint32_t* first = partials + static_cast<size_t>(s.firstSlot * kCtas + rank) * kSlotWords + offset;
 #pragma unroll
                 for (uint32_t j = 0; j < 16; ++j) {
                     total[j] = __ldcg(first + j * kTileLanes);
                 }
 #pragma unroll 2
                 for (uint32_t part = 1; part < s.parts; ++part) {
-                    const uint32_t* next = partials + static_cast<size_t>(2u * (s.firstCta + part)) * kSlotWords +
-                                           j0 * kTileLanes + row;
+                    const uint32_t slot = 2u * (s.firstWorker + part) * kCtas + rank;
+                    const uint32_t* next = partials + static_cast<size_t>(slot) * kSlotWords + offset;
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) {
                         total[j] = AddSums<kInt8>(total[j], __ldcg(next + j * kTileLanes));
@@ -500,9 +585,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && gaveUp != 0u) {
         atomicAdd(buffer, 1u);
     }
+    if constexpr (kCtas == 2) {
+        ClusterSync();  // neither CTA leaves while the other may still reach its shared memory
+    }
     if (warp == 2) {
         TmemFenceAfter();
-        TmemFree(tmem, 2u * kColumns);
+        TmemFree<kCtas>(tmem, 2u * kColumns);
     }
 }
 
@@ -561,13 +649,26 @@ bool Mappable(const void* base, int64_t ld, int64_t batchStride, uint64_t bytes)
 
 template <bool kInt8, uint32_t kColumns, bool kGradient>
 void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* buffer, const AclspGroupedParams& p,
-            uint32_t leftMn, uint32_t grid, cudaStream_t s)
+            uint32_t leftMn, uint32_t sms, cudaStream_t s)
 {
-    auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient>;
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<kColumns>::kBytes));
+    constexpr uint32_t kCtas = kColumns == 256u ? 2u : 1u;
+    constexpr uint32_t kBytes = Ring<kColumns, kCtas>::kBytes;
+    auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient, kCtas>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
     AclspCountLaunches(1);
-    kernel<<<grid, kThreads, Ring<kColumns>::kBytes, s>>>(left, right, c, static_cast<uint32_t*>(buffer), p, leftMn,
-                                                          kJoinBlocks);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(sms / kCtas * kCtas);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kBytes;
+    config.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = kCtas;
+    cluster.val.clusterDim.y = 1;
+    cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kJoinBlocks);
 }
 
 }  // namespace

@@ -27,6 +27,24 @@ __device__ __forceinline__ void BarArrive(uint32_t bar)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 
+// The address of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t PeerAddress(uint32_t address, uint32_t rank)
+{
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there) : "r"(address), "r"(rank));
+    return there;
+}
+
+__device__ __forceinline__ void BarArrivePeer(uint32_t peerBar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(peerBar) : "memory");
+}
+
+__device__ __forceinline__ void ClusterSync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
 __device__ __forceinline__ void BarExpect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
@@ -37,7 +55,7 @@ __device__ __forceinline__ bool BarTry(uint32_t bar, uint32_t parity)
     uint32_t done;
     asm volatile(
         "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -78,20 +96,34 @@ __device__ __forceinline__ void TmaPrefetch(const CUtensorMap* map)
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
+// A box of a matrix or of a batch of them into this CTA's shared memory.  With kCtas == 2 the barrier may be the
+// other CTA's of the pair.
+template <uint32_t kCtas>
 __device__ __forceinline__ void TmaLoad2(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y)
 {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y)
-        : "memory");
+    if constexpr (kCtas == 2) {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
+            "[%2];\n" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n" ::"r"(
+                dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    }
 }
 
+template <uint32_t kCtas>
 __device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y, int32_t z)
 {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
+    if constexpr (kCtas == 2) {
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, "
+            "%5}], [%2];\n" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n" ::"r"(
+                dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    }
 }
 
 // Writes of this thread to shared memory become visible to the asynchronous proxy (TMA, tcgen05.mma).
@@ -100,44 +132,66 @@ __device__ __forceinline__ void FenceProxyAsync()
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }
 
+// Tensor memory: of this CTA, or with kCtas == 2 of both CTAs of the pair, each of which calls.
+template <uint32_t kCtas>
 __device__ __forceinline__ void TmemAlloc(uint32_t smemResult, uint32_t columns)
 {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smemResult), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    if constexpr (kCtas == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smemResult), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smemResult), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
 }
 
+template <uint32_t kCtas>
 __device__ __forceinline__ void TmemFree(uint32_t address, uint32_t columns)
 {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(address), "r"(columns) : "memory");
+    if constexpr (kCtas == 2) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(address), "r"(columns) : "memory");
+    } else {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(address), "r"(columns) : "memory");
+    }
 }
 
 __device__ __forceinline__ void TmemFenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void TmemFenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 
-// `bar` gets one arrival when every tcgen05.mma that this thread has issued so far is done.
+// `bar` gets one arrival, in both CTAs of a pair, when every tcgen05.mma that this thread has issued so far is done.
+template <uint32_t kCtas>
 __device__ __forceinline__ void MmaCommit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
-}
-
-// D (128 lanes x N columns of tensor memory at d) = A * B, or += when accumulate.
-template <bool kInt8>
-__device__ __forceinline__ void Mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t accumulate)
-{
-    if constexpr (kInt8) {
-        asm volatile(
-            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-            "l"(a), "l"(b), "r"(shape), "r"(accumulate)
-            : "memory");
+    if constexpr (kCtas == 2) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+                     "h"(static_cast<uint16_t>(3))
+                     : "memory");
     } else {
-        asm volatile(
-            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-            "l"(a), "l"(b), "r"(shape), "r"(accumulate)
-            : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
     }
 }
+
+// D (128 lanes per CTA x N columns of tensor memory at d) = A * B, or += when accumulate.  In a pair each CTA holds its
+// own 128 rows of A and half of B's N columns, at the same shared-memory addresses.
+#define ACLSP_MMA(group, kind)                                                                              \
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"                                                \
+                 "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n}\n" ::"r"(d),      \
+                 "l"(a), "l"(b), "r"(shape), "r"(accumulate)                                                \
+                 : "memory")
+template <bool kInt8, uint32_t kCtas>
+__device__ __forceinline__ void Mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t accumulate)
+{
+    if constexpr (kInt8 && kCtas == 2) {
+        ACLSP_MMA("2", "i8");
+    } else if constexpr (kInt8) {
+        ACLSP_MMA("1", "i8");
+    } else if constexpr (kCtas == 2) {
+        ACLSP_MMA("2", "f16");
+    } else {
+        ACLSP_MMA("1", "f16");
+    }
+}
+#undef ACLSP_MMA
 
 // 16 columns of this warp's 32 lanes: thread i gets lane i's.
 __device__ __forceinline__ void TmemLoad16(uint32_t address, uint32_t (&r)[16])
@@ -160,13 +214,13 @@ __device__ __forceinline__ uint64_t OperandDescriptor(uint32_t smem, uint32_t bl
            static_cast<uint64_t>(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// Instruction descriptor without N: dense, 128 x N, sums fp32 (fp16 or bf16 operands) or int32 (int8 operands).
-__device__ __forceinline__ uint32_t MmaShape(bool int8, bool bf16, bool aTransposed, bool bTransposed)
+// Instruction descriptor without N: dense, (128 per CTA) x N, sums fp32 (fp16 or bf16 operands) or int32 (int8 operands).
+__device__ __forceinline__ uint32_t MmaShape(uint32_t ctas, bool int8, bool bf16, bool aTransposed, bool bTransposed)
 {
     const uint32_t sums = int8 ? 2u : 1u;
     const uint32_t operand = int8 || bf16 ? 1u : 0u;  // int8: 1 signed; fp16: 0, bf16: 1
     return sums << 4 | operand << 7 | operand << 10 | (aTransposed ? 1u : 0u) << 15 | (bTransposed ? 1u : 0u) << 16 |
-           (128u / 16u) << 24;
+           ctas * (128u / 16u) << 24;
 }
 __device__ __forceinline__ uint32_t MmaColumns(uint32_t n) { return n / 8u << 17; }
 
