@@ -51,7 +51,7 @@ template <uint32_t kColumns, uint32_t kCtas>
 struct Ring {
     static constexpr uint32_t kRightRows = kColumns / kCtas;  // of the right operand in one CTA
     static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
-    static constexpr uint32_t kStages = 200u * 1024u / kStageBytes;
+    static constexpr uint32_t kStages = 224u * 1024u / kStageBytes;
     static constexpr uint32_t kBytes = kStageBytes * kStages + 1024u;  // stages start on multiples of 1024
     static constexpr uint32_t kBox = kColumns < 64u ? kColumns : 64u;  // rows of one load of the right operand
 };
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t bytes = kLeftBytes + boxes * R::kBox * 128u;
             const uint32_t leftAt = s.left + rank * kTileLanes;
             const uint32_t rightAt = (kGradient ? s.right : s.row0) + rank * share;
-            if (lane == 0) {
+            if (ElectLane()) {
                 for (uint32_t b = s.block0; b < s.block1; ++b) {
                     if (!BarWait(SmemAddress(empty + stage), parity ^ 1u, stop)) {
                         good = false;
@@ -356,11 +356,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     parity ^= stage == 0u ? 1u : 0u;
                 }
             }
-            good = __shfl_sync(0xFFFFFFFFu, good ? 1 : 0, 0) != 0;
+            __syncwarp();
+            good = __all_sync(0xFFFFFFFFu, good) != 0;
         }
         // A CTA that gives up must not end under its copies.  The first CTA's barriers know when they have landed; the
         // second one of a pair, which has no barrier for them, gives them the limit of a wait.
-        if (lane == 0 && !good) {
+        if (loads != 0u && !good) {  // the lane that issued them
             const uint32_t last = loads < R::kStages ? loads : R::kStages;
             uint32_t never = 0;
             for (uint32_t i = 0; i < last; ++i) {
@@ -416,25 +417,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                TmemFenceAfter();
-                if (lane == 0) {
+                if (ElectLane()) {
                     const uint64_t a = OperandDescriptor(left, 8192u);
                     const uint64_t w = OperandDescriptor(right, 8192u);
-                    for (uint32_t i = 0; i < steps; ++i) {
-                        Mma<kInt8, kCtas>(d, a + i * leftStep, w + i * rightStep, instruction,
-                                          b != s.block0 || i != 0u ? 1u : 0u);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; ++i) {
+                        if (i < steps) {
+                            Mma<kInt8, kCtas>(d, a + i * leftStep, w + i * rightStep, instruction,
+                                              b != s.block0 || i != 0u ? 1u : 0u);
+                        }
                     }
                     MmaCommit<kCtas>(SmemAddress(empty + stage));
                 }
                 stage = stage + 1u == R::kStages ? 0u : stage + 1u;
                 parity ^= stage == 0u ? 1u : 0u;
             }
-            if (good && lane == 0) {
+            if (good && ElectLane()) {
                 MmaCommit<kCtas>(SmemAddress(sumsFull + half));
             }
             __syncwarp();
         }
-        if (!good && lane == 0) {  // not under instructions that still read tensor memory
+        if (!good && ElectLane()) {  // not under instructions that still read tensor memory
             uint32_t never = 0;
             MmaCommit<kCtas>(SmemAddress(&drained));
             (void)BarWait(SmemAddress(&drained), 0, &never);
