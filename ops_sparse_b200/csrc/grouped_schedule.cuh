@@ -1,7 +1,7 @@
 /*
  * Which part of which tile a worker - a CTA, or a pair of them - of the tensor-core
- * kernel works on, in order.  Every warp of it asks for itself and gets the same
- * answers.
+ * kernel works on, in order.  One warp of each CTA asks and tells the others
+ * through shared memory.
  *
  * A tile is (128 per CTA) x tileColumns results; its summed index is cut into blocks of
  * 128 bytes.  Forward products run whole tiles in waves of one per worker, and what

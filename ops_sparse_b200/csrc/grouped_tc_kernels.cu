@@ -16,9 +16,10 @@
  * loading; the pair loads 32 KB each.
  *
  * One CTA per SM, persistent: warp 0 loads blocks of 128 bytes of the summed index
- * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 7 read
+ * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 11 read
  * the finished sums and write results while the next tile computes in the other
- * half of tensor memory.  Tiles that do not fill a wave are split along the summed
+ * half of tensor memory.  Warp 3 works out the next tiles ahead of all of them: done by
+ * the MMA warp itself it left the tensor cores idle for 600 cycles per tile.  Tiles that do not fill a wave are split along the summed
  * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and the one
  * that arrives last adds them in the CTAs' order, so that the result does not
  * depend on who that is.
@@ -43,7 +44,9 @@ namespace {
 
 using namespace aclsp;
 
-constexpr int kThreads = 256;
+constexpr uint32_t kResultWarps = 8;  // two for each quarter of the lanes of tensor memory
+constexpr int kThreads = 128 + 32 * kResultWarps;
+constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kGradientColumns = 256;
 
@@ -157,11 +160,19 @@ __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void*
         }
     }
     if (count == 16u && reinterpret_cast<uintptr_t>(at) % 16u == 0u) {
-        const uint4* from = reinterpret_cast<const uint4*>(out);
-        uint4* to = reinterpret_cast<uint4*>(at);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(out);
+        if (reinterpret_cast<uintptr_t>(at) % 32u == 0u) {
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(out) / 16u; ++i) {
-            to[i] = from[i];
+            for (uint32_t i = 0; i < sizeof(out) / 32u; ++i) {
+                const uint32_t eight[8] = {words[8 * i],     words[8 * i + 1], words[8 * i + 2], words[8 * i + 3],
+                                           words[8 * i + 4], words[8 * i + 5], words[8 * i + 6], words[8 * i + 7]};
+                Store32(reinterpret_cast<unsigned char*>(at) + 32u * i, eight);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof(out) / 16u; ++i) {
+                reinterpret_cast<uint4*>(at)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+            }
         }
     } else {
 #pragma unroll
@@ -208,15 +219,6 @@ __device__ __forceinline__ uint32_t AddSums(uint32_t a, uint32_t b)
     return kInt8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
-template <bool kGradient>
-struct ScheduleOf {
-    using Type = ForwardSchedule;
-};
-template <>
-struct ScheduleOf<true> {
-    using Type = GradientSchedule;
-};
-
 template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
     GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
@@ -232,7 +234,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint64_t empty[R::kStages];
     __shared__ uint64_t sumsFull[2];
     __shared__ uint64_t sumsEmpty[2];
-    __shared__ uint64_t joined;     // the four result warps meet here
+    __shared__ uint64_t segmentFull[kSegments];
+    __shared__ uint64_t segmentEmpty[kSegments];
+    __shared__ Segment segments[kSegments];
+    __shared__ uint64_t joined;     // the result warps meet here
     __shared__ uint64_t drained;
     __shared__ uint64_t tailReady[R::kStages];  // first CTA of a pair: the second one has cut a block's last rows off
     __shared__ uint32_t tmemAddress;
@@ -243,6 +248,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane = threadIdx.x % 32u;
     const uint32_t rank = kCtas == 2 ? blockIdx.x % 2u : 0u;  // in the pair; rank 0 issues the MMAs
     const Workers workers{blockIdx.x / kCtas, gridDim.x / kCtas};
+    // warp 1 issues the MMAs in the first CTA, and cuts blocks off in the second one
+    const bool readsSegments = rank == 0u || kGradient;
     const uint32_t ring = (SmemAddress(dynamic) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < R::kStages; ++i) {
@@ -252,9 +259,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (uint32_t i = 0; i < 2; ++i) {
             BarInit(SmemAddress(sumsFull + i), 1);
-            BarInit(SmemAddress(sumsEmpty + i), 4u * kCtas);
+            BarInit(SmemAddress(sumsEmpty + i), kResultWarps * kCtas);
         }
-        BarInit(SmemAddress(&joined), 4);
+        for (uint32_t i = 0; i < kSegments; ++i) {
+            BarInit(SmemAddress(segmentFull + i), 1);
+            BarInit(SmemAddress(segmentEmpty + i), 1u + kResultWarps + (readsSegments ? 1u : 0u));
+        }
+        BarInit(SmemAddress(&joined), kResultWarps);
         BarInit(SmemAddress(&drained), 1);
         gaveUp = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -274,12 +285,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = tmemAddress;
     volatile uint32_t* const stop = &gaveUp;
 
-    auto makeSchedule = [&]() {
-        if constexpr (kGradient) {
-            return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock);
-        } else {
-            return ForwardSchedule(p, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
+    // The next segment of the schedule, for one of the warps that follow it; parts == 0 ends it.
+    uint32_t taken = 0;
+    auto nextSegment = [&](Segment* s) {
+        const uint32_t i = taken % kSegments;
+        if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop))) {
+            return false;
         }
+        *s = segments[i];
+        __syncwarp();
+        if (lane == 0) {
+            BarArrive(SmemAddress(segmentEmpty + i));
+        }
+        ++taken;
+        return s->parts != 0u;
     };
     // Gradient: rows of block b that belong to the group.  The last block of a group may hold rows behind it; those of
     // the last MMA's share are somebody else's and are overwritten with zeros, in both operands, so that no infinity or
@@ -299,13 +318,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp == 0) {
-        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         Segment s;
         uint32_t stage = 0;
         uint32_t parity = 0;
         uint32_t loads = 0;
         bool good = true;
-        while (good && schedule.Next(&s)) {
+        while (good && nextSegment(&s)) {
             const uint32_t share = (s.columns + kColumnStep - 1u) / kColumnStep * 16u;  // of the columns, in this CTA
             const uint32_t boxes = (share + R::kBox - 1u) / R::kBox;
             const uint32_t bytes = kLeftBytes + boxes * R::kBox * 128u;
@@ -371,7 +389,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1 && rank == 0u) {
-        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         const bool leftT = kGradient || leftMn != 0u;
         const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
         // 32 bytes of the summed index per instruction: inside a 128-byte row, or as many rows as it has elements
@@ -383,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t tile = 0;
         uint32_t cuts = 0;  // a bit per stage: the parity of its next cut block
         bool good = true;
-        while (good && schedule.Next(&s)) {
+        while (good && nextSegment(&s)) {
             const uint32_t half = tile & 1u;
             good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop)) != 0;
             if (!good) {
@@ -444,11 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (kGradient && kCtas == 2 && warp == 1) {
         // second CTA of a pair: cuts the last rows of its share of a block off, then tells the first one
-        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         Segment s;
         uint32_t block = 0;  // of all that this worker loads: the stage is block % kStages
         uint32_t cuts = 0;
-        while (schedule.Next(&s)) {
+        while (nextSegment(&s)) {
             const uint32_t count = s.block1 - s.block0;
             const uint32_t valid = count != 0u ? validRows(s, s.block1 - 1u) : 0u;
             if (valid % kStepElements != 0u) {
@@ -464,18 +480,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             block += count;
         }
+    } else if (warp == 3) {
+        auto schedule = [&]() {
+            if constexpr (kGradient) {
+                return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock);
+            } else {
+                return ForwardSchedule(p, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
+            }
+        }();
+        bool more = true;
+        for (uint32_t given = 0; more; ++given) {
+            Segment s;
+            more = schedule.Next(&s);
+            s.parts = more ? s.parts : 0u;
+            const uint32_t i = given % kSegments;
+            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentEmpty + i), (given / kSegments & 1u) ^ 1u, stop))) {
+                break;
+            }
+            if (lane == 0) {
+                segments[i] = s;
+                BarArrive(SmemAddress(segmentFull + i));
+            }
+            __syncwarp();
+        }
     } else if (warp >= 4) {
-        typename ScheduleOf<kGradient>::Type schedule = makeSchedule();
         const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
         const float beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
-        const uint32_t tmemLane = threadIdx.x - 128u;
+        const uint32_t tmemLane = threadIdx.x % 128u;
+        const uint32_t firstChunk = (warp - 4u) / 4u * 16u;  // of the columns: warps that share lanes take turns
+        constexpr uint32_t kChunkStep = kResultWarps / 4u * 16u;
         uint32_t* const counters = buffer + kGroupedHeaderWords;
-        uint32_t* const partials = counters + kGroupedCounters;
-        constexpr uint32_t kSlotWords = kTileLanes * kColumns;
+        uint4* const partials = reinterpret_cast<uint4*>(counters + kGroupedCounters);
+        constexpr uint32_t kSlotVectors = kTileLanes * kColumns / 4u;
         Segment s;
         uint32_t tile = 0;
         uint32_t meetings = 0;
-        // The four warps meet; bounded like every wait.
+        // The result warps meet; bounded like every wait.
         auto meet = [&]() {
             __syncwarp();
             if (lane == 0) {
@@ -496,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         };
-        while (schedule.Next(&s)) {
+        while (nextSegment(&s)) {
             const uint32_t half = tile & 1u;
             if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsFull + half), tile >> 1 & 1u, stop))) {
                 break;
@@ -511,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + row);
             }
             if (s.parts == 1u) {
-                for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+                for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
                     uint32_t bits[16];
                     Lane16 sums;
                     __syncwarp();
@@ -526,14 +566,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release(half);
                 continue;
             }
-            uint32_t* const mine = partials + static_cast<size_t>(s.slot * kCtas + rank) * kSlotWords + tmemLane;
-            for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+            // Partial sums lie four columns of a lane to a vector: [columns / 4][lanes][4].
+            uint4* const mine = partials + static_cast<size_t>(s.slot * kCtas + rank) * kSlotVectors + tmemLane;
+            for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
                 uint32_t bits[16];
+                __syncwarp();
                 TmemLoad16(from + j0, bits);
                 TmemLoadWait();
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    __stcg(mine + (j0 + j) * kTileLanes, bits[j]);
+                for (uint32_t j = 0; j < 4; ++j) {
+                    __stcg(mine + (j0 / 4u + j) * kTileLanes,
+                           make_uint4(bits[4 * j], bits[4 * j + 1], bits[4 * j + 2], bits[4 * j + 3]));
                 }
             }
             release(half);
@@ -541,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!meet()) {
                 break;
             }
-            if (tmemLane == 0) {
+            if (threadIdx.x == 128u) {
                 uint32_t* const counter = counters + s.counter * kCtas + rank;
                 const uint32_t before = atomicAdd(counter, 1u);
                 isLast = before + 1u == s.parts ? 1u : 0u;
@@ -557,21 +600,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue;
             }
             __threadfence();
-            for (uint32_t j0 = 0; j0 < s.columns; j0 += 16u) {
+            for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
+                const uint4* at = partials + tmemLane + j0 / 4u * kTileLanes;
+                auto part = [&](uint32_t i, uint4 (&v)[4]) {
+                    const uint32_t slot = i == 0u ? s.firstSlot : 2u * (s.firstWorker + i);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        v[j] = __ldcg(at + static_cast<size_t>(slot * kCtas + rank) * kSlotVectors + j * kTileLanes);
+                    }
+                };
                 uint32_t total[16];
-                const uint32_t offset = j0 * kTileLanes + tmemLane;
-                const uint32_t* first = partials + static_cast<size_t>(s.firstSlot * kCtas + rank) * kSlotWords + offset;
+                uint4 v[4];
+                part(0, v);
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    total[j] = __ldcg(first + j * kTileLanes);
+                for (uint32_t j = 0; j < 4; ++j) {
+                    total[4 * j] = v[j].x;
+                    total[4 * j + 1] = v[j].y;
+                    total[4 * j + 2] = v[j].z;
+                    total[4 * j + 3] = v[j].w;
                 }
-#pragma unroll 2
-                for (uint32_t part = 1; part < s.parts; ++part) {
-                    const uint32_t slot = 2u * (s.firstWorker + part) * kCtas + rank;
-                    const uint32_t* next = partials + static_cast<size_t>(slot) * kSlotWords + offset;
+#pragma unroll 4
+                for (uint32_t i = 1; i < s.parts; ++i) {
+                    part(i, v);
 #pragma unroll
-                    for (uint32_t j = 0; j < 16; ++j) {
-                        total[j] = AddSums<kInt8>(total[j], __ldcg(next + j * kTileLanes));
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        total[4 * j] = AddSums<kInt8>(total[4 * j], v[j].x);
+                        total[4 * j + 1] = AddSums<kInt8>(total[4 * j + 1], v[j].y);
+                        total[4 * j + 2] = AddSums<kInt8>(total[4 * j + 2], v[j].z);
+                        total[4 * j + 3] = AddSums<kInt8>(total[4 * j + 3], v[j].w);
                     }
                 }
                 Lane16 sums;

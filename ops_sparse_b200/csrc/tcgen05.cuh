@@ -215,6 +215,14 @@ __device__ __forceinline__ void TmemLoad16(uint32_t address, uint32_t (&r)[16])
         : "r"(address));
 }
 
+// 32 bytes to a 32-byte aligned address: one whole sector.
+__device__ __forceinline__ void Store32(void* p, const uint32_t (&r)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 __device__ __forceinline__ void TmemLoadWait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
 // Shared-memory descriptor of an operand in rows of 128 bytes with the 128-byte swizzle, eight rows (1024 bytes) per
