@@ -12,6 +12,7 @@
 constexpr uint32_t kGroupedHeaderWords = 16;
 // What writing and joining partial sums costs, in blocks of the summed index: a tile is split only where more is saved.
 constexpr uint32_t kJoinBlocks = 8;
+constexpr uint32_t kJoinBlocksWide = 48;  // tiles of 256 columns
 
 // Columns of a tile: rows of a group that one tile takes (forward), columns of C_g (gradient).
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p);

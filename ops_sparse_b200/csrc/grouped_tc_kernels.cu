@@ -18,8 +18,9 @@
  * One CTA per SM, persistent: warp 0 loads blocks of 128 bytes of the summed index
  * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 11 read
  * the finished sums and write results while the next tile computes in the other
- * half of tensor memory.  Warp 3 works out the next tiles ahead of all of them: done by
- * the MMA warp itself it left the tensor cores idle for 600 cycles per tile.  Tiles that do not fill a wave are split along the summed
+ * half of tensor memory.  Warp 3 works out the next tiles ahead of all of them, and
+ * warp 2 cuts the ends of groups off; done by the MMA warp itself either left the
+ * tensor cores idle for 600 cycles per tile.  Tiles that do not fill a wave are split along the summed
  * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and the one
  * that arrives last adds them in the CTAs' order, so that the result does not
  * depend on who that is.
@@ -49,6 +50,7 @@ constexpr int kThreads = 128 + 32 * kResultWarps;
 constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kGradientColumns = 256;
+constexpr uint64_t kDrainNs = 10000000ull;
 
 template <uint32_t kColumns, uint32_t kCtas>
 struct Ring {
@@ -56,7 +58,7 @@ struct Ring {
     static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
     static constexpr uint32_t kStages = 224u * 1024u / kStageBytes;
     static constexpr uint32_t kBytes = kStageBytes * kStages + 1024u;  // stages start on multiples of 1024
-    static constexpr uint32_t kBox = kColumns < 64u ? kColumns : 64u;  // rows of one load of the right operand
+    static constexpr uint32_t kBox = 32;                       // rows of one load of the right operand
 };
 
 // One result in the type of C; beta == 0 does not read C.
@@ -239,7 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Segment segments[kSegments];
     __shared__ uint64_t joined;     // the result warps meet here
     __shared__ uint64_t drained;
-    __shared__ uint64_t tailReady[R::kStages];  // first CTA of a pair: the second one has cut a block's last rows off
+    __shared__ uint64_t cutFull[R::kStages];  // a block whose last rows are to be cut off has landed in this CTA
+    __shared__ uint64_t cutDone[R::kStages];  // first CTA: a block's last rows are cut off, in both CTAs
     __shared__ uint32_t tmemAddress;
     __shared__ uint32_t gaveUp;
     __shared__ uint32_t isLast;
@@ -248,14 +251,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane = threadIdx.x % 32u;
     const uint32_t rank = kCtas == 2 ? blockIdx.x % 2u : 0u;  // in the pair; rank 0 issues the MMAs
     const Workers workers{blockIdx.x / kCtas, gridDim.x / kCtas};
-    // warp 1 issues the MMAs in the first CTA, and cuts blocks off in the second one
-    const bool readsSegments = rank == 0u || kGradient;
     const uint32_t ring = (SmemAddress(dynamic) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < R::kStages; ++i) {
             BarInit(SmemAddress(full + i), 1);
             BarInit(SmemAddress(empty + i), 1);
-            BarInit(SmemAddress(tailReady + i), 1);
+            BarInit(SmemAddress(cutFull + i), 1);
+            BarInit(SmemAddress(cutDone + i), kCtas);
         }
         for (uint32_t i = 0; i < 2; ++i) {
             BarInit(SmemAddress(sumsFull + i), 1);
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (uint32_t i = 0; i < kSegments; ++i) {
             BarInit(SmemAddress(segmentFull + i), 1);
-            BarInit(SmemAddress(segmentEmpty + i), 1u + kResultWarps + (readsSegments ? 1u : 0u));
+            BarInit(SmemAddress(segmentEmpty + i), 1u + kResultWarps + (rank == 0u ? 1u : 0u) + (kGradient ? 1u : 0u));
         }
         BarInit(SmemAddress(&joined), kResultWarps);
         BarInit(SmemAddress(&drained), 1);
@@ -318,15 +320,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp == 0) {
+        constexpr uint32_t kBox = kGradient ? 64u : R::kBox;
         Segment s;
         uint32_t stage = 0;
         uint32_t parity = 0;
-        uint32_t loads = 0;
         bool good = true;
         while (good && nextSegment(&s)) {
             const uint32_t share = (s.columns + kColumnStep - 1u) / kColumnStep * 16u;  // of the columns, in this CTA
-            const uint32_t boxes = (share + R::kBox - 1u) / R::kBox;
-            const uint32_t bytes = kLeftBytes + boxes * R::kBox * 128u;
+            const uint32_t boxes = (share + kBox - 1u) / kBox;
+            const uint32_t bytes = kLeftBytes + boxes * kBox * 128u;
             const uint32_t leftAt = s.left + rank * kTileLanes;
             const uint32_t rightAt = (kGradient ? s.right : s.row0) + rank * share;
             if (ElectLane()) {
@@ -335,17 +337,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         good = false;
                         break;
                     }
-                    // A pair's blocks are announced to the first CTA, except those whose last rows are cut off: the
-                    // second CTA has to see to its own share first.
-                    const uint32_t bar0 = SmemAddress(full + stage);
                     const uint32_t left = ring + stage * R::kStageBytes;
                     const uint32_t right = left + kLeftBytes;
                     const bool cut = kGradient && validRows(s, b) % kStepElements != 0u;
-                    const bool own = rank == 0u || cut;
-                    if (own) {
-                        BarExpect(bar0, kCtas == 2 && !cut ? 2u * bytes : bytes);
+                    // A pair's blocks are announced to the first CTA, except those whose last rows are cut off: each
+                    // CTA's warp 2 sees to its share first, and the MMAs wait for that.
+                    uint32_t bar = SmemAddress((cut ? cutFull : full) + stage);
+                    if (cut) {
+                        BarExpect(bar, bytes);
+                        if (rank == 0u) {
+                            BarArrive(SmemAddress(full + stage));
+                        }
+                    } else if (rank == 0u) {
+                        BarExpect(bar, kCtas * bytes);
+                    } else {
+                        bar = PeerAddress(bar, 0);
                     }
-                    const uint32_t bar = own ? bar0 : PeerAddress(bar0, 0);
                     const int32_t at = static_cast<int32_t>(b * kBlock);
                     if constexpr (kGradient) {
                         const int32_t row = static_cast<int32_t>(s.row0) + at;
@@ -365,11 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                         for (uint32_t i = 0; i < boxes; ++i) {
-                            TmaLoad2<kCtas>(right + i * R::kBox * 128u, &rightMap, bar, at,
-                                            static_cast<int32_t>(rightAt + i * R::kBox));
+                            TmaLoad2<kCtas>(right + i * kBox * 128u, &rightMap, bar, at,
+                                            static_cast<int32_t>(rightAt + i * kBox));
                         }
                     }
-                    ++loads;
                     stage = stage + 1u == R::kStages ? 0u : stage + 1u;
                     parity ^= stage == 0u ? 1u : 0u;
                 }
@@ -377,15 +383,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             good = __all_sync(0xFFFFFFFFu, good) != 0;
         }
-        // A CTA that gives up must not end under its copies.  The first CTA's barriers know when they have landed; the
-        // second one of a pair, which has no barrier for them, gives them the limit of a wait.
-        if (loads != 0u && !good) {  // the lane that issued them
-            const uint32_t last = loads < R::kStages ? loads : R::kStages;
-            uint32_t never = 0;
-            for (uint32_t i = 0; i < last; ++i) {
-                stage = stage == 0u ? R::kStages - 1u : stage - 1u;
-                parity ^= stage == R::kStages - 1u ? 1u : 0u;
-                (void)BarWait(SmemAddress(full + stage), rank == 0u ? parity : 0u, &never);
+        // A CTA that gives up must not end under its copies: they have this long to land.
+        if (!good) {
+            const uint64_t began = Nanoseconds();
+            while (Nanoseconds() - began < kDrainNs) {
             }
         }
     } else if (warp == 1 && rank == 0u) {
@@ -400,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t tile = 0;
         uint32_t cuts = 0;  // a bit per stage: the parity of its next cut block
         bool good = true;
-        while (good && nextSegment(&s)) {
+        bool more = nextSegment(&s);
+        while (more) {
             const uint32_t half = tile & 1u;
             good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop)) != 0;
             if (!good) {
@@ -411,6 +413,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t d = tmem + half * kColumns;
             const uint32_t instruction = shape | MmaColumns((s.columns + kColumnStep - 1u) / kColumnStep * kColumnStep);
             const uint32_t length = kGradient ? s.rows : p.k;
+            Segment next;
+            if (s.block0 == s.block1) {
+                more = nextSegment(&next);
+            }
             for (uint32_t b = s.block0; b < s.block1; ++b) {
                 good = BarWait(SmemAddress(full + stage), parity, stop);
                 good = __all_sync(0xFFFFFFFFu, good) != 0;
@@ -423,14 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t steps = (valid + kStepElements - 1u) / kStepElements;
                 if constexpr (kGradient) {
                     if (valid % kStepElements != 0u) {
-                        cutRows(valid, left);
-                        if constexpr (kCtas == 2) {
-                            good = __all_sync(0xFFFFFFFFu,
-                                              BarWait(SmemAddress(tailReady + stage), cuts >> stage & 1u, stop)) != 0;
-                            cuts ^= 1u << stage;
-                            if (!good) {
-                                break;
-                            }
+                        good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop)) != 0;
+                        cuts ^= 1u << stage;
+                        if (!good) {
+                            break;
                         }
                     }
                 }
@@ -446,6 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     MmaCommit<kCtas>(SmemAddress(empty + stage));
                 }
+                if (b == s.block0) {
+                    more = nextSegment(&next);  // while this tile computes
+                }
                 stage = stage + 1u == R::kStages ? 0u : stage + 1u;
                 parity ^= stage == 0u ? 1u : 0u;
             }
@@ -453,29 +458,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 MmaCommit<kCtas>(SmemAddress(sumsFull + half));
             }
             __syncwarp();
+            more = more && good;
+            s = next;
         }
         if (!good && ElectLane()) {  // not under instructions that still read tensor memory
             uint32_t never = 0;
             MmaCommit<kCtas>(SmemAddress(&drained));
             (void)BarWait(SmemAddress(&drained), 0, &never);
         }
-    } else if (kGradient && kCtas == 2 && warp == 1) {
-        // second CTA of a pair: cuts the last rows of its share of a block off, then tells the first one
+    } else if (kGradient && warp == 2) {
         Segment s;
-        uint32_t block = 0;  // of all that this worker loads: the stage is block % kStages
-        uint32_t cuts = 0;
+        uint32_t block = 0;  // of all that this CTA loads: the stage is block % kStages
+        uint32_t cuts = 0;   // a bit per stage: the parity of its next cut block
         while (nextSegment(&s)) {
             const uint32_t count = s.block1 - s.block0;
             const uint32_t valid = count != 0u ? validRows(s, s.block1 - 1u) : 0u;
             if (valid % kStepElements != 0u) {
                 const uint32_t stage = (block + count - 1u) % R::kStages;
-                if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(full + stage), cuts >> stage & 1u, stop))) {
+                if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutFull + stage), cuts >> stage & 1u, stop))) {
                     break;
                 }
                 cuts ^= 1u << stage;
                 cutRows(valid, ring + stage * R::kStageBytes);
                 if (lane == 0) {
-                    BarArrivePeer(PeerAddress(SmemAddress(tailReady + stage), 0));
+                    const uint32_t done = SmemAddress(cutDone + stage);
+                    if (rank == 0u) {
+                        BarArrive(done);
+                    } else {
+                        BarArrivePeer(PeerAddress(done, 0));
+                    }
                 }
             }
             block += count;
@@ -727,7 +738,7 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kJoinBlocks);
+    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
 }
 
 }  // namespace
@@ -785,7 +796,7 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
     const uint64_t rightStride[1] = {static_cast<uint64_t>(p.aOuter)};
     const uint32_t leftBox = leftMn != 0 ? static_cast<uint32_t>(128u / bytes) : kTileLanes;
     if (!Encode(&left, p, b, 3, leftSizes, leftStrides, leftBox) ||
-        !Encode(&right, p, a, 2, rightSizes, rightStride, columns < 64u ? columns : 64u)) {
+        !Encode(&right, p, a, 2, rightSizes, rightStride, Ring<256, 2>::kBox)) {
         return false;
     }
     const bool int8 = p.inType == ACLSP_TYPE_I8;

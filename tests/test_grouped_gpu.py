@@ -145,6 +145,14 @@ def test_forward_strides_and_alignment(dtype, order, pad, shift):
     Forward([40, 0, 9, 150], 96, 160, dtype, order=order, pad=pad, shift=shift, batch_pad=16).check()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,k,n", [([700, 1, 0, 1500, 333, 256, 900, 40], 320, 2304), ([130] * 9, 1040, 4096),
+                                       ([6000], 208, 1536)])
+def test_forward_many_waves_of_tiles(dtype, sizes, k, n):
+    """More tiles than CTAs, several times over: every stage of the ring and both halves of the sums are reused."""
+    Forward(sizes, k, n, dtype, seed=n, first=1, behind=2).check()
+
+
 def test_forward_rows_outside_the_groups_stay():
     Forward([5, 0, 70], 64, 64, torch.bfloat16, first=7, behind=300).check()
 
@@ -333,6 +341,12 @@ def test_gradient_shapes(dtype, order, m, n):
 @pytest.mark.parametrize("sizes", [[1], [15], [16], [17], [63], [64], [65], [0], [0, 0], [700], [1] * 40, [300, 0, 513, 31, 32]])
 def test_gradient_group_sizes(sizes):
     Gradient(sizes, 144, 272, torch.bfloat16, first=2, behind=3, seed=len(sizes)).check()
+
+
+@pytest.mark.parametrize("sizes", [[150, 0, 1, 700, 64, 65, 31, 2, 0, 400, 17, 300], [3] * 12, [1000] + [0] * 11])
+def test_gradient_many_tiles(sizes):
+    """Several tiles per CTA, most of them with rows to cut off, in every stage of the ring."""
+    Gradient(sizes, 1280, 1288, torch.bfloat16, first=5, behind=9, seed=sizes[0]).check()
 
 
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
