@@ -17,7 +17,8 @@ constexpr uint32_t kJoinBlocksWide = 48;  // tiles of 256 columns
 // Columns of a tile: rows of a group that one tile takes (forward), columns of C_g (gradient).
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p);
 
-// Launches the product; false, and nothing launched, where the operands do not fit tensor maps.
+// Launches the product; false, and nothing launched, where there is nothing to sum over or the tiles are too many to
+// number.
 bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
                               cudaStream_t stream);
 
