@@ -2,9 +2,12 @@
  * Grouped matrix products: one dense matrix per ragged group of rows (forward),
  * and the gradient of those matrices, a sum over a ragged group of rows.
  *
- * PlainKernel: 64 x 64 tiles of the result, operands staged through shared
- * memory element by element with any strides, products and sums in registers
- * (fp32 FMA; int32 for int8).
+ * The work is done on the tensor cores (grouped_tc_kernels.cu).  Here are the
+ * kernels around that: CopyRowsKernel, which brings operands of odd widths to rows
+ * that TMA can load, and PlainKernel for what is left: bases that are not 16-byte
+ * aligned, sums over nothing, and sizes beyond 2^28.  It computes 64 x 64 tiles,
+ * operands staged through shared memory element by element, products and sums in
+ * registers (fp32 FMA; int32 for int8).
  */
 #include <cstdint>
 
@@ -25,8 +28,6 @@ using aclsp::kBF16;
 using aclsp::kF16;
 using aclsp::kI8;
 
-// The part of the buffer that Preprocess clears, and where partial sums begin.
-constexpr uint32_t kCountersEnd = 4u * (kGroupedHeaderWords + aclsp::kGroupedCounters);
 
 template <int kIn>
 struct Plain {
@@ -154,18 +155,96 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
     }
 }
 
+// The word at `at`, zeros in place of bytes outside [begin, end).
+__device__ __forceinline__ uint32_t WordOf(const unsigned char* at, const unsigned char* begin, const unsigned char* end)
+{
+    if (at >= begin && at + 4 <= end) {
+        return __ldg(reinterpret_cast<const uint32_t*>(at));
+    }
+    uint32_t v = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (at + i >= begin && at + i < end) {
+            v |= static_cast<uint32_t>(__ldg(at + i)) << (8 * i);
+        }
+    }
+    return v;
+}
+
+constexpr uint32_t kCopyThreads = 256;
+constexpr uint32_t kCopyWords = 4;  // words of a row that a lane has under way
+
+// A warp per stretch of kCopyWords * 128 bytes of a row: it reads aligned words, also the one behind each (from L1 or a
+// neighbour's line), shifts the bytes into place and writes aligned words, the last of a row with what lies behind it.
+// Bound by HBM: every byte is read and written once.
+__global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const unsigned char* __restrict__ src,
+                                                               unsigned char* __restrict__ dst, uint32_t rows,
+                                                               uint32_t batches, int64_t rowBytes, int64_t pitch,
+                                                               int64_t batchPitch, int64_t dstPitch, int64_t dstBatchPitch,
+                                                               const int32_t* offsets, uint32_t offsetRows)
+{
+    const uint32_t lane = threadIdx.x % 32u;
+    const uint32_t stretches = static_cast<uint32_t>((dstPitch + kCopyWords * 128 - 1) / (kCopyWords * 128));
+    const int64_t perBatch = static_cast<int64_t>(rows) * stretches;
+    const int64_t all = perBatch * batches;
+    const unsigned char* const end = src + (batches - 1) * batchPitch + (rows - 1) * pitch + rowBytes;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kCopyThreads / 32u);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kCopyThreads / 32u) + threadIdx.x / 32u; i < all; i += warps) {
+        const uint32_t batch = static_cast<uint32_t>(i / perBatch);
+        if (batches > 1u) {
+            uint32_t first, last;
+            aclsp::GroupRows(offsets, batch, offsetRows, &first, &last);
+            if (first == last) {  // nobody reads this matrix: on to the next one's stretches
+                i += (perBatch * (batch + 1) - i - 1) / warps * warps;
+                continue;
+            }
+        }
+        const uint32_t inBatch = static_cast<uint32_t>(i - batch * perBatch);
+        const uint32_t row = inBatch / stretches;
+        const int64_t byte = static_cast<int64_t>(inBatch % stretches) * (kCopyWords * 128) + 4 * lane;
+        const unsigned char* from = src + batch * batchPitch + row * pitch + byte;
+        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 3u;
+        from -= shift;
+        uint32_t low[kCopyWords];
+        uint32_t high[kCopyWords];
+#pragma unroll
+        for (uint32_t w = 0; w < kCopyWords; ++w) {
+            const bool wanted = byte + 128 * w < rowBytes;
+            low[w] = wanted ? WordOf(from + 128 * w, src, end) : 0u;
+            high[w] = wanted && shift != 0u ? WordOf(from + 128 * w + 4, src, end) : 0u;
+        }
+        unsigned char* const to = dst + batch * dstBatchPitch + row * dstPitch + byte;
+#pragma unroll
+        for (uint32_t w = 0; w < kCopyWords; ++w) {
+            if (byte + 128 * w < dstPitch) {
+                *reinterpret_cast<uint32_t*>(to + 128 * w) = __funnelshift_r(low[w], high[w], 8u * shift);
+            }
+        }
+    }
+}
+
 }  // namespace
+
+void AclspGroupedCopyRows(const void* src, void* dst, const AclspGroupedOperand& from, uint64_t ld,
+                          const AclspGroupedParams& p, cudaStream_t stream)
+{
+    const int64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1 : 2;
+    AclspCountLaunches(1);
+    CopyRowsKernel<<<148 * 8, kCopyThreads, 0, stream>>>(
+        static_cast<const unsigned char*>(src), static_cast<unsigned char*>(dst), static_cast<uint32_t>(from.rows),
+        static_cast<uint32_t>(from.batches), static_cast<int64_t>(from.rowElements) * bytes,
+        static_cast<int64_t>(from.ld) * bytes, static_cast<int64_t>(from.batchStride) * bytes, static_cast<int64_t>(ld) * bytes,
+        static_cast<int64_t>(from.rows * ld) * bytes, p.offsets, p.rows);
+}
 
 extern "C" uint64_t aclsp_b200_grouped_buffer_bytes(const AclspGroupedParams* params)
 {
-    // two partial tiles per CTA at most
-    return kCountersEnd + 2ull * aclsp::kGroupedMaxCtas * aclsp::kTileLanes * AclspGroupedColumns(*params) * 4u;
+    return AclspGroupedDescribe(*params).bufferBytes;
 }
 
 extern "C" void aclsp_b200_grouped_preprocess_kernel_do(void* buffer, void* stream)
 {
     AclspCountLaunches(1);
-    cudaMemsetAsync(buffer, 0, kCountersEnd, static_cast<cudaStream_t>(stream));
+    cudaMemsetAsync(buffer, 0, kGroupedCountersEnd, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" void aclsp_b200_grouped_mm_kernel_do(const void* a, const void* b, void* c, void* buffer,

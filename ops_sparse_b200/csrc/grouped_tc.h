@@ -8,8 +8,11 @@
 #include <cuda_runtime.h>
 
 #include "aclsparse_b200_kernels.h"
+#include "grouped_schedule.cuh"
 
 constexpr uint32_t kGroupedHeaderWords = 16;
+// Where the partial sums begin; what is before them is what Preprocess clears.
+constexpr uint32_t kGroupedCountersEnd = 4u * (kGroupedHeaderWords + aclsp::kGroupedCounters);
 // What writing and joining partial sums costs, in blocks of the summed index: a tile is split only where more is saved.
 constexpr uint32_t kJoinBlocks = 8;
 constexpr uint32_t kJoinBlocksWide = 48;  // tiles of 256 columns
@@ -17,8 +20,32 @@ constexpr uint32_t kJoinBlocksWide = 48;  // tiles of 256 columns
 // Columns of a tile: rows of a group that one tile takes (forward), columns of C_g (gradient).
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p);
 
-// Launches the product; false, and nothing launched, where there is nothing to sum over or the tiles are too many to
-// number.
+// An operand as rows of contiguous elements, one batch of them per group (forward's dense matrix) or a single one.
+struct AclspGroupedOperand {
+    uint64_t rowElements;
+    uint64_t rows;
+    uint64_t batches;
+    uint64_t ld;
+    uint64_t batchStride;
+    // Rows that do not start on multiples of 16 bytes, which a tensor map asks for, are copied to ones that do, behind
+    // the partial sums; 0 where there is no need.
+    uint64_t copyBytes;
+    uint64_t copyOffset;
+};
+struct AclspGroupedOperands {
+    AclspGroupedOperand left;   // along the lanes: B, or A in the gradient
+    AclspGroupedOperand right;  // along the columns
+    uint64_t bufferBytes;
+};
+AclspGroupedOperands AclspGroupedDescribe(const AclspGroupedParams& p);
+
+// dst gets the operand's rows, its own ld and batchStride being those of `from`, with rows of ld (and batches of rows * ld)
+// elements.  Batches whose group has no rows are left out.
+void AclspGroupedCopyRows(const void* src, void* dst, const AclspGroupedOperand& from, uint64_t ld,
+                          const AclspGroupedParams& p, cudaStream_t stream);
+
+// Launches the product; false, and nothing launched, where a base is not 16-byte aligned, there is nothing to sum over
+// or the sizes are too large to number tiles and blocks.
 bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
                               cudaStream_t stream);
 

@@ -25,8 +25,9 @@
  * that arrives last adds them in the CTAs' order, so that the result does not
  * depend on who that is.
  *
- * Operands that no tensor map describes (kPanels) are loaded by eight more warps, word by word (panel_load.cuh), in
- * tiles of one CTA and 128 columns at most.
+ * Operands whose rows do not start on multiples of 16 bytes (odd widths) cannot be loaded by TMA: they are copied to
+ * rows that do first (grouped_kernels.cu), in the buffer.  Warps that bring such rows into shared memory themselves,
+ * shifting each word into place, were built and measured: 128 x 128 x 64 blocks took 3000 cycles instead of 256.
  *
  * Every wait is bounded.  One that runs out makes the CTA leave: the loads in
  * flight are waited for (bounded again), tensor memory is freed, and the buffer's
@@ -41,7 +42,6 @@
 #include "element_types.cuh"
 #include "grouped_schedule.cuh"
 #include "grouped_tc.h"
-#include "panel_load.cuh"
 #include "plan_kernels.h"
 #include "tcgen05.cuh"
 
@@ -49,12 +49,8 @@ namespace {
 
 using namespace aclsp;
 
-// Warps that write results: two for each quarter of the lanes of tensor memory, one where the loading warps of the
-// other form need the registers.
-template <bool kPanels>
-constexpr uint32_t kResultWarpsOf = kPanels ? 4u : 8u;
-template <bool kPanels>
-constexpr uint32_t kThreads = 32u * (4u + kResultWarpsOf<kPanels> + (kPanels ? kPanelWarps : 0u));
+constexpr uint32_t kResultWarps = 8;  // two for each quarter of the lanes of tensor memory
+constexpr int kThreads = 128 + 32 * kResultWarps;
 constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kGradientColumns = 256;
@@ -229,16 +225,15 @@ __device__ __forceinline__ uint32_t AddSums(uint32_t a, uint32_t b)
     return kInt8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
-template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas, bool kPanels>
-__global__ void __launch_bounds__(kThreads<kPanels>, 1)
+template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas>
+__global__ void __launch_bounds__(kThreads, 1)
     GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
-                        const void* __restrict__ leftBase, const void* __restrict__ rightBase, void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
+                        void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
                         const uint32_t leftMn, const uint32_t joinBlocks)
 {
     using R = Ring<kColumns, kCtas>;
     constexpr uint32_t kBlock = kInt8 ? 128u : 64u;         // elements of the summed index in a block
     constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;   // and in one MMA
-    constexpr uint32_t kResultWarps = kResultWarpsOf<kPanels>;
     constexpr uint32_t kColumnStep = 16u * kCtas;           // N of the MMA is a multiple of this
     extern __shared__ unsigned char dynamic[];
     __shared__ uint64_t full[R::kStages];
@@ -263,7 +258,7 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
     const uint32_t ring = (SmemAddress(dynamic) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < R::kStages; ++i) {
-            BarInit(SmemAddress(full + i), kPanels ? kPanelWarps : 1u);
+            BarInit(SmemAddress(full + i), 1);
             BarInit(SmemAddress(empty + i), 1);
             BarInit(SmemAddress(cutFull + i), 1);
             BarInit(SmemAddress(cutDone + i), kCtas);
@@ -274,18 +269,15 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
         }
         for (uint32_t i = 0; i < kSegments; ++i) {
             BarInit(SmemAddress(segmentFull + i), 1);
-            BarInit(SmemAddress(segmentEmpty + i), (kPanels ? kPanelWarps : 1u) + kResultWarps + (rank == 0u ? 1u : 0u) +
-                                                      (kGradient && !kPanels ? 1u : 0u));
+            BarInit(SmemAddress(segmentEmpty + i), 1u + kResultWarps + (rank == 0u ? 1u : 0u) + (kGradient ? 1u : 0u));
         }
         BarInit(SmemAddress(&joined), kResultWarps);
         BarInit(SmemAddress(&drained), 1);
         gaveUp = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         FenceProxyAsync();
-        if constexpr (!kPanels) {
-            TmaPrefetch(&leftMap);
-            TmaPrefetch(&rightMap);
-        }
+        TmaPrefetch(&leftMap);
+        TmaPrefetch(&rightMap);
     }
     if (warp == 2) {
         TmemAlloc<kCtas>(SmemAddress(&tmemAddress), 2u * kColumns);
@@ -331,7 +323,7 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
         __syncwarp();
     };
 
-    if (!kPanels && warp == 0) {
+    if (warp == 0) {
         constexpr uint32_t kBox = kGradient ? 64u : R::kBox;
         Segment s;
         uint32_t stage = 0;
@@ -439,7 +431,7 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
                 const uint32_t right = left + kLeftBytes;
                 const uint32_t valid = length - b * kBlock < kBlock ? length - b * kBlock : kBlock;
                 const uint32_t steps = (valid + kStepElements - 1u) / kStepElements;
-                if constexpr (kGradient && !kPanels) {
+                if constexpr (kGradient) {
                     if (valid % kStepElements != 0u) {
                         good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop)) != 0;
                         cuts ^= 1u << stage;
@@ -478,7 +470,7 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
             MmaCommit<kCtas>(SmemAddress(&drained));
             (void)BarWait(SmemAddress(&drained), 0, &never);
         }
-    } else if (kGradient && !kPanels && warp == 2) {
+    } else if (kGradient && warp == 2) {
         Segment s;
         uint32_t block = 0;  // of all that this CTA loads: the stage is block % kStages
         uint32_t cuts = 0;   // a bit per stage: the parity of its next cut block
@@ -525,75 +517,6 @@ __global__ void __launch_bounds__(kThreads<kPanels>, 1)
                 BarArrive(SmemAddress(segmentFull + i));
             }
             __syncwarp();
-        }
-    } else if (kPanels && warp >= 4u + kResultWarps) {
-        constexpr uint32_t kElement = kInt8 ? 1u : 2u;
-        const uint32_t loader = warp - 4u - kResultWarps;
-        const bool leftT = kGradient || leftMn != 0u;
-        // the matrices as rows of bytes: those of the left one in a forward product are a group's, from base to base
-        Panel left{};
-        Panel right{};
-        left.pitch = (kGradient ? p.aInner : (leftT ? p.bInner : p.bOuter)) * kElement;
-        left.rowBytes = static_cast<int64_t>(kGradient ? p.m : (leftT ? p.n : p.k)) * kElement;
-        right.pitch = (kGradient ? p.bInner : p.aOuter) * kElement;
-        right.rowBytes = static_cast<int64_t>(kGradient ? p.n : p.k) * kElement;
-        right.base = static_cast<const unsigned char*>(rightBase);
-        right.end = right.base + static_cast<int64_t>(p.rows - 1u) * right.pitch + right.rowBytes;
-        Segment s;
-        uint32_t stage = 0;
-        uint32_t parity = 0;
-        bool good = true;
-        while (good && nextSegment(&s)) {
-            left.base = static_cast<const unsigned char*>(leftBase);
-            if constexpr (!kGradient) {
-                left.base += static_cast<int64_t>(s.group) * p.bBatchStride * kElement;
-            }
-            left.end = left.base + static_cast<int64_t>((kGradient ? p.rows : (leftT ? p.k : p.n)) - 1u) * left.pitch + left.rowBytes;
-            const uint32_t rightRows = kGradient ? kColumns / 64u * 64u : (s.columns + 15u) / 16u * 16u;
-            for (uint32_t b = s.block0; b < s.block1; ++b) {
-                const uint32_t at = b * kBlock;
-                if constexpr (kGradient) {
-                    left.origin = right.origin = s.row0 + at;
-                    left.rows = right.rows = s.rows - at;
-                    left.firstByte = static_cast<int64_t>(s.left) * kElement;
-                    right.firstByte = static_cast<int64_t>(s.right) * kElement;
-                } else {
-                    left.origin = leftT ? at : s.left;
-                    left.rows = leftT ? p.k - at : p.n - s.left;
-                    left.firstByte = static_cast<int64_t>(leftT ? s.left : at) * kElement;
-                    right.origin = s.row0;
-                    right.rows = s.columns;
-                    right.firstByte = static_cast<int64_t>(at) * kElement;
-                }
-                PanelWords leftWords;
-                PanelWords rightWords;
-                // 16-bit operands with the summed index outside lie in two blocks of 64 such rows
-                constexpr uint32_t kTransposedRows = kInt8 ? 128u : 64u;
-                if (leftT) {
-                    PanelRead<kTransposedRows>(left, loader, lane, kTileLanes, &leftWords);
-                } else {
-                    PanelRead<128>(left, loader, lane, kTileLanes, &leftWords);
-                }
-                PanelRead<kGradient ? 64u : 128u>(right, loader, lane, rightRows, &rightWords);
-                good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(empty + stage), parity ^ 1u, stop)) != 0;
-                if (!good) {
-                    break;
-                }
-                const uint32_t smem = ring + stage * R::kStageBytes;
-                if (leftT) {
-                    PanelWrite<kTransposedRows>(left, loader, lane, kTileLanes, leftWords, smem);
-                } else {
-                    PanelWrite<128>(left, loader, lane, kTileLanes, leftWords, smem);
-                }
-                PanelWrite<kGradient ? 64u : 128u>(right, loader, lane, rightRows, rightWords, smem + kLeftBytes);
-                FenceProxyAsync();
-                __syncwarp();
-                if (lane == 0) {
-                    BarArrive(SmemAddress(full + stage));
-                }
-                stage = stage + 1u == R::kStages ? 0u : stage + 1u;
-                parity ^= stage == 0u ? 1u : 0u;
-            }
         }
     } else if (warp >= 4) {
         const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
@@ -789,34 +712,18 @@ bool Encode(CUtensorMap* map, const AclspGroupedParams& p, const void* base, uin
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// What a tensor map asks of a matrix: 16-byte aligned, strides of multiples of 16 bytes below 2^40.
-bool Mappable(const void* base, int64_t ld, int64_t batchStride, uint64_t bytes)
-{
-    const uint64_t pitch = static_cast<uint64_t>(ld) * bytes;
-    const uint64_t batch = static_cast<uint64_t>(batchStride) * bytes;
-    return reinterpret_cast<uintptr_t>(base) % 16u == 0u && pitch % 16u == 0u && batch % 16u == 0u && pitch < 1ull << 40 &&
-           batch < 1ull << 40;
-}
-
-struct Operands {
-    CUtensorMap leftMap;   // without kPanels
-    CUtensorMap rightMap;
-    const void* left;      // with kPanels
-    const void* right;
-};
-
-template <bool kInt8, uint32_t kColumns, bool kGradient, bool kPanels>
-void Launch(const Operands& o, void* c, void* buffer, const AclspGroupedParams& p, uint32_t leftMn, uint32_t sms,
-            cudaStream_t s)
+template <bool kInt8, uint32_t kColumns, bool kGradient>
+void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* buffer, const AclspGroupedParams& p,
+            uint32_t leftMn, uint32_t sms, cudaStream_t s)
 {
     constexpr uint32_t kCtas = kColumns == 256u ? 2u : 1u;
     constexpr uint32_t kBytes = Ring<kColumns, kCtas>::kBytes;
-    auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient, kCtas, kPanels>;
+    auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient, kCtas>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
     AclspCountLaunches(1);
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(sms / kCtas * kCtas);
-    config.blockDim = dim3(kThreads<kPanels>);
+    config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kBytes;
     config.stream = s;
     cudaLaunchAttribute cluster{};
@@ -826,8 +733,7 @@ void Launch(const Operands& o, void* c, void* buffer, const AclspGroupedParams& 
     cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, kernel, o.leftMap, o.rightMap, o.left, o.right, c, static_cast<uint32_t*>(buffer), p, leftMn,
-                       kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
+    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
 }
 
 }  // namespace
@@ -843,60 +749,96 @@ uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
     return average <= 24u ? 32u : average <= 96u ? 128u : 256u;
 }
 
+AclspGroupedOperands AclspGroupedDescribe(const AclspGroupedParams& p)
+{
+    AclspGroupedOperands o{};
+    if (p.weightGrad != 0) {
+        o.left = {p.m, p.rows, 1, static_cast<uint64_t>(p.aInner), 0, 0, 0};
+        o.right = {p.n, p.rows, 1, static_cast<uint64_t>(p.bInner), 0, 0, 0};
+    } else {
+        const bool kContiguous = p.bInner == 1;
+        o.left = {kContiguous ? p.k : p.n, kContiguous ? p.n : p.k, p.groups,
+                  static_cast<uint64_t>(kContiguous ? p.bOuter : p.bInner), static_cast<uint64_t>(p.bBatchStride), 0, 0};
+        o.right = {p.k, p.rows, 1, static_cast<uint64_t>(p.aOuter), 0, 0, 0};
+    }
+    o.bufferBytes = kGroupedCountersEnd + 2ull * kGroupedMaxCtas * kTileLanes * AclspGroupedColumns(p) * 4u;
+    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    for (AclspGroupedOperand* x : {&o.left, &o.right}) {
+        const bool strides = x->ld * bytes % 16u == 0u && (x->batches == 1u || x->batchStride * bytes % 16u == 0u);
+        if (!strides && x->rowElements != 0u && x->rows != 0u) {
+            x->copyOffset = (o.bufferBytes + 255u) / 256u * 256u;
+            x->copyBytes = x->batches * x->rows * ((x->rowElements * bytes + 15u) / 16u * 16u);
+            o.bufferBytes = x->copyOffset + x->copyBytes;
+        }
+    }
+    return o;
+}
+
 bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
                               cudaStream_t s)
 {
     constexpr uint32_t kLongest = 1u << 28;  // block and tile numbers stay far inside 32 bits
+    constexpr uint64_t kFarthest = 1ull << 40;  // strides that a tensor map takes, in bytes
     const uint32_t columns = AclspGroupedColumns(p);
-    const uint64_t tiles = p.weightGrad != 0
-                               ? static_cast<uint64_t>(p.groups) * ((p.m + kTileLanes - 1u) / kTileLanes) * ((p.n + 127u) / 128u)
-                               : (static_cast<uint64_t>(p.rows) / 32u + p.groups) * ((p.n + kTileLanes - 1u) / kTileLanes);
-    if (p.rows > kLongest || p.k > kLongest || (p.weightGrad == 0 && p.k == 0) || p.rows == 0 || tiles > 1u << 30) {
+    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    const uint64_t down = ((p.weightGrad != 0 ? p.m : p.n) + kTileLanes - 1u) / kTileLanes;
+    const uint64_t tiles = p.weightGrad != 0 ? p.groups * down * ((p.n + columns - 1u) / columns)
+                                             : (static_cast<uint64_t>(p.rows) / columns + p.groups) * down;
+    if (p.rows > kLongest || p.k > kLongest || (p.weightGrad == 0 && p.k == 0) || p.rows == 0 || tiles > 1u << 30 ||
+        Encoder() == nullptr) {
         return false;
+    }
+    AclspGroupedOperands o = AclspGroupedDescribe(p);
+    const void* bases[2] = {p.weightGrad != 0 ? a : b, p.weightGrad != 0 ? b : a};
+    AclspGroupedOperand* const operands[2] = {&o.left, &o.right};
+    for (uint32_t i = 0; i < 2; ++i) {
+        const AclspGroupedOperand& x = *operands[i];
+        const uint64_t batch = x.batches > 1u ? x.batchStride : 0u;
+        if (x.copyBytes == 0u && (reinterpret_cast<uintptr_t>(bases[i]) % 16u != 0u || x.ld * bytes >= kFarthest ||
+                                  batch * bytes >= kFarthest)) {
+            return false;
+        }
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+        AclspGroupedOperand* const x = operands[i];
+        if (x->copyBytes != 0u) {
+            void* const copy = static_cast<unsigned char*>(buffer) + x->copyOffset;
+            const uint64_t ld = (x->rowElements * bytes + 15u) / 16u * 16u / bytes;
+            AclspGroupedCopyRows(bases[i], copy, *x, ld, p, s);
+            bases[i] = copy;
+            x->ld = ld;
+            x->batchStride = x->rows * ld;
+        }
     }
     uint32_t sms = AclspSmCount();
     sms = sms == 0 || sms > kGroupedMaxCtas ? kGroupedMaxCtas : sms;
-    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
-    const bool int8 = p.inType == ACLSP_TYPE_I8;
-    Operands o{};
+    CUtensorMap left;
+    CUtensorMap right;
+    const uint64_t leftSizes[3] = {o.left.rowElements, o.left.rows, o.left.batches};
+    const uint64_t leftStrides[2] = {o.left.ld, o.left.batches > 1u ? o.left.batchStride : o.left.ld};
+    const uint64_t rightSizes[2] = {o.right.rowElements, o.right.rows};
+    const uint64_t rightStride[1] = {o.right.ld};
     if (p.weightGrad != 0) {
-        const uint64_t leftSizes[2] = {p.m, p.rows};
-        const uint64_t rightSizes[2] = {p.n, p.rows};
-        const uint64_t leftStride[1] = {static_cast<uint64_t>(p.aInner)};
-        const uint64_t rightStride[1] = {static_cast<uint64_t>(p.bInner)};
-        o.left = a;
-        o.right = b;
-        const bool mapped = Encoder() != nullptr && Mappable(a, p.aInner, 0, bytes) && Mappable(b, p.bInner, 0, bytes) &&
-                            Encode(&o.leftMap, p, a, 2, leftSizes, leftStride, 64) &&
-                            Encode(&o.rightMap, p, b, 2, rightSizes, rightStride, 64);
-        (mapped ? Launch<false, kGradientColumns, true, false> : Launch<false, 128, true, true>)(o, c, buffer, p, 1u, sms, s);
+        if (!Encode(&left, p, bases[0], 2, leftSizes, leftStrides, 64) ||
+            !Encode(&right, p, bases[1], 2, rightSizes, rightStride, 64)) {
+            return false;
+        }
+        Launch<false, kGradientColumns, true>(left, right, c, buffer, p, 1u, sms, s);
         return true;
     }
     const uint32_t leftMn = p.bInner == 1 ? 0u : 1u;
-    const int64_t ld = leftMn != 0 ? p.bInner : p.bOuter;
-    const int64_t batch = p.groups > 1 ? p.bBatchStride : ld;
-    const uint64_t leftSizes[3] = {leftMn != 0 ? p.n : p.k, leftMn != 0 ? p.k : p.n, p.groups};
-    const uint64_t leftStrides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(batch)};
-    const uint64_t rightSizes[2] = {p.k, p.rows};
-    const uint64_t rightStride[1] = {static_cast<uint64_t>(p.aOuter)};
     const uint32_t leftBox = leftMn != 0 ? static_cast<uint32_t>(128u / bytes) : kTileLanes;
-    o.left = b;
-    o.right = a;
-    const bool mapped = Encoder() != nullptr && Mappable(a, p.aOuter, 0, bytes) && Mappable(b, ld, batch, bytes) &&
-                        Encode(&o.leftMap, p, b, 3, leftSizes, leftStrides, leftBox) &&
-                        Encode(&o.rightMap, p, a, 2, rightSizes, rightStride, Ring<256, 2>::kBox);
-    decltype(&Launch<false, 32, false, false>) run;
-    if (mapped) {
-        run = int8 ? (columns == 32u    ? Launch<true, 32, false, false>
-                      : columns == 128u ? Launch<true, 128, false, false>
-                                        : Launch<true, 256, false, false>)
-                   : (columns == 32u    ? Launch<false, 32, false, false>
-                      : columns == 128u ? Launch<false, 128, false, false>
-                                        : Launch<false, 256, false, false>);
-    } else {
-        run = int8 ? (columns == 32u ? Launch<true, 32, false, true> : Launch<true, 128, false, true>)
-                   : (columns == 32u ? Launch<false, 32, false, true> : Launch<false, 128, false, true>);
+    if (!Encode(&left, p, bases[0], 3, leftSizes, leftStrides, leftBox) ||
+        !Encode(&right, p, bases[1], 2, rightSizes, rightStride, Ring<256, 2>::kBox)) {
+        return false;
     }
-    run(o, c, buffer, p, leftMn, sms, s);
+    const bool int8 = p.inType == ACLSP_TYPE_I8;
+    auto run = int8 ? (columns == 32u    ? Launch<true, 32, false>
+                       : columns == 128u ? Launch<true, 128, false>
+                                         : Launch<true, 256, false>)
+                    : (columns == 32u    ? Launch<false, 32, false>
+                       : columns == 128u ? Launch<false, 128, false>
+                                         : Launch<false, 256, false>);
+    run(left, right, c, buffer, p, leftMn, sms, s);
     return true;
 }
