@@ -289,6 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     TmemFenceAfter();
     const uint32_t tmem = tmemAddress;
+    WaitForPreviousKernel();
+    LetNextKernelStart();
     volatile uint32_t* const stop = &gaveUp;
 
     // The next segment of the schedule, for one of the warps that follow it; parts == 0 ends it.
@@ -726,13 +728,15 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kBytes;
     config.stream = s;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = kCtas;
-    cluster.val.clusterDim.y = 1;
-    cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = kCtas;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = kCtas > 1u ? 2u : 1u;
     cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
 }
 

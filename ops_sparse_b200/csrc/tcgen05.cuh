@@ -138,6 +138,11 @@ __device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map, u
     }
 }
 
+// A kernel launched with programmatic serialization starts while the one before it in the stream still runs: nothing of
+// that one's may be read, nor anything written, before this wait.  The other call lets the next such kernel start.
+__device__ __forceinline__ void WaitForPreviousKernel() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void LetNextKernelStart() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
 // Writes of this thread to shared memory become visible to the asynchronous proxy (TMA, tcgen05.mma).
 __device__ __forceinline__ void FenceProxyAsync()
 {
