@@ -50,6 +50,13 @@ public:
         const uint32_t begin = __shfl_sync(0xFFFFFFFFu, begin_, lane);
         const uint32_t size = __shfl_sync(0xFFFFFFFFu, size_, lane);
         const uint32_t pieces = (size + tileRows_ - 1u) / tileRows_;
+        tile->group = base_ + static_cast<uint32_t>(lane);
+        tile->row0 = begin;
+        if (pieces == 1u) {  // a decoding batch's case, where each division shows
+            tile->across = t - (__shfl_sync(0xFFFFFFFFu, inclusive_, lane) - across_);
+            tile->count = size;
+            return true;
+        }
         const uint32_t local = t - (__shfl_sync(0xFFFFFFFFu, inclusive_, lane) - pieces * across_);
         // Bands of eight pieces, all tiles across for each: the tiles that run at one time share their operands
         // (a wave of 148 tiles reads about 8 + 19 different ones), also in a group far larger than the L2 cache.
@@ -59,7 +66,6 @@ public:
         const uint32_t piece = band * kBand + inBand % width;
         const uint32_t length = ((size + pieces - 1u) / pieces + 15u) / 16u * 16u;
         const uint32_t from = piece * length < size ? piece * length : size;
-        tile->group = base_ + static_cast<uint32_t>(lane);
         tile->across = inBand / width;
         tile->row0 = begin + from;
         tile->count = size - from < length ? size - from : length;

@@ -3,13 +3,16 @@
  * kernel works on, in order.  One warp of each CTA asks and tells the others
  * through shared memory.
  *
- * A tile is (128 per CTA) x tileColumns results; its summed index is cut into blocks of
- * 128 bytes.  Forward products run whole tiles in waves of one per worker, and what
- * is left after the last full wave is split along the summed index over all of them
- * where that saves more time than joining the partial sums costs.  Weight
- * gradients, whose tiles differ in length with their groups, run whole tiles
- * round robin when there are many and are split into equal runs of blocks when
- * there are few.
+ * A tile is (128 per CTA) x tileColumns results; its summed index is cut into blocks
+ * of 128 bytes.  Forward products run whole tiles in waves of one per worker; the
+ * tiles left after the last full wave are each split along the summed index into as
+ * many equal parts as there are workers for them, where that saves more time than
+ * joining the parts' sums costs.  Weight gradients, whose tiles differ in length with
+ * their groups, are split where there are few of them, into parts of about the same
+ * length.  A tile's parts are equal and start together, so that they also end
+ * together: with runs of blocks that ignore the tiles' borders every worker is busy to
+ * the last, but one that begins a tile after the end of another arrives late, alone,
+ * and the others' sums wait for it (512 x 512 from 16384 rows: 73 us).
  */
 #ifndef ACLSPARSE_B200_GROUPED_SCHEDULE_CUH_
 #define ACLSPARSE_B200_GROUPED_SCHEDULE_CUH_
@@ -24,8 +27,10 @@ namespace aclsp {
 constexpr uint32_t kTileLanes = 128;      // results along the first operand per CTA: lanes of tensor memory
 constexpr uint32_t kGroupedMaxCtas = 148;
 constexpr uint32_t kMinSplitBlocks = 4;   // shortest run of blocks worth a worker of its own
-constexpr uint32_t kWholeTileWaves = 4;   // gradient: with this many tiles per worker nothing is split
-constexpr uint32_t kGroupedCounters = kWholeTileWaves * kGroupedMaxCtas;
+constexpr uint32_t kWholeTileWaves = 2;   // gradient: with this many tiles per worker nothing is split
+// A counter per quarter of a tile's lanes in a CTA and sixteen of its columns.
+constexpr uint32_t kTileCounters = 4u * 256u / 16u;
+constexpr uint32_t kGroupedCounters = kWholeTileWaves * kGroupedMaxCtas * kTileCounters;
 
 struct Segment {
     uint32_t group;
@@ -36,11 +41,10 @@ struct Segment {
     uint32_t columns;   // results along the other dimension
     uint32_t block0;    // blocks [block0, block1) of the summed index
     uint32_t block1;
-    uint32_t parts;     // workers that share the tile; 1: the result is complete here
-    uint32_t counter;   // parts > 1: the tile's counter,
-    uint32_t firstWorker;  // its first worker, whose partial sums are in slot firstSlot; worker w's after it in slot 2 * w
-    uint32_t firstSlot;
-    uint32_t slot;      // this worker's slot
+    uint32_t parts;     // parts of the tile; 1: the result is complete here
+    uint32_t part;      // which one this is
+    uint32_t slot;      // parts > 1: where its sums are left; those of the tile's other parts lie around it, in order
+    uint32_t counter;   // and the tile's counters
 };
 
 struct Workers {
@@ -48,58 +52,52 @@ struct Workers {
     uint32_t count;
 };
 
-// The workers that share units [start, start + length) of runs of `per` units each.
-__device__ __forceinline__ void SetParts(Segment* s, const Workers& w, uint32_t start, uint32_t length, uint32_t per,
-                                         uint32_t counter)
-{
-    s->firstWorker = start / per;
-    s->parts = (start + length - 1u) / per - s->firstWorker + 1u;
-    // a worker's run holds two partial tiles at most: one that it continues (slot 0) and one that it begins (slot 1)
-    s->firstSlot = 2u * s->firstWorker + (s->firstWorker * per < start ? 1u : 0u);
-    s->slot = w.index == s->firstWorker ? s->firstSlot : 2u * w.index;
-    s->counter = counter;
-}
-
 class ForwardSchedule {
 public:
     __device__ __forceinline__ ForwardSchedule(const AclspGroupedParams& p, Workers workers, uint32_t tileLanes,
                                                uint32_t tileRows, uint32_t blocks, uint32_t joinBlocks)
         : walk_(p.offsets, p.groups, p.rows, tileRows, (p.n + tileLanes - 1u) / tileLanes), workers_(workers),
-          tileLanes_(tileLanes), blocks_(blocks)
+          tileLanes_(tileLanes), blocks_(blocks), length_(blocks)
     {
-        const uint32_t tiles = walk_.Count();
+        tiles_ = walk_.Count();
         walk_.Restart();
-        waves_ = tiles / workers_.count;
-        const uint32_t units = (tiles - waves_ * workers_.count) * blocks;
-        per_ = (units + workers_.count - 1u) / workers_.count;
-        per_ = per_ > kMinSplitBlocks ? per_ : kMinSplitBlocks;
-        per_ = per_ + joinBlocks < blocks ? per_ : blocks;
-        unit_ = workers_.index * per_ < units ? workers_.index * per_ : units;
-        unitEnd_ = unit_ + per_ < units ? unit_ + per_ : units;
+        tile_ = workers.index;
+        whole_ = tiles_ / workers.count * workers.count;
+        const uint32_t left = tiles_ - whole_;
+        if (left != 0u && 2u * left <= workers.count && blocks > kMinSplitBlocks + joinBlocks) {
+            const uint32_t parts = workers.count / left;
+            const uint32_t length = (blocks + parts - 1u) / parts;
+            length_ = length > kMinSplitBlocks ? length : kMinSplitBlocks;
+            length_ = length_ + joinBlocks < blocks ? length_ : blocks;
+        }
+        parts_ = length_ < blocks ? (blocks + length_ - 1u) / length_ : 1u;
     }
 
     __device__ __forceinline__ bool Next(Segment* s)
     {
-        uint32_t t;
+        uint32_t t = tile_;
         s->block0 = 0;
         s->block1 = blocks_;
         s->parts = 1;
-        if (wave_ < waves_) {
-            t = wave_ * workers_.count + workers_.index;
-            ++wave_;
-        } else {
-            if (unit_ >= unitEnd_) {
+        s->part = 0;
+        if (t >= whole_ && parts_ > 1u) {
+            // the parts of what is left of the tiles, one per worker
+            const uint32_t local = workers_.index / parts_;
+            t = whole_ + local;
+            if (done_ || t >= tiles_) {
                 return false;
             }
-            const uint32_t local = unit_ / blocks_;
-            const uint32_t start = local * blocks_;
-            t = waves_ * workers_.count + local;
-            s->block0 = unit_ - start;
-            const uint32_t until = s->block0 + (unitEnd_ - unit_);
-            s->block1 = until < blocks_ ? until : blocks_;
-            unit_ += s->block1 - s->block0;
-            SetParts(s, workers_, start, blocks_, per_, local);
+            done_ = true;
+            s->parts = parts_;
+            s->part = workers_.index - local * parts_;
+            s->slot = workers_.index;
+            s->counter = local;
+            s->block0 = s->part * length_;
+            s->block1 = s->block0 + length_ < blocks_ ? s->block0 + length_ : blocks_;
+        } else if (t >= tiles_) {
+            return false;
         }
+        tile_ += workers_.count;
         GroupTile tile;
         if (!walk_.Find(t, &tile)) {
             return false;
@@ -118,94 +116,117 @@ private:
     Workers workers_;
     uint32_t tileLanes_;
     uint32_t blocks_;
-    uint32_t waves_;
-    uint32_t wave_ = 0;
-    uint32_t per_;
-    uint32_t unit_;
-    uint32_t unitEnd_;
+    uint32_t length_;  // of a part
+    uint32_t parts_;
+    uint32_t tiles_;
+    uint32_t whole_;   // tiles in full waves
+    uint32_t tile_;
+    bool done_ = false;
 };
 
 class GradientSchedule {
 public:
     __device__ __forceinline__ GradientSchedule(const AclspGroupedParams& p, Workers workers, uint32_t tileLanes,
-                                                uint32_t tileColumns, uint32_t blockRows)
-        : workers_(workers), tileLanes_(tileLanes), offsets_(p.offsets), groups_(p.groups), rows_(p.rows), n_(p.n), tileColumns_(tileColumns), blockRows_(blockRows),
-          across_((p.n + tileColumns - 1u) / tileColumns), perGroup_(across_ * ((p.m + tileLanes - 1u) / tileLanes))
+                                                uint32_t tileColumns, uint32_t blockRows, uint32_t joinBlocks)
+        : workers_(workers), tileLanes_(tileLanes), offsets_(p.offsets), groups_(p.groups), rows_(p.rows), n_(p.n),
+          tileColumns_(tileColumns), blockRows_(blockRows), across_((p.n + tileColumns - 1u) / tileColumns),
+          perGroup_(across_ * ((p.m + tileLanes - 1u) / tileLanes))
     {
-        total_ = groups_ * perGroup_;
-        split_ = total_ < kWholeTileWaves * workers_.count;
-        tile_ = workers_.index;
-        if (split_) {
-            Load();
-            while (base_ + 32u < groups_) {
-                base_ += 32u;
-                Load();
-            }
-            const uint32_t units = end_;
-            per_ = (units + workers_.count - 1u) / workers_.count;
-            per_ = per_ > kMinSplitBlocks ? per_ : kMinSplitBlocks;
-            unit_ = workers_.index * per_ < units ? workers_.index * per_ : units;
-            unitEnd_ = unit_ + per_ < units ? unit_ + per_ : units;
-            if (base_ != 0u) {
-                base_ = 0;
-                end_ = 0;
-                Load();
+        const uint32_t tiles = groups_ * perGroup_;
+        next_ = workers_.index;
+        // Few tiles: the shortest parts that make no more of them than the workers take in one turn (in two, where
+        // there are more tiles than workers).
+        if (tiles < kWholeTileWaves * workers_.count) {
+            const uint32_t most = tiles <= workers_.count ? workers_.count : kWholeTileWaves * workers_.count;
+            uint32_t longest = 0;
+            uint32_t all = 0;
+            Sum(1u, &all, &longest);
+            uint32_t length = (all + workers_.count - 1u) / workers_.count;
+            length = length > kMinSplitBlocks ? length : kMinSplitBlocks;
+            if (length + joinBlocks < longest) {
+                uint32_t unused;
+                uint32_t parts;
+                for (;;) {
+                    Sum(length, &parts, &unused);
+                    if (parts <= most || length >= longest) {
+                        break;
+                    }
+                    length += length / 8u + 1u;
+                }
+                length_ = length;
             }
         }
+        Load();
     }
 
     __device__ __forceinline__ bool Next(Segment* s)
     {
-        uint32_t inGroup;
-        s->parts = 1;
-        if (!split_) {
-            if (tile_ >= total_) {
+        while (next_ >= end_) {
+            if (base_ + 32u >= groups_) {
                 return false;
             }
-            s->group = tile_ / perGroup_;
-            inGroup = tile_ % perGroup_;
-            tile_ += workers_.count;
-            uint32_t last;
-            GroupRows(offsets_, s->group, rows_, &s->row0, &last);
-            s->rows = last - s->row0;
-            s->block0 = 0;
-            s->block1 = (s->rows + blockRows_ - 1u) / blockRows_;
-        } else {
-            if (unit_ >= unitEnd_) {
-                return false;
-            }
-            while (unit_ >= end_ && base_ + 32u < groups_) {
-                base_ += 32u;
-                Load();
-            }
-            const uint32_t ballot = __ballot_sync(0xFFFFFFFFu, unit_ < inclusive_);
-            const int lane = __ffs(static_cast<int>(ballot)) - 1;
-            s->group = base_ + static_cast<uint32_t>(lane);
-            s->row0 = __shfl_sync(0xFFFFFFFFu, begin_, lane);
-            s->rows = __shfl_sync(0xFFFFFFFFu, size_, lane);
-            const uint32_t blocks = (s->rows + blockRows_ - 1u) / blockRows_;
-            const uint32_t units = blocks > 0u ? blocks : 1u;
-            const uint32_t first = __shfl_sync(0xFFFFFFFFu, inclusive_, lane) - units * perGroup_;
-            inGroup = (unit_ - first) / units;
-            const uint32_t start = first + inGroup * units;
-            s->block0 = unit_ - start;
-            const uint32_t until = s->block0 + (unitEnd_ - unit_);
-            s->block1 = until < units ? until : units;
-            unit_ += s->block1 - s->block0;
-            if (blocks == 0u) {
-                s->block1 = 0;  // an empty group: beta * C
-            } else {
-                SetParts(s, workers_, start, units, per_, s->group * perGroup_ + inGroup);
-            }
+            base_ += 32u;
+            Load();
         }
-        s->left = inGroup / across_ * tileLanes_;
-        s->right = inGroup % across_ * tileColumns_;
+        const uint32_t ballot = __ballot_sync(0xFFFFFFFFu, next_ < inclusive_);
+        const int lane = __ffs(static_cast<int>(ballot)) - 1;
+        s->group = base_ + static_cast<uint32_t>(lane);
+        s->row0 = __shfl_sync(0xFFFFFFFFu, begin_, lane);
+        s->rows = __shfl_sync(0xFFFFFFFFu, size_, lane);
+        const uint32_t blocks = (s->rows + blockRows_ - 1u) / blockRows_;
+        const uint32_t parts = Parts(blocks, length_);
+        const uint32_t inGroup = next_ - (__shfl_sync(0xFFFFFFFFu, inclusive_, lane) - parts * perGroup_);
+        const uint32_t tile = inGroup / parts;
+        s->parts = parts;
+        s->part = inGroup - tile * parts;
+        s->slot = next_;
+        s->counter = s->group * perGroup_ + tile;
+        const uint32_t length = (blocks + parts - 1u) / parts;
+        s->block0 = s->part * length < blocks ? s->part * length : blocks;
+        s->block1 = s->block0 + length < blocks ? s->block0 + length : blocks;
+        s->left = tile / across_ * tileLanes_;
+        s->right = tile % across_ * tileColumns_;
         s->columns = n_ - s->right < tileColumns_ ? n_ - s->right : tileColumns_;
+        next_ += workers_.count;
         return true;
     }
 
 private:
-    // Units of 32 groups: a group has perGroup_ tiles of as many units as its rows make blocks, an empty one of one.
+    // Parts of a tile: none longer than `length`, and none empty.  An empty group's tile is one part of no blocks.
+    static __device__ __forceinline__ uint32_t Parts(uint32_t blocks, uint32_t length)
+    {
+        if (blocks <= length) {
+            return 1u;
+        }
+        const uint32_t parts = (blocks + length - 1u) / length;
+        const uint32_t even = (blocks + parts - 1u) / parts;
+        return (blocks + even - 1u) / even;
+    }
+
+    __device__ __forceinline__ uint32_t Blocks(uint32_t g, uint32_t* first, uint32_t* size) const
+    {
+        uint32_t last;
+        GroupRows(offsets_, g, rows_, first, &last);
+        *size = last - *first;
+        return (*size + blockRows_ - 1u) / blockRows_;
+    }
+
+    // All groups' parts of this length, and the longest group's blocks; with length 1 the parts are blocks.
+    __device__ __forceinline__ void Sum(uint32_t length, uint32_t* parts, uint32_t* longest) const
+    {
+        uint32_t sum = 0;
+        uint32_t top = 0;
+        for (uint32_t g = threadIdx.x % 32u; g < groups_; g += 32u) {
+            uint32_t first, size;
+            const uint32_t blocks = Blocks(g, &first, &size);
+            sum += perGroup_ * Parts(blocks, length);
+            top = blocks > top ? blocks : top;
+        }
+        *parts = __reduce_add_sync(0xFFFFFFFFu, sum);
+        *longest = __reduce_max_sync(0xFFFFFFFFu, top);
+    }
+
+    // The parts of 32 groups, numbered.
     __device__ __forceinline__ void Load()
     {
         const uint32_t lane = threadIdx.x % 32u;
@@ -214,11 +235,7 @@ private:
         size_ = 0;
         uint32_t sum = 0;
         if (g < groups_) {
-            uint32_t last;
-            GroupRows(offsets_, g, rows_, &begin_, &last);
-            size_ = last - begin_;
-            const uint32_t blocks = (size_ + blockRows_ - 1u) / blockRows_;
-            sum = perGroup_ * (blocks > 0u ? blocks : 1u);
+            sum = perGroup_ * Parts(Blocks(g, &begin_, &size_), length_);
         }
         for (int d = 1; d < 32; d *= 2) {
             const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
@@ -238,12 +255,8 @@ private:
     uint32_t blockRows_;
     uint32_t across_;
     uint32_t perGroup_;
-    uint32_t total_;
-    bool split_;
-    uint32_t tile_;
-    uint32_t per_ = 1;
-    uint32_t unit_ = 0;
-    uint32_t unitEnd_ = 0;
+    uint32_t length_ = 0xFFFFFFFFu;  // longest part
+    uint32_t next_;                  // number of the next part
     uint32_t base_ = 0;
     uint32_t end_ = 0;
     uint32_t begin_ = 0;

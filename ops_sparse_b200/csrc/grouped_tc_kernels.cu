@@ -21,9 +21,12 @@
  * half of tensor memory.  Warp 3 works out the next tiles ahead of all of them, and
  * warp 2 cuts the ends of groups off; done by the MMA warp itself either left the
  * tensor cores idle for 600 cycles per tile.  Tiles that do not fill a wave are split along the summed
- * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and the one
- * that arrives last adds them in the CTAs' order, so that the result does not
- * depend on who that is.
+ * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and for each
+ * piece of the tile, 32 lanes x 16 columns, the warp that arrives last adds them in
+ * the CTAs' order, so that the result does not depend on who that is.  CTAs go
+ * through the pieces from different ones on: arriving together, each is the last one
+ * for some, and the adding is shared (512 x 512 from 16384 rows, 19 CTAs to a tile:
+ * 62 us with one CTA adding a whole tile).
  *
  * Operands whose rows do not start on multiples of 16 bytes (odd widths) cannot be loaded by TMA: they are copied to
  * rows that do first (grouped_kernels.cu), in the buffer.  Warps that bring such rows into shared memory themselves,
@@ -243,13 +246,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint64_t segmentFull[kSegments];
     __shared__ uint64_t segmentEmpty[kSegments];
     __shared__ Segment segments[kSegments];
-    __shared__ uint64_t joined;     // the result warps meet here
     __shared__ uint64_t drained;
     __shared__ uint64_t cutFull[R::kStages];  // a block whose last rows are to be cut off has landed in this CTA
     __shared__ uint64_t cutDone[R::kStages];  // first CTA: a block's last rows are cut off, in both CTAs
     __shared__ uint32_t tmemAddress;
     __shared__ uint32_t gaveUp;
-    __shared__ uint32_t isLast;
 
     const uint32_t warp = threadIdx.x / 32u;
     const uint32_t lane = threadIdx.x % 32u;
@@ -271,7 +272,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             BarInit(SmemAddress(segmentFull + i), 1);
             BarInit(SmemAddress(segmentEmpty + i), 1u + kResultWarps + (rank == 0u ? 1u : 0u) + (kGradient ? 1u : 0u));
         }
-        BarInit(SmemAddress(&joined), kResultWarps);
         BarInit(SmemAddress(&drained), 1);
         gaveUp = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 3) {
         auto schedule = [&]() {
             if constexpr (kGradient) {
-                return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock);
+                return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock, joinBlocks);
             } else {
                 return ForwardSchedule(p, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
             }
@@ -531,15 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kSlotVectors = kTileLanes * kColumns / 4u;
         Segment s;
         uint32_t tile = 0;
-        uint32_t meetings = 0;
-        // The result warps meet; bounded like every wait.
-        auto meet = [&]() {
-            __syncwarp();
-            if (lane == 0) {
-                BarArrive(SmemAddress(&joined));
-            }
-            return __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(&joined), meetings++ & 1u, stop)) != 0;
-        };
         // This warp has read its share of the sums: the tensor memory may be written again.
         auto release = [&](uint32_t half) {
             TmemFenceBefore();
@@ -598,29 +589,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             release(half);
             __threadfence();
-            if (!meet()) {
-                break;
-            }
-            if (threadIdx.x == 128u) {
-                uint32_t* const counter = counters + s.counter * kCtas + rank;
-                const uint32_t before = atomicAdd(counter, 1u);
-                isLast = before + 1u == s.parts ? 1u : 0u;
-                if (before + 1u == s.parts) {
-                    *counter = 0;  // clear for the next product
+            __syncwarp();
+            const uint32_t pieces = s.columns > firstChunk ? (s.columns - firstChunk + kChunkStep - 1u) / kChunkStep : 0u;
+            uint32_t* const tileCounters = counters + (s.counter * kCtas + rank) * kTileCounters + warp % 4u;
+            for (uint32_t i = 0; i < pieces; ++i) {
+                const uint32_t j0 = firstChunk + (s.part + i) % pieces * kChunkStep;
+                uint32_t before = 0;
+                if (lane == 0) {
+                    before = atomicAdd(tileCounters + j0 / 16u * 4u, 1u);
+                }
+                before = __shfl_sync(0xFFFFFFFFu, before, 0);
+                if (before + 1u != s.parts) {
+                    continue;
+                }
+                if (lane == 0) {
+                    tileCounters[j0 / 16u * 4u] = 0;  // clear for the next product
                 }
                 __threadfence();
-            }
-            if (!meet()) {
-                break;
-            }
-            if (isLast == 0u) {
-                continue;
-            }
-            __threadfence();
-            for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
                 const uint4* at = partials + tmemLane + j0 / 4u * kTileLanes;
                 auto part = [&](uint32_t i, uint4 (&v)[4]) {
-                    const uint32_t slot = i == 0u ? s.firstSlot : 2u * (s.firstWorker + i);
+                    const uint32_t slot = s.slot - s.part + i;
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         v[j] = __ldcg(at + static_cast<size_t>(slot * kCtas + rank) * kSlotVectors + j * kTileLanes);
@@ -637,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     total[4 * j + 3] = v[j].w;
                 }
 #pragma unroll 4
-                for (uint32_t i = 1; i < s.parts; ++i) {
-                    part(i, v);
+                for (uint32_t k = 1; k < s.parts; ++k) {
+                    part(k, v);
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         total[4 * j] = AddSums<kInt8>(total[4 * j], v[j].x);
