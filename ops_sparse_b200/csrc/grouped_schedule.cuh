@@ -134,27 +134,17 @@ public:
     {
         const uint32_t tiles = groups_ * perGroup_;
         next_ = workers_.index;
-        // Few tiles: the shortest parts that make no more of them than the workers take in one turn (in two, where
+        // Few tiles: parts so short that there are just no more of them than the workers take in one turn (in two, where
         // there are more tiles than workers).
         if (tiles < kWholeTileWaves * workers_.count) {
             const uint32_t most = tiles <= workers_.count ? workers_.count : kWholeTileWaves * workers_.count;
-            uint32_t longest = 0;
-            uint32_t all = 0;
-            Sum(1u, &all, &longest);
-            uint32_t length = (all + workers_.count - 1u) / workers_.count;
+            uint32_t longest;
+            uint32_t all;
+            Sum(&all, &longest);
+            // ceil(blocks / length) summed over the tiles is at most all / length + tiles
+            uint32_t length = most > tiles ? (all + most - tiles - 1u) / (most - tiles) : longest;
             length = length > kMinSplitBlocks ? length : kMinSplitBlocks;
-            if (length + joinBlocks < longest) {
-                uint32_t unused;
-                uint32_t parts;
-                for (;;) {
-                    Sum(length, &parts, &unused);
-                    if (parts <= most || length >= longest) {
-                        break;
-                    }
-                    length += length / 8u + 1u;
-                }
-                length_ = length;
-            }
+            length_ = length + joinBlocks < longest ? length : length_;
         }
         Load();
     }
@@ -211,18 +201,18 @@ private:
         return (*size + blockRows_ - 1u) / blockRows_;
     }
 
-    // All groups' parts of this length, and the longest group's blocks; with length 1 the parts are blocks.
-    __device__ __forceinline__ void Sum(uint32_t length, uint32_t* parts, uint32_t* longest) const
+    // The blocks of all tiles, and the longest tile's.
+    __device__ __forceinline__ void Sum(uint32_t* blocks, uint32_t* longest) const
     {
         uint32_t sum = 0;
         uint32_t top = 0;
         for (uint32_t g = threadIdx.x % 32u; g < groups_; g += 32u) {
             uint32_t first, size;
-            const uint32_t blocks = Blocks(g, &first, &size);
-            sum += perGroup_ * Parts(blocks, length);
-            top = blocks > top ? blocks : top;
+            const uint32_t own = Blocks(g, &first, &size);
+            sum += perGroup_ * own;
+            top = own > top ? own : top;
         }
-        *parts = __reduce_add_sync(0xFFFFFFFFu, sum);
+        *blocks = __reduce_add_sync(0xFFFFFFFFu, sum);
         *longest = __reduce_max_sync(0xFFFFFFFFu, top);
     }
 

@@ -289,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     TmemFenceAfter();
     const uint32_t tmem = tmemAddress;
-    WaitForPreviousKernel();
-    LetNextKernelStart();
+    LetNextKernelStart();  // each warp waits for the previous one itself, before it touches global memory
     volatile uint32_t* const stop = &gaveUp;
 
     // The next segment of the schedule, for one of the warps that follow it; parts == 0 ends it.
@@ -327,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         constexpr uint32_t kBox = kGradient ? 64u : R::kBox;
+        WaitForPreviousKernel();
         Segment s;
         uint32_t stage = 0;
         uint32_t parity = 0;
@@ -498,6 +498,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             block += count;
         }
     } else if (warp == 3) {
+        if (p.offsets != nullptr) {  // without them the schedule needs nothing from memory
+            WaitForPreviousKernel();
+        }
         auto schedule = [&]() {
             if constexpr (kGradient) {
                 return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock, joinBlocks);
@@ -521,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp >= 4) {
+        WaitForPreviousKernel();
         const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
         const float beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
         const uint32_t tmemLane = threadIdx.x % 128u;
@@ -591,48 +595,56 @@ __global__ void __launch_bounds__(kThreads, 1)
             __threadfence();
             __syncwarp();
             const uint32_t pieces = s.columns > firstChunk ? (s.columns - firstChunk + kChunkStep - 1u) / kChunkStep : 0u;
+            uint32_t lasts = 0;
             uint32_t* const tileCounters = counters + (s.counter * kCtas + rank) * kTileCounters + warp % 4u;
+            // Two pieces at a time, from one that differs from part to part on.
             for (uint32_t i = 0; i < pieces; ++i) {
-                const uint32_t j0 = firstChunk + (s.part + i) % pieces * kChunkStep;
-                uint32_t before = 0;
-                if (lane == 0) {
-                    before = atomicAdd(tileCounters + j0 / 16u * 4u, 1u);
+                const uint32_t inTwo = i % 2u;
+                const uint32_t j0 = firstChunk + (2u * s.part + i) % pieces * kChunkStep;
+                if (inTwo == 0u) {
+                    bool last = false;
+                    if (lane < 2u && i + lane < pieces) {
+                        uint32_t* const counter =
+                            tileCounters + (firstChunk + (2u * s.part + i + lane) % pieces * kChunkStep) / 16u * 4u;
+                        last = atomicAdd(counter, 1u) + 1u == s.parts;
+                        if (last) {
+                            *counter = 0;  // clear for the next product
+                        }
+                    }
+                    lasts = __ballot_sync(0xFFFFFFFFu, last);
+                    if (lasts != 0u) {
+                        __threadfence();
+                    }
                 }
-                before = __shfl_sync(0xFFFFFFFFu, before, 0);
-                if (before + 1u != s.parts) {
+                if ((lasts >> inTwo & 1u) == 0u) {
                     continue;
                 }
-                if (lane == 0) {
-                    tileCounters[j0 / 16u * 4u] = 0;  // clear for the next product
-                }
-                __threadfence();
-                const uint4* at = partials + tmemLane + j0 / 4u * kTileLanes;
-                auto part = [&](uint32_t i, uint4 (&v)[4]) {
-                    const uint32_t slot = s.slot - s.part + i;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        v[j] = __ldcg(at + static_cast<size_t>(slot * kCtas + rank) * kSlotVectors + j * kTileLanes);
-                    }
-                };
+                const uint4* const at = partials + tmemLane + j0 / 4u * kTileLanes;
                 uint32_t total[16];
-                uint4 v[4];
-                part(0, v);
+                for (uint32_t k = 0; k < s.parts; k += 4u) {
+                    uint4 v[4][4];  // four parts under way together
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    total[4 * j] = v[j].x;
-                    total[4 * j + 1] = v[j].y;
-                    total[4 * j + 2] = v[j].z;
-                    total[4 * j + 3] = v[j].w;
-                }
-#pragma unroll 4
-                for (uint32_t k = 1; k < s.parts; ++k) {
-                    part(k, v);
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        if (k + q < s.parts) {
+                            const uint32_t slot = (s.slot - s.part + k + q) * kCtas + rank;
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        total[4 * j] = AddSums<kInt8>(total[4 * j], v[j].x);
-                        total[4 * j + 1] = AddSums<kInt8>(total[4 * j + 1], v[j].y);
-                        total[4 * j + 2] = AddSums<kInt8>(total[4 * j + 2], v[j].z);
-                        total[4 * j + 3] = AddSums<kInt8>(total[4 * j + 3], v[j].w);
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                v[q][j] = __ldcg(at + static_cast<size_t>(slot) * kSlotVectors + j * kTileLanes);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        if (k + q < s.parts) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                const uint32_t w[4] = {v[q][j].x, v[q][j].y, v[q][j].z, v[q][j].w};
+#pragma unroll
+                                for (uint32_t e = 0; e < 4; ++e) {
+                                    total[4 * j + e] = k + q == 0u ? w[e] : AddSums<kInt8>(total[4 * j + e], w[e]);
+                                }
+                            }
+                        }
                     }
                 }
                 Lane16 sums;
