@@ -158,7 +158,7 @@ aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t handle, con
                                                    void* externalBuffer);
 
 /* Rows of a matrix in 8 bits with one scale each, the operand of the int8 product above:
- *     scales[r] = max_k |X[r, k]| / 127   (fp32, correctly rounded),
+ *     scales[r] = max_k |X[r, k]| * (1 / 127)   (in fp32, 1 / 127 being its nearest fp32 number),
  *     Q[r, k]   = X[r, k] / scales[r], the exact quotient rounded to the nearest integer, ties to even
  * (and held to +-127, which only matters where the scale is subnormal).
  * matX fp32, fp16 or bf16, matQ int8, both rows x cols, row-major with any leading dimension; scales: DEVICE array of

@@ -383,7 +383,7 @@ class GroupedMMWeightGrad(_Grouped):
 
 
 class QuantizeRows:
-    """scales[r] = max|X[r]| / 127 and Q[r] = X[r] / scales[r] in int8, rounded to the nearest integer, ties to even."""
+    """scales[r] = max|X[r]| * (1 / 127) in fp32 and Q[r] = X[r] / scales[r] in int8, rounded to the nearest integer, ties to even."""
 
     def __init__(self, handle: Handle, x: DnMat, q: DnMat, scales):
         _device_array("scales", scales, torch.float32, x.rows)

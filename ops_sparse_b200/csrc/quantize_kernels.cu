@@ -1,5 +1,5 @@
 /*
- * Rows in 8 bits: scale s = max|x| / 127 of every row, q = x / s to the nearest
+ * Rows in 8 bits: scale s = max|x| * (1/127) of every row, q = x / s to the nearest
  * integer, ties to even.
  *
  * The quotient that is rounded is the exact one, not an fp32 value of it: next to a
@@ -115,7 +115,7 @@ struct RowScale {
 
     __device__ __forceinline__ explicit RowScale(float top)
     {
-        scale = __fdiv_rn(top, 127.0f);
+        scale = top * (1.0f / 127.0f);
         zeros = !(scale > 0.0f && scale <= 3.402823466e38f);
         small = scale < kSmallestScale;
         inverse = __fdiv_rn(1.0f, scale);

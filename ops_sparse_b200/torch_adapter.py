@@ -355,7 +355,8 @@ def int8_mm(x: torch.Tensor, weight: torch.Tensor, x_scales: torch.Tensor, w_sca
 
 
 def quantize_rows(x: torch.Tensor) -> "tuple[torch.Tensor, torch.Tensor]":
-    """int8 rows ``q`` and float32 ``scales`` with ``x[r]`` close to ``scales[r] * q[r]``: scales[r] = max|x[r]| / 127.
+    """int8 rows ``q`` and float32 ``scales`` with ``x[r]`` close to ``scales[r] * q[r]``: scales[r] = max|x[r]| / 127
+    (as the fp32 product with the fp32 number nearest to 1 / 127).
 
     Rows are rounded to the nearest integer, ties to even; a row with an infinity or a NaN gets zeros and that scale.
     """

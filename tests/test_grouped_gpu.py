@@ -411,7 +411,8 @@ def test_gradient_is_repeatable_and_captures():
 # ---- rows in 8 bits ----
 
 def quantized(x):
-    scale = (x.double().abs().amax(dim=1) / 127).float()
+    # the product of two fp32 numbers is exact in 64 bits: rounded once
+    scale = (x.double().abs().amax(dim=1) * torch.tensor(1 / 127, dtype=torch.float32).double()).float()
     ratio = x.double() / torch.where(scale == 0, torch.ones_like(scale), scale).double()[:, None]
     return torch.where(scale[:, None] == 0, 0.0, torch.round(ratio)).clamp(-127, 127).to(torch.int8), scale
 
@@ -443,10 +444,17 @@ def test_quantize_ties_and_near_ties():
     for s in scale.double():
         near = (halves * s).float()
         up, down = torch.nextafter(near, near.new_tensor(3e38)), torch.nextafter(near, near.new_tensor(-3e38))
-        rows.append(torch.cat([(127 * s).float().reshape(1), near, up, down]))
+        # the row's largest value: one whose scale is s, where there is one
+        tops = (127 * s).float().view(torch.int32) + torch.arange(-2, 3, device=DEV, dtype=torch.int32)
+        tops = tops.view(torch.float32)
+        fits = tops * torch.tensor(1 / 127, device=DEV, dtype=torch.float32) == s.float()
+        rows.append(torch.cat([tops[fits][:1] if fits.any() else tops[2:3], near, up, down]))
     x = torch.stack(rows)
+    assert (x.abs().amax(dim=1) == x[:, 0]).all()
     q, scales = A.quantize_rows(x)
     want, want_scales = quantized(x)
+    ratio = x.double() / want_scales.double()[:, None]
+    assert int(((2 * ratio) % 2 == 1).sum()) > 250  # ties, exactly
     assert torch.equal(scales, want_scales) and torch.equal(q, want)
 
 
