@@ -56,16 +56,20 @@ constexpr uint32_t kResultWarps = 8;  // two for each quarter of the lanes of te
 constexpr int kThreads = 128 + 32 * kResultWarps;
 constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
-constexpr uint32_t kGradientColumns = 256;
+constexpr uint32_t kRightBox = 32;  // rows of one load of a forward product's right operand
+// A warp's 32 lanes x 16 results on their way to rows of C that are not aligned: each lane's one word longer than they
+// are, so that the lanes write to different banks.
+constexpr uint32_t kTurnWarpBytes = 32u * (16u * 4u + 4u);
 constexpr uint64_t kDrainNs = 10000000ull;
 
-template <uint32_t kColumns, uint32_t kCtas>
+template <uint32_t kColumns, uint32_t kCtas, bool kGradient>
 struct Ring {
     static constexpr uint32_t kRightRows = kColumns / kCtas;  // of the right operand in one CTA
     static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
-    static constexpr uint32_t kStages = 224u * 1024u / kStageBytes;
-    static constexpr uint32_t kBytes = kStageBytes * kStages + 1024u;  // stages start on multiples of 1024
-    static constexpr uint32_t kBox = 32;                       // rows of one load of the right operand
+    static constexpr uint32_t kTurnBytes = kGradient ? kResultWarps * kTurnWarpBytes : 0u;
+    static constexpr uint32_t kStages = (224u * 1024u - kTurnBytes) / kStageBytes;
+    static constexpr uint32_t kTurn = kStageBytes * kStages;           // behind the stages: StoreGradient's room
+    static constexpr uint32_t kBytes = kTurn + kTurnBytes + 1024u;     // stages start on multiples of 1024
 };
 
 // One result in the type of C; beta == 0 does not read C.
@@ -144,14 +148,15 @@ __device__ __forceinline__ void StoreForward(const AclspGroupedParams& p, void* 
     }
 }
 
-// Gradient: the lane is a row of C_g, the sixteen values are neighbours in it.
+// Gradient: the lane is a row of C_g, the sixteen values are neighbours in it.  Called by whole warps.  Where the rows
+// are aligned, each lane writes its own in whole sectors; elsewhere (odd widths, a last column tile) the warp turns the
+// values round in shared memory and writes rows element by element, sixteen lanes to one: a lane at a time to its own row
+// would send every element to the memory by itself (2047 x 2049 from 8192 rows: 306 us).
 template <typename T>
 __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
-                                              uint32_t j0, const Lane16& sums, float laneScale, float beta)
+                                              uint32_t j0, const Lane16& sums, float laneScale, float beta, uint32_t turn)
 {
-    if (row >= p.m) {
-        return;
-    }
+    const bool hasRow = row < p.m;
     T* at = static_cast<T*>(c) + static_cast<int64_t>(s.group) * p.cBatchStride + static_cast<int64_t>(row) * p.ldc +
             s.right + j0;
     const uint32_t count = s.columns - j0 < 16u ? s.columns - j0 : 16u;
@@ -159,7 +164,7 @@ __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void*
     if (beta != 0.0f) {
 #pragma unroll
         for (uint32_t j = 0; j < 16; ++j) {
-            const float old = j < count ? ToFloat(at[j]) : 0.0f;
+            const float old = hasRow && j < count ? ToFloat(at[j]) : 0.0f;
             out[j] = FromFloat<T>(fmaf(beta, old, sums.v[j] * laneScale));
         }
     } else {
@@ -168,42 +173,64 @@ __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void*
             out[j] = FromFloat<T>(sums.v[j] * laneScale);
         }
     }
-    if (count == 16u && reinterpret_cast<uintptr_t>(at) % 16u == 0u) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(out);
-        if (reinterpret_cast<uintptr_t>(at) % 32u == 0u) {
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(out);
+    if (__all_sync(0xFFFFFFFFu, count == 16u && reinterpret_cast<uintptr_t>(at) % 16u == 0u)) {
+        if (hasRow && reinterpret_cast<uintptr_t>(at) % 32u != 0u) {
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof(out) / 16u; ++i) {
+                reinterpret_cast<uint4*>(at)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+            }
+        } else if (hasRow) {
 #pragma unroll
             for (uint32_t i = 0; i < sizeof(out) / 32u; ++i) {
                 const uint32_t eight[8] = {words[8 * i],     words[8 * i + 1], words[8 * i + 2], words[8 * i + 3],
                                            words[8 * i + 4], words[8 * i + 5], words[8 * i + 6], words[8 * i + 7]};
                 Store32(reinterpret_cast<unsigned char*>(at) + 32u * i, eight);
             }
-        } else {
+        }
+        return;
+    }
+    constexpr uint32_t kPitch = 16u * sizeof(T) + 4u;
+    const uint32_t lane = threadIdx.x % 32u;
+    __syncwarp();
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof(out) / 16u; ++i) {
-                reinterpret_cast<uint4*>(at)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+    for (uint32_t i = 0; i < sizeof(out) / 4u; ++i) {
+        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(turn + lane * kPitch + 4u * i), "r"(words[i]) : "memory");
+    }
+    __syncwarp();
+    const uint32_t column = lane % 16u;
+    T* to = at - static_cast<int64_t>(lane) * p.ldc + static_cast<int64_t>(lane / 16u) * p.ldc + column;
+    const uint32_t rowsLeft = p.m - (row - lane) > 32u || row - lane >= p.m ? (row - lane >= p.m ? 0u : 32u) : p.m - (row - lane);
+#pragma unroll 4
+    for (uint32_t r = lane / 16u; r < rowsLeft; r += 2u) {
+        if (column < count) {
+            const uint32_t address = turn + r * kPitch + column * static_cast<uint32_t>(sizeof(T));
+            if constexpr (sizeof(T) == 4) {
+                uint32_t v;
+                asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(address) : "memory");
+                *reinterpret_cast<uint32_t*>(to) = v;
+            } else {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(address) : "memory");
+                *reinterpret_cast<uint16_t*>(to) = v;
             }
         }
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) {
-            if (j < count) {
-                at[j] = out[j];
-            }
-        }
+        to += 2 * p.ldc;
     }
 }
 
 template <bool kGradient>
 __device__ __forceinline__ void StoreResults(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
-                                             uint32_t j0, const Lane16& sums, float laneScale, float beta)
+                                             uint32_t j0, const Lane16& sums, float laneScale, float beta,
+                                             uint32_t turn)
 {
     if constexpr (kGradient) {
         if (p.outType == ACLSP_TYPE_F32) {
-            StoreGradient<float>(p, c, s, row, j0, sums, laneScale, beta);
+            StoreGradient<float>(p, c, s, row, j0, sums, laneScale, beta, turn);
         } else if (p.outType == ACLSP_TYPE_F16) {
-            StoreGradient<__half>(p, c, s, row, j0, sums, laneScale, beta);
+            StoreGradient<__half>(p, c, s, row, j0, sums, laneScale, beta, turn);
         } else {
-            StoreGradient<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta);
+            StoreGradient<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta, turn);
         }
     } else {
         if (p.outType == ACLSP_TYPE_F32) {
@@ -234,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
                         const uint32_t leftMn, const uint32_t joinBlocks)
 {
-    using R = Ring<kColumns, kCtas>;
+    using R = Ring<kColumns, kCtas, kGradient>;
     constexpr uint32_t kBlock = kInt8 ? 128u : 64u;         // elements of the summed index in a block
     constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;   // and in one MMA
     constexpr uint32_t kColumnStep = 16u * kCtas;           // N of the MMA is a multiple of this
@@ -325,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp == 0) {
-        constexpr uint32_t kBox = kGradient ? 64u : R::kBox;
+        constexpr uint32_t kBox = kGradient ? 64u : kRightBox;
         WaitForPreviousKernel();
         Segment s;
         uint32_t stage = 0;
@@ -530,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tmemLane = threadIdx.x % 128u;
         const uint32_t firstChunk = (warp - 4u) / 4u * 16u;  // of the columns: warps that share lanes take turns
         constexpr uint32_t kChunkStep = kResultWarps / 4u * 16u;
+        const uint32_t turn = ring + R::kTurn + (warp - 4u) * kTurnWarpBytes;
         uint32_t* const counters = buffer + kGroupedHeaderWords;
         uint4* const partials = reinterpret_cast<uint4*>(counters + kGroupedCounters);
         constexpr uint32_t kSlotVectors = kTileLanes * kColumns / 4u;
@@ -573,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (uint32_t j = 0; j < 16; ++j) {
                         sums.v[j] = nothing ? 0.0f : SumToFloat<kInt8>(bits[j]);
                     }
-                    StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta);
+                    StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta, turn);
                 }
                 release(half);
                 continue;
@@ -652,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t j = 0; j < 16; ++j) {
                     sums.v[j] = SumToFloat<kInt8>(total[j]);
                 }
-                StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta);
+                StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta, turn);
             }
         }
     }
@@ -719,7 +747,7 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
             uint32_t leftMn, uint32_t sms, cudaStream_t s)
 {
     constexpr uint32_t kCtas = kColumns == 256u ? 2u : 1u;
-    constexpr uint32_t kBytes = Ring<kColumns, kCtas>::kBytes;
+    constexpr uint32_t kBytes = Ring<kColumns, kCtas, kGradient>::kBytes;
     auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient, kCtas>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
     AclspCountLaunches(1);
@@ -742,15 +770,43 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
 
 }  // namespace
 
+// The width of a tile.  What a choice costs is the number of turns that the workers take for all tiles times what a turn
+// takes: the blocks of the summed index at the rate that an SM gets operands from L2 (a block of a 128 x 32 tile is 20 KB,
+// of a 128 x 64 one 24 KB, of 128 x 128 32 KB; in a pair's 256 x 256 tile each CTA loads 32 KB), and the results of the
+// last turn.  The host knows the rows of an average group only; larger groups are cut into more tiles, which read the
+// dense matrix again, from L2, smaller ones leave columns unused.
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
 {
-    if (p.weightGrad != 0) {
-        return kGradientColumns;
+    struct Choice {
+        uint32_t columns;
+        uint32_t workers;
+        uint64_t block;    // relative cost of a block
+        uint64_t results;  // and of reading a tile's sums and writing its results
+    };
+    constexpr Choice kChoices[] = {{256, 74, 32, 320}, {128, 148, 32, 160}, {64, 148, 24, 100}, {32, 148, 20, 60}};
+    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    const uint64_t groups = p.groups < p.rows ? p.groups : (p.rows > 0 ? p.rows : 1u);  // that can have rows
+    const uint64_t average = (p.rows + groups - 1u) / groups;
+    const uint64_t length = p.weightGrad != 0 ? average : p.k;
+    const uint64_t blocks = (length * bytes + 127u) / 128u;
+    uint32_t best = 0;
+    uint64_t least = ~0ull;
+    for (const Choice& c : kChoices) {
+        if (p.weightGrad != 0 && c.columns < 128u) {
+            break;  // two blocks of 64 columns are the least that the gradient's loads make
+        }
+        const uint64_t lanes = kTileLanes * (c.columns == 256u ? 2u : 1u);
+        const uint64_t down = ((p.weightGrad != 0 ? p.m : p.n) + lanes - 1u) / lanes;
+        const uint64_t across = ((p.weightGrad != 0 ? p.n : average) + c.columns - 1u) / c.columns;
+        const uint64_t tiles = (p.weightGrad != 0 ? p.groups : groups) * down * across;
+        const uint64_t turns = (tiles + c.workers - 1u) / c.workers;
+        const uint64_t cost = turns * blocks * c.block + c.results * (p.weightGrad != 0 ? turns : 1u);
+        if (cost < least) {
+            least = cost;
+            best = c.columns;
+        }
     }
-    // Rows per group on average: what the host knows.  Larger groups are cut into more pieces, which read the
-    // weights again (from L2); smaller ones only leave part of the stages unused.
-    const uint64_t average = p.rows / p.groups;
-    return average <= 24u ? 32u : average <= 96u ? 128u : 256u;
+    return best;
 }
 
 AclspGroupedOperands AclspGroupedDescribe(const AclspGroupedParams& p)
@@ -827,20 +883,22 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
             !Encode(&right, p, bases[1], 2, rightSizes, rightStride, 64)) {
             return false;
         }
-        Launch<false, kGradientColumns, true>(left, right, c, buffer, p, 1u, sms, s);
+        (columns == 256u ? Launch<false, 256, true> : Launch<false, 128, true>)(left, right, c, buffer, p, 1u, sms, s);
         return true;
     }
     const uint32_t leftMn = p.bInner == 1 ? 0u : 1u;
     const uint32_t leftBox = leftMn != 0 ? static_cast<uint32_t>(128u / bytes) : kTileLanes;
     if (!Encode(&left, p, bases[0], 3, leftSizes, leftStrides, leftBox) ||
-        !Encode(&right, p, bases[1], 2, rightSizes, rightStride, Ring<256, 2>::kBox)) {
+        !Encode(&right, p, bases[1], 2, rightSizes, rightStride, kRightBox)) {
         return false;
     }
     const bool int8 = p.inType == ACLSP_TYPE_I8;
     auto run = int8 ? (columns == 32u    ? Launch<true, 32, false>
+                       : columns == 64u  ? Launch<true, 64, false>
                        : columns == 128u ? Launch<true, 128, false>
                                          : Launch<true, 256, false>)
                     : (columns == 32u    ? Launch<false, 32, false>
+                       : columns == 64u  ? Launch<false, 64, false>
                        : columns == 128u ? Launch<false, 128, false>
                                          : Launch<false, 256, false>);
     run(left, right, c, buffer, p, leftMn, sms, s);
