@@ -19,6 +19,7 @@
 #include "grouped_schedule.cuh"
 #include "grouped_tc.h"
 #include "plan_kernels.h"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -173,50 +174,76 @@ __device__ __forceinline__ uint32_t WordOf(const unsigned char* at, const unsign
 constexpr uint32_t kCopyThreads = 256;
 constexpr uint32_t kCopyWords = 4;  // words of a row that a lane has under way
 
-// A warp per stretch of kCopyWords * 128 bytes of a row: it reads aligned words, also the one behind each (from L1 or a
-// neighbour's line), shifts the bytes into place and writes aligned words, the last of a row with what lies behind it.
-// Bound by HBM: every byte is read and written once.
-__global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const unsigned char* __restrict__ src,
-                                                               unsigned char* __restrict__ dst, uint32_t rows,
-                                                               uint32_t batches, int64_t rowBytes, int64_t pitch,
-                                                               int64_t batchPitch, int64_t dstPitch, int64_t dstBatchPitch,
-                                                               const int32_t* offsets, uint32_t offsetRows)
+// Rows to copy, in bytes.
+struct CopyJob {
+    const unsigned char* src;
+    unsigned char* dst;
+    uint32_t rows;
+    uint32_t batches;
+    int64_t rowBytes;
+    int64_t pitch;
+    int64_t batchPitch;
+    int64_t dstPitch;
+    int64_t dstBatchPitch;
+};
+struct CopyJobs {
+    CopyJob job[2];
+};
+
+// A warp per row: it reads aligned words, also the one behind each (from L1 or a neighbour's line), shifts the bytes
+// into place and writes aligned words, the last of a row with what lies behind it.  Bound by HBM: every byte is read and
+// written once.  One launch for both operands: blockIdx.y is the job.
+__global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const CopyJobs jobs, const int32_t* offsets,
+                                                               uint32_t offsetRows)
 {
+    aclsp::WaitForPreviousKernel();
+    aclsp::LetNextKernelStart();
+    const CopyJob& c = jobs.job[blockIdx.y];
     const uint32_t lane = threadIdx.x % 32u;
-    const uint32_t stretches = static_cast<uint32_t>((dstPitch + kCopyWords * 128 - 1) / (kCopyWords * 128));
-    const int64_t perBatch = static_cast<int64_t>(rows) * stretches;
-    const int64_t all = perBatch * batches;
-    const unsigned char* const end = src + (batches - 1) * batchPitch + (rows - 1) * pitch + rowBytes;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kCopyThreads / 32u);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kCopyThreads / 32u) + threadIdx.x / 32u; i < all; i += warps) {
-        const uint32_t batch = static_cast<uint32_t>(i / perBatch);
-        if (batches > 1u) {
+    const uint64_t all = static_cast<uint64_t>(c.rows) * c.batches;
+    const unsigned char* const end = c.src + (c.batches - 1) * c.batchPitch + (c.rows - 1) * c.pitch + c.rowBytes;
+    const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32u);
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * (kCopyThreads / 32u) + threadIdx.x / 32u; i < all; i += warps) {
+        uint32_t batch = 0;
+        if (c.batches > 1u) {
+            batch = all >> 32 == 0u ? static_cast<uint32_t>(i) / c.rows : static_cast<uint32_t>(i / c.rows);
             uint32_t first, last;
             aclsp::GroupRows(offsets, batch, offsetRows, &first, &last);
-            if (first == last) {  // nobody reads this matrix: on to the next one's stretches
-                i += (perBatch * (batch + 1) - i - 1) / warps * warps;
+            if (first == last) {  // nobody reads this matrix: on to the next one's rows
+                i += (static_cast<uint64_t>(c.rows) * (batch + 1u) - i - 1u) / warps * warps;
                 continue;
             }
         }
-        const uint32_t inBatch = static_cast<uint32_t>(i - batch * perBatch);
-        const uint32_t row = inBatch / stretches;
-        const int64_t byte = static_cast<int64_t>(inBatch % stretches) * (kCopyWords * 128) + 4 * lane;
-        const unsigned char* from = src + batch * batchPitch + row * pitch + byte;
+        const int64_t row = static_cast<int64_t>(i - static_cast<uint64_t>(batch) * c.rows);
+        const unsigned char* from = c.src + batch * c.batchPitch + row * c.pitch;
         const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 3u;
         from -= shift;
-        uint32_t low[kCopyWords];
-        uint32_t high[kCopyWords];
+        unsigned char* const to = c.dst + batch * c.dstBatchPitch + row * c.dstPitch;
+        // words that reach over an end of the matrix: in its first and its last few rows
+        const bool inside = from >= c.src && from + c.rowBytes + 8 <= end;
+        for (int64_t byte = 4 * lane; byte < c.dstPitch; byte += 128 * kCopyWords) {
+            uint32_t low[kCopyWords];
+            uint32_t high[kCopyWords];
 #pragma unroll
-        for (uint32_t w = 0; w < kCopyWords; ++w) {
-            const bool wanted = byte + 128 * w < rowBytes;
-            low[w] = wanted ? WordOf(from + 128 * w, src, end) : 0u;
-            high[w] = wanted && shift != 0u ? WordOf(from + 128 * w + 4, src, end) : 0u;
-        }
-        unsigned char* const to = dst + batch * dstBatchPitch + row * dstPitch + byte;
+            for (uint32_t w = 0; w < kCopyWords; ++w) {
+                const int64_t at = byte + 128 * w;
+                low[w] = 0;
+                high[w] = 0;
+                if (at < c.rowBytes) {
+                    if (inside) {
+                        low[w] = __ldg(reinterpret_cast<const uint32_t*>(from + at));
+                        high[w] = __ldg(reinterpret_cast<const uint32_t*>(from + at + 4));
+                    } else {
+                        low[w] = WordOf(from + at, c.src, end);
+                        high[w] = WordOf(from + at + 4, c.src, end);
+                    }
+                }
+            }
 #pragma unroll
-        for (uint32_t w = 0; w < kCopyWords; ++w) {
-            if (byte + 128 * w < dstPitch) {
-                *reinterpret_cast<uint32_t*>(to + 128 * w) = __funnelshift_r(low[w], high[w], 8u * shift);
+            for (uint32_t w = 0; w < kCopyWords; ++w) {
+                if (byte + 128 * w < c.dstPitch) {
+                    *reinterpret_cast<uint32_t*>(to + byte + 128 * w) = __funnelshift_r(low[w], high[w], 8u * shift);
+                }
             }
         }
     }
@@ -224,16 +251,47 @@ __global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const unsigned ch
 
 }  // namespace
 
-void AclspGroupedCopyRows(const void* src, void* dst, const AclspGroupedOperand& from, uint64_t ld,
+void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void** right, void* buffer,
                           const AclspGroupedParams& p, cudaStream_t stream)
 {
     const int64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1 : 2;
+    CopyJobs jobs{};
+    uint32_t count = 0;
+    AclspGroupedOperand* const operands[2] = {&o->left, &o->right};
+    const void** const bases[2] = {left, right};
+    for (uint32_t i = 0; i < 2; ++i) {
+        AclspGroupedOperand* const x = operands[i];
+        if (x->copyBytes == 0u) {
+            continue;
+        }
+        CopyJob& c = jobs.job[count++];
+        c.src = static_cast<const unsigned char*>(*bases[i]);
+        c.dst = static_cast<unsigned char*>(buffer) + x->copyOffset;
+        c.rows = static_cast<uint32_t>(x->rows);
+        c.batches = static_cast<uint32_t>(x->batches);
+        c.rowBytes = static_cast<int64_t>(x->rowElements) * bytes;
+        c.pitch = static_cast<int64_t>(x->ld) * bytes;
+        c.batchPitch = static_cast<int64_t>(x->batchStride) * bytes;
+        c.dstPitch = (c.rowBytes + 15) / 16 * 16;
+        c.dstBatchPitch = c.dstPitch * static_cast<int64_t>(x->rows);
+        *bases[i] = c.dst;
+        x->ld = static_cast<uint64_t>(c.dstPitch / bytes);
+        x->batchStride = x->rows * x->ld;
+    }
+    if (count == 0u) {
+        return;
+    }
     AclspCountLaunches(1);
-    CopyRowsKernel<<<148 * 8, kCopyThreads, 0, stream>>>(
-        static_cast<const unsigned char*>(src), static_cast<unsigned char*>(dst), static_cast<uint32_t>(from.rows),
-        static_cast<uint32_t>(from.batches), static_cast<int64_t>(from.rowElements) * bytes,
-        static_cast<int64_t>(from.ld) * bytes, static_cast<int64_t>(from.batchStride) * bytes, static_cast<int64_t>(ld) * bytes,
-        static_cast<int64_t>(from.rows * ld) * bytes, p.offsets, p.rows);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(148 * 8 / count, count);
+    config.blockDim = dim3(kCopyThreads);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, CopyRowsKernel, jobs, p.offsets, p.rows);
 }
 
 extern "C" uint64_t aclsp_b200_grouped_buffer_bytes(const AclspGroupedParams* params)

@@ -39,9 +39,9 @@ struct AclspGroupedOperands {
 };
 AclspGroupedOperands AclspGroupedDescribe(const AclspGroupedParams& p);
 
-// dst gets the operand's rows, its own ld and batchStride being those of `from`, with rows of ld (and batches of rows * ld)
-// elements.  Batches whose group has no rows are left out.
-void AclspGroupedCopyRows(const void* src, void* dst, const AclspGroupedOperand& from, uint64_t ld,
+// Copies the operands that need it, in one launch, and makes bases, ld and batchStride those of the copies.  Batches
+// whose group has no rows are left out.
+void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void** right, void* buffer,
                           const AclspGroupedParams& p, cudaStream_t stream);
 
 // Launches the product; false, and nothing launched, where a base is not 16-byte aligned, there is nothing to sum over

@@ -850,7 +850,7 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
     }
     AclspGroupedOperands o = AclspGroupedDescribe(p);
     const void* bases[2] = {p.weightGrad != 0 ? a : b, p.weightGrad != 0 ? b : a};
-    AclspGroupedOperand* const operands[2] = {&o.left, &o.right};
+    const AclspGroupedOperand* const operands[2] = {&o.left, &o.right};
     for (uint32_t i = 0; i < 2; ++i) {
         const AclspGroupedOperand& x = *operands[i];
         const uint64_t batch = x.batches > 1u ? x.batchStride : 0u;
@@ -859,17 +859,7 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
             return false;
         }
     }
-    for (uint32_t i = 0; i < 2; ++i) {
-        AclspGroupedOperand* const x = operands[i];
-        if (x->copyBytes != 0u) {
-            void* const copy = static_cast<unsigned char*>(buffer) + x->copyOffset;
-            const uint64_t ld = (x->rowElements * bytes + 15u) / 16u * 16u / bytes;
-            AclspGroupedCopyRows(bases[i], copy, *x, ld, p, s);
-            bases[i] = copy;
-            x->ld = ld;
-            x->batchStride = x->rows * ld;
-        }
-    }
+    AclspGroupedCopyRows(&o, &bases[0], &bases[1], buffer, p, s);
     uint32_t sms = AclspSmCount();
     sms = sms == 0 || sms > kGroupedMaxCtas ? kGroupedMaxCtas : sms;
     CUtensorMap left;

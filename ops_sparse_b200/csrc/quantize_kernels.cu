@@ -24,6 +24,7 @@
 #include "aclsparse_b200_kernels.h"
 #include "element_types.cuh"
 #include "plan_kernels.h"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -180,6 +181,8 @@ __global__ void __launch_bounds__(kThreads, kVec == 1 ? 8 : 6) QuantizeRowsKerne
                                                                uint32_t cols, int64_t ldx, int64_t ldq)
 {
     __shared__ uint32_t warpTop[kThreads / 32];
+    aclsp::WaitForPreviousKernel();
+    aclsp::LetNextKernelStart();
     constexpr uint32_t kRows = kThreads / kLanes;
     const uint32_t lane = threadIdx.x % kLanes;
     const uint32_t row = blockIdx.x * kRows + threadIdx.x / kLanes;
@@ -274,8 +277,16 @@ void LaunchForm(const void* x, signed char* q, float* scales, uint32_t rows, uin
                 cudaStream_t s)
 {
     constexpr uint32_t kRows = kThreads / kLanes;
-    QuantizeRowsKernel<kIn, kVec, kLanes, kHold, kTwice><<<(rows + kRows - 1u) / kRows, kThreads, 0, s>>>(x, q, scales, rows,
-                                                                                                   cols, ldx, ldq);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((rows + kRows - 1u) / kRows);
+    config.blockDim = dim3(kThreads);
+    config.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, QuantizeRowsKernel<kIn, kVec, kLanes, kHold, kTwice>, x, q, scales, rows, cols, ldx, ldq);
 }
 
 template <int kIn, int kVec>
