@@ -159,10 +159,8 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
 // The word at `at`, zeros in place of bytes outside [begin, end).
 __device__ __forceinline__ uint32_t WordOf(const unsigned char* at, const unsigned char* begin, const unsigned char* end)
 {
-    if (at >= begin && at + 4 <= end) {
-        return __ldg(reinterpret_cast<const uint32_t*>(at));
-    }
     uint32_t v = 0;
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (at + i >= begin && at + i < end) {
             v |= static_cast<uint32_t>(__ldg(at + i)) << (8 * i);
@@ -172,7 +170,6 @@ __device__ __forceinline__ uint32_t WordOf(const unsigned char* at, const unsign
 }
 
 constexpr uint32_t kCopyThreads = 256;
-constexpr uint32_t kCopyWords = 4;  // words of a row that a lane has under way
 
 // Rows to copy, in bytes.
 struct CopyJob {
@@ -190,62 +187,58 @@ struct CopyJobs {
     CopyJob job[2];
 };
 
-// A warp per row: it reads aligned words, also the one behind each (from L1 or a neighbour's line), shifts the bytes
-// into place and writes aligned words, the last of a row with what lies behind it.  Bound by HBM: every byte is read and
-// written once.  One launch for both operands: blockIdx.y is the job.
+// A thread per 16 bytes of a copied row: it reads the five aligned words that they come from, shifts the bytes into place
+// and writes one vector, the last of a row with what lies behind it.  Bound by HBM: every byte is read and written once
+// (neighbours' common words come from L1).  One launch for both operands: blockIdx.y is the job.  Measured and left: a
+// warp per row (one stretch of it under way at a time: 13 us for 51 rows of 4462 bytes), and a warp per 512 bytes of a
+// row (short last stretches, 11 us for 5005 rows of 1554 bytes).
 __global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const CopyJobs jobs, const int32_t* offsets,
                                                                uint32_t offsetRows)
 {
     aclsp::WaitForPreviousKernel();
     aclsp::LetNextKernelStart();
     const CopyJob& c = jobs.job[blockIdx.y];
-    const uint32_t lane = threadIdx.x % 32u;
-    const uint64_t all = static_cast<uint64_t>(c.rows) * c.batches;
+    const uint32_t vectors = static_cast<uint32_t>(c.dstPitch / 16);
+    const uint64_t all = static_cast<uint64_t>(c.rows) * c.batches * vectors;
+    const bool fewer = all >> 32 == 0u;  // 32-bit divisions do
     const unsigned char* const end = c.src + (c.batches - 1) * c.batchPitch + (c.rows - 1) * c.pitch + c.rowBytes;
-    const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kCopyThreads / 32u);
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * (kCopyThreads / 32u) + threadIdx.x / 32u; i < all; i += warps) {
+    const uint64_t threads = static_cast<uint64_t>(gridDim.x) * kCopyThreads;
+#pragma unroll 2
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < all; i += threads) {
+        uint64_t row = fewer ? static_cast<uint32_t>(i) / vectors : i / vectors;
+        const int64_t byte = static_cast<int64_t>(i - row * vectors) * 16;
         uint32_t batch = 0;
         if (c.batches > 1u) {
-            batch = all >> 32 == 0u ? static_cast<uint32_t>(i) / c.rows : static_cast<uint32_t>(i / c.rows);
+            batch = fewer ? static_cast<uint32_t>(row) / c.rows : static_cast<uint32_t>(row / c.rows);
+            row -= static_cast<uint64_t>(batch) * c.rows;
             uint32_t first, last;
             aclsp::GroupRows(offsets, batch, offsetRows, &first, &last);
-            if (first == last) {  // nobody reads this matrix: on to the next one's rows
-                i += (static_cast<uint64_t>(c.rows) * (batch + 1u) - i - 1u) / warps * warps;
-                continue;
+            if (first == last) {
+                continue;  // nobody reads this matrix
             }
         }
-        const int64_t row = static_cast<int64_t>(i - static_cast<uint64_t>(batch) * c.rows);
-        const unsigned char* from = c.src + batch * c.batchPitch + row * c.pitch;
+        const unsigned char* from = c.src + batch * c.batchPitch + static_cast<int64_t>(row) * c.pitch + byte;
         const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 3u;
         from -= shift;
-        unsigned char* const to = c.dst + batch * c.dstBatchPitch + row * c.dstPitch;
-        // words that reach over an end of the matrix: in its first and its last few rows
-        const bool inside = from >= c.src && from + c.rowBytes + 8 <= end;
-        for (int64_t byte = 4 * lane; byte < c.dstPitch; byte += 128 * kCopyWords) {
-            uint32_t low[kCopyWords];
-            uint32_t high[kCopyWords];
+        uint32_t w[5];
+        if (from >= c.src && from + 20 <= end) {
 #pragma unroll
-            for (uint32_t w = 0; w < kCopyWords; ++w) {
-                const int64_t at = byte + 128 * w;
-                low[w] = 0;
-                high[w] = 0;
-                if (at < c.rowBytes) {
-                    if (inside) {
-                        low[w] = __ldg(reinterpret_cast<const uint32_t*>(from + at));
-                        high[w] = __ldg(reinterpret_cast<const uint32_t*>(from + at + 4));
-                    } else {
-                        low[w] = WordOf(from + at, c.src, end);
-                        high[w] = WordOf(from + at + 4, c.src, end);
-                    }
-                }
+            for (uint32_t k = 0; k < 5; ++k) {
+                w[k] = __ldg(reinterpret_cast<const uint32_t*>(from) + k);
             }
+        } else {  // next to an end of the matrix
 #pragma unroll
-            for (uint32_t w = 0; w < kCopyWords; ++w) {
-                if (byte + 128 * w < c.dstPitch) {
-                    *reinterpret_cast<uint32_t*>(to + byte + 128 * w) = __funnelshift_r(low[w], high[w], 8u * shift);
-                }
+            for (uint32_t k = 0; k < 5; ++k) {
+                w[k] = WordOf(from + 4 * k, c.src, end);
             }
         }
+        uint32_t v[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            v[k] = __funnelshift_r(w[k], w[k + 1], 8u * shift);
+        }
+        unsigned char* const to = c.dst + batch * c.dstBatchPitch + static_cast<int64_t>(row) * c.dstPitch + byte;
+        *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
 
