@@ -219,27 +219,27 @@ __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void*
     }
 }
 
-template <bool kGradient>
+template <bool kGradient, typename T>
 __device__ __forceinline__ void StoreResults(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
-                                             uint32_t j0, const Lane16& sums, float laneScale, float beta,
-                                             uint32_t turn)
+                                             uint32_t j0, const Lane16& sums, float laneScale, float beta, uint32_t turn)
 {
     if constexpr (kGradient) {
-        if (p.outType == ACLSP_TYPE_F32) {
-            StoreGradient<float>(p, c, s, row, j0, sums, laneScale, beta, turn);
-        } else if (p.outType == ACLSP_TYPE_F16) {
-            StoreGradient<__half>(p, c, s, row, j0, sums, laneScale, beta, turn);
-        } else {
-            StoreGradient<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta, turn);
-        }
+        StoreGradient<T>(p, c, s, row, j0, sums, laneScale, beta, turn);
     } else {
-        if (p.outType == ACLSP_TYPE_F32) {
-            StoreForward<float>(p, c, s, row, j0, sums, laneScale, beta);
-        } else if (p.outType == ACLSP_TYPE_F16) {
-            StoreForward<__half>(p, c, s, row, j0, sums, laneScale, beta);
-        } else {
-            StoreForward<__nv_bfloat16>(p, c, s, row, j0, sums, laneScale, beta);
-        }
+        StoreForward<T>(p, c, s, row, j0, sums, laneScale, beta);
+    }
+}
+
+// Calls f with a value of C's type: outside the loops over a tile's columns, which are then straight code.
+template <typename F>
+__device__ __forceinline__ void WithOutType(uint32_t type, F f)
+{
+    if (type == ACLSP_TYPE_F32) {
+        f(float{});
+    } else if (type == ACLSP_TYPE_F16) {
+        f(__half{});
+    } else {
+        f(__nv_bfloat16{});
     }
 }
 
@@ -591,18 +591,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + row);
             }
             if (s.parts == 1u) {
-                for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
-                    uint32_t bits[16];
-                    Lane16 sums;
-                    __syncwarp();
-                    TmemLoad16(from + j0, bits);
-                    TmemLoadWait();
+                WithOutType(p.outType, [&](auto type) {
+                    for (uint32_t j0 = firstChunk; j0 < s.columns; j0 += kChunkStep) {
+                        uint32_t bits[16];
+                        Lane16 sums;
+                        __syncwarp();
+                        TmemLoad16(from + j0, bits);
+                        TmemLoadWait();
 #pragma unroll
-                    for (uint32_t j = 0; j < 16; ++j) {
-                        sums.v[j] = nothing ? 0.0f : SumToFloat<kInt8>(bits[j]);
+                        for (uint32_t j = 0; j < 16; ++j) {
+                            sums.v[j] = nothing ? 0.0f : SumToFloat<kInt8>(bits[j]);
+                        }
+                        StoreResults<kGradient, decltype(type)>(p, c, s, row, j0, sums, laneScale, beta, turn);
                     }
-                    StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta, turn);
-                }
+                });
                 release(half);
                 continue;
             }
@@ -680,7 +682,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t j = 0; j < 16; ++j) {
                     sums.v[j] = SumToFloat<kInt8>(total[j]);
                 }
-                StoreResults<kGradient>(p, c, s, row, j0, sums, laneScale, beta, turn);
+                WithOutType(p.outType, [&](auto type) {
+                    StoreResults<kGradient, decltype(type)>(p, c, s, row, j0, sums, laneScale, beta, turn);
+                });
             }
         }
     }
@@ -772,8 +776,8 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
 
 // The width of a tile.  What a choice costs is the number of turns that the workers take for all tiles times what a turn
 // takes: the blocks of the summed index at the rate that an SM gets operands from L2 (a block of a 128 x 32 tile is 20 KB,
-// of a 128 x 64 one 24 KB, of 128 x 128 32 KB; in a pair's 256 x 256 tile each CTA loads 32 KB), and the results of the
-// last turn.  The host knows the rows of an average group only; larger groups are cut into more tiles, which read the
+// of a 128 x 64 one 24 KB, of 128 x 128 32 KB; in a pair's 256 x 256 tile each CTA loads 32 KB), or writing the results
+// of the tile before, where that is longer; and the results of the last one.  The host knows the rows of an average group only; larger groups are cut into more tiles, which read the
 // dense matrix again, from L2, smaller ones leave columns unused.
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
 {
@@ -800,7 +804,8 @@ uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
         const uint64_t across = ((p.weightGrad != 0 ? p.n : average) + c.columns - 1u) / c.columns;
         const uint64_t tiles = (p.weightGrad != 0 ? p.groups : groups) * down * across;
         const uint64_t turns = (tiles + c.workers - 1u) / c.workers;
-        const uint64_t cost = turns * blocks * c.block + c.results * (p.weightGrad != 0 ? turns : 1u);
+        const uint64_t results = p.inType == ACLSP_TYPE_I8 ? c.results + c.results / 2u : c.results;
+        const uint64_t cost = turns * (blocks * c.block > results ? blocks * c.block : results) + results;
         if (cost < least) {
             least = cost;
             best = c.columns;
