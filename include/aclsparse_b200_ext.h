@@ -157,6 +157,12 @@ aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t handle, con
                                                    aclsparseDnMatDescr_t matC, aclDataType computeType,
                                                    void* externalBuffer);
 
+/* How many CTAs of grouped products over `externalBuffer` gave up a wait since its counters were last cleared.  Every
+ * wait of those kernels is bounded, at four seconds; a CTA whose wait runs out leaves its tiles unfinished and counts
+ * itself here.  Anything but 0 means that results since then are not to be used; the call then clears the counters, so
+ * that the next product can use the buffer again.  Synchronises `stream`.  No counterpart in the reference. */
+aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stream, void* externalBuffer, unsigned* count);
+
 /* Rows of a matrix in 8 bits with one scale each, the operand of the int8 product above:
  *     scales[r] = max_k |X[r, k]| * (1 / 127)   (in fp32, 1 / 127 being its nearest fp32 number),
  *     Q[r, k]   = X[r, k] / scales[r], the exact quotient rounded to the nearest integer, ties to even

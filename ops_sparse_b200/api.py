@@ -11,6 +11,7 @@ status the C function returned.
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import byref, c_float, c_size_t, c_void_p
 
 import torch
@@ -311,8 +312,20 @@ def _device_array(name: str, t, dtype, count: int):
         raise ValueError(f"{name} must have {count} elements, but has {t.numel()}")
 
 
+@functools.lru_cache(maxsize=64)
+def _float_scalars(alpha: float, beta: float):
+    return _scalars(alpha, beta)
+
+
+def _address(t) -> "int | None":
+    return None if t is None else t.data_ptr()
+
+
 class _Grouped:
-    """The three phases of a grouped product; the subclasses supply the C functions' names and operands."""
+    """The three phases of a grouped product; the subclasses supply the C functions' names and operands.
+
+    A small product takes the GPU less time than a careless call takes the host: scalars and functions are looked up,
+    not made anew."""
 
     name = ""
 
@@ -320,8 +333,10 @@ class _Grouped:
         raise NotImplementedError
 
     def _call(self, phase: str, alpha, beta, last) -> None:
-        pa, pb, _keep = _scalars(alpha, beta)
-        check(self.name + phase, getattr(L.lib(), self.name + phase)(*self._args(pa, pb), last))
+        pa, pb, _keep = _scalars(alpha, beta) if isinstance(alpha, torch.Tensor) else _float_scalars(alpha, beta)
+        status = getattr(L.lib(), self.name + phase)(*self._args(pa, pb), last)
+        if status != L.SUCCESS:
+            raise AclsparseError(self.name + phase, status)
 
     def buffer_size(self, alpha=1.0, beta=0.0) -> int:
         size = c_size_t(0)
@@ -336,12 +351,21 @@ class _Grouped:
     def preprocess(self, alpha=1.0, beta=0.0) -> None:
         if self.buffer is None:
             self.allocate(alpha, beta)
-        self._call("Preprocess", alpha, beta, _ptr(self.buffer))
+        self._call("Preprocess", alpha, beta, self.buffer.data_ptr())
 
     def __call__(self, alpha=1.0, beta=0.0) -> None:
         if self.buffer is None:
             self.allocate(alpha, beta)
-        self._call("", alpha, beta, _ptr(self.buffer))
+        self._call("", alpha, beta, self.buffer.data_ptr())
+
+    def wait_failures(self) -> int:
+        """CTAs that gave up a wait since the buffer's counters were last cleared (0 after healthy products); waits for
+        the handle's stream."""
+        count, stream = ctypes.c_uint32(0), c_void_p(None)
+        check("aclsparseGetStream", L.lib().aclsparseGetStream(self.handle.raw, byref(stream)))
+        check("aclsparseB200GroupedMMWaitFailures",
+              L.lib().aclsparseB200GroupedMMWaitFailures(stream, _ptr(self.buffer), byref(count)))
+        return int(count.value)
 
 
 class GroupedMM(_Grouped):
@@ -364,8 +388,8 @@ class GroupedMM(_Grouped):
         self.buffer = None
 
     def _args(self, pa, pb):
-        return (self.handle.raw, self.op_b, pa, self.a.raw, _ptr(self.offsets), self.b.raw, _ptr(self.row_scales),
-                _ptr(self.col_scales), pb, self.c.raw, L.ACL_FLOAT)
+        return (self.handle.raw, self.op_b, pa, self.a.raw, _address(self.offsets), self.b.raw, _address(self.row_scales),
+                _address(self.col_scales), pb, self.c.raw, L.ACL_FLOAT)
 
 
 class GroupedMMWeightGrad(_Grouped):
@@ -379,7 +403,7 @@ class GroupedMMWeightGrad(_Grouped):
         self.buffer = None
 
     def _args(self, pa, pb):
-        return (self.handle.raw, pa, self.a.raw, self.b.raw, _ptr(self.offsets), pb, self.c.raw, L.ACL_FLOAT)
+        return (self.handle.raw, pa, self.a.raw, self.b.raw, _address(self.offsets), pb, self.c.raw, L.ACL_FLOAT)
 
 
 class QuantizeRows:
@@ -391,7 +415,7 @@ class QuantizeRows:
 
     def __call__(self) -> None:
         check("aclsparseB200QuantizeRows", L.lib().aclsparseB200QuantizeRows(self.handle.raw, self.x.raw, self.q.raw,
-                                                                             _ptr(self.scales)))
+                                                                             self.scales.data_ptr()))
 
 
 def kernel_launches() -> int:

@@ -410,6 +410,27 @@ extern "C" aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t 
                    externalBuffer, p);
 }
 
+extern "C" aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stream, void* externalBuffer,
+                                                                unsigned* count)
+{
+    if (externalBuffer == nullptr || count == nullptr) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    auto s = static_cast<cudaStream_t>(stream);
+    uint32_t value = 0;  // the buffer's first word
+    if (cudaMemcpyAsync(&value, externalBuffer, sizeof(value), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return ACL_SPARSE_STATUS_EXECUTION_FAILED;
+    }
+    *count = value;
+    if (value != 0) {
+        aclsp_b200_grouped_preprocess_kernel_do(externalBuffer, stream);
+        return Enqueued("aclsparseB200GroupedMMWaitFailures");
+    }
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
 extern "C" aclsparseStatus_t aclsparseB200QuantizeRows(aclsparseHandle_t handle, aclsparseConstDnMatDescr_t matX,
                                                        aclsparseDnMatDescr_t matQ, float* scales)
 {

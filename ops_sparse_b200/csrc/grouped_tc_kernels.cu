@@ -36,6 +36,7 @@
  * flight are waited for (bounded again), tensor memory is freed, and the buffer's
  * first word counts it.
  */
+#include <atomic>
 #include <cstdint>
 
 #include <cuda.h>
@@ -753,7 +754,16 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     constexpr uint32_t kCtas = kColumns == 256u ? 2u : 1u;
     constexpr uint32_t kBytes = Ring<kColumns, kCtas, kGradient>::kBytes;
     auto kernel = GroupedTensorKernel<kInt8, kColumns, kGradient, kCtas>;
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes));
+    // once per device: a small product takes the GPU about as long as this call takes the host with its launch
+    static std::atomic<uint64_t> allowed{0};
+    int device = 0;
+    (void)cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if ((allowed.load(std::memory_order_relaxed) & bit) == 0u) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytes)) == cudaSuccess) {
+            allowed.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     AclspCountLaunches(1);
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(sms / kCtas * kCtas);

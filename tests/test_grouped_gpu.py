@@ -223,6 +223,17 @@ def test_forward_is_repeatable_and_its_buffer_is_reusable():
     case.check()
 
 
+def test_wait_failures_are_counted_and_cleared():
+    """No wait runs out in a healthy product; a count left in the buffer is reported once and cleared."""
+    case = Forward([1, 3], 2048, 256, torch.bfloat16)
+    case.op.preprocess()
+    case.op()
+    assert case.op.wait_failures() == 0
+    case.op.buffer[:4].view(torch.int32).fill_(3)
+    assert case.op.wait_failures() == 3 and case.op.wait_failures() == 0
+    case.check()
+
+
 def test_two_products_share_a_buffer_in_turn():
     one, two = Forward([1, 2], 2048, 128, torch.bfloat16), Forward([5], 4096, 256, torch.float16, seed=3)
     size = max(one.op.buffer_size(), two.op.buffer_size())
@@ -645,6 +656,23 @@ def test_adapter_checks_its_arguments():
     y = A.grouped_mm(x[:0].requires_grad_(), w.requires_grad_(), offsets)
     gw, = torch.autograd.grad(y, w, torch.zeros_like(y))
     assert gw.shape == w.shape and (gw == 0).all()
+
+
+def test_gradient_of_a_broadcast_result():
+    """dy with strides of zero, as the gradient of a sum has them, and a gradient for one operand only."""
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    offsets = torch.tensor([0, 7, 20], dtype=torch.int32, device=DEV)
+    x, w = randn(20, 24, dtype=torch.bfloat16, gen=gen), randn(2, 16, 24, dtype=torch.bfloat16, gen=gen)
+    w1 = w.clone().requires_grad_()
+    A.grouped_mm(x, w1, offsets).sum().backward()
+    want = torch.stack([x[:7].double().sum(0).expand(16, 24), x[7:].double().sum(0).expand(16, 24)])
+    size = torch.stack([x[:7].double().abs().sum(0).expand(16, 24), x[7:].double().abs().sum(0).expand(16, 24)])
+    close(w1.grad, want, sum_bound(13, size, False))
+    x1 = x.clone().requires_grad_()
+    A.grouped_mm(x1, w, offsets).sum().backward()
+    want = torch.cat([w[0].double().sum(0).expand(7, 24), w[1].double().sum(0).expand(13, 24)])
+    size = torch.cat([w[0].double().abs().sum(0).expand(7, 24), w[1].double().abs().sum(0).expand(13, 24)])
+    close(x1.grad, want, sum_bound(16, size, False))
 
 
 def test_training_step_replays_in_a_graph():

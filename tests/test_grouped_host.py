@@ -136,6 +136,12 @@ def test_gradient_accepts_and_refuses(lib, handle, mat):
         assert fn(handle, ONE, a, b, FAKE[9], ONE, c, L.ACL_FLOAT, c_void_p(0x10010)) == L.INVALID_VALUE
 
 
+def test_wait_failure_counter_refusals(lib):
+    count = ctypes.c_uint32(7)
+    assert lib.aclsparseB200GroupedMMWaitFailures(FAKE[1], None, byref(count)) == L.INVALID_VALUE
+    assert lib.aclsparseB200GroupedMMWaitFailures(FAKE[1], FAKE[0], None) == L.INVALID_VALUE
+
+
 def test_quantize_refusals(lib, handle, mat):
     x, q = mat(4, 8), mat(4, 8, dtype=L.ACL_INT8)
     call = lib.aclsparseB200QuantizeRows
