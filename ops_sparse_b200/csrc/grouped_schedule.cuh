@@ -64,8 +64,10 @@ public:
         tile_ = workers.index;
         whole_ = tiles_ / workers.count * workers.count;
         const uint32_t left = tiles_ - whole_;
-        if (left != 0u && 2u * left <= workers.count && blocks > kMinSplitBlocks + joinBlocks) {
-            const uint32_t parts = workers.count / left;
+        // one part per SM: a second one there would only share its loads
+        const uint32_t most = workers.count < kGroupedMaxCtas ? workers.count : kGroupedMaxCtas;
+        if (left != 0u && 2u * left <= most && blocks > kMinSplitBlocks + joinBlocks) {
+            const uint32_t parts = most / left;
             const uint32_t length = (blocks + parts - 1u) / parts;
             length_ = length > kMinSplitBlocks ? length : kMinSplitBlocks;
             length_ = length_ + joinBlocks < blocks ? length_ : blocks;

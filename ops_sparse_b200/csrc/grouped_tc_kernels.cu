@@ -53,8 +53,16 @@ namespace {
 
 using namespace aclsp;
 
-constexpr uint32_t kResultWarps = 8;  // two for each quarter of the lanes of tensor memory
-constexpr int kThreads = 128 + 32 * kResultWarps;
+// Narrow tiles are for few rows, where reading the dense matrix is all: two CTAs to an SM, with half its shared memory
+// each, so that one loads while the other starts or ends (2048 x 4096 matrices of 64 groups of 4 rows: 172 us with one
+// CTA and all of it).
+template <uint32_t kColumns>
+constexpr uint32_t kCtasPerSm = kColumns <= 64u ? 2u : 1u;
+// Warps that write results: one or two for each quarter of the lanes of tensor memory.
+template <uint32_t kColumns>
+constexpr uint32_t kResultWarpsOf = kColumns <= 64u ? 4u : 8u;
+template <uint32_t kColumns>
+constexpr uint32_t kThreads = 128u + 32u * kResultWarpsOf<kColumns>;
 constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kRightBox = 32;  // rows of one load of a forward product's right operand
@@ -67,8 +75,8 @@ template <uint32_t kColumns, uint32_t kCtas, bool kGradient>
 struct Ring {
     static constexpr uint32_t kRightRows = kColumns / kCtas;  // of the right operand in one CTA
     static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
-    static constexpr uint32_t kTurnBytes = kGradient ? kResultWarps * kTurnWarpBytes : 0u;
-    static constexpr uint32_t kStages = (224u * 1024u - kTurnBytes) / kStageBytes;
+    static constexpr uint32_t kTurnBytes = kGradient ? kResultWarpsOf<kColumns> * kTurnWarpBytes : 0u;
+    static constexpr uint32_t kStages = ((kCtasPerSm<kColumns> == 2u ? 111u : 224u) * 1024u - kTurnBytes) / kStageBytes;
     static constexpr uint32_t kTurn = kStageBytes * kStages;           // behind the stages: StoreGradient's room
     static constexpr uint32_t kBytes = kTurn + kTurnBytes + 1024u;     // stages start on multiples of 1024
 };
@@ -257,7 +265,7 @@ __device__ __forceinline__ uint32_t AddSums(uint32_t a, uint32_t b)
 }
 
 template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
                         void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
                         const uint32_t leftMn, const uint32_t joinBlocks)
@@ -265,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using R = Ring<kColumns, kCtas, kGradient>;
     constexpr uint32_t kBlock = kInt8 ? 128u : 64u;         // elements of the summed index in a block
     constexpr uint32_t kStepElements = kInt8 ? 32u : 16u;   // and in one MMA
+    constexpr uint32_t kResultWarps = kResultWarpsOf<kColumns>;
     constexpr uint32_t kColumnStep = 16u * kCtas;           // N of the MMA is a multiple of this
     extern __shared__ unsigned char dynamic[];
     __shared__ uint64_t full[R::kStages];
@@ -652,10 +661,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const uint4* const at = partials + tmemLane + j0 / 4u * kTileLanes;
                 uint32_t total[16];
-                for (uint32_t k = 0; k < s.parts; k += 4u) {
-                    uint4 v[4][4];  // four parts under way together
+                constexpr uint32_t kTogether = kColumns <= 64u ? 2u : 4u;  // parts under way together
+                for (uint32_t k = 0; k < s.parts; k += kTogether) {
+                    uint4 v[kTogether][4];
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; ++q) {
+                    for (uint32_t q = 0; q < kTogether; ++q) {
                         if (k + q < s.parts) {
                             const uint32_t slot = (s.slot - s.part + k + q) * kCtas + rank;
 #pragma unroll
@@ -665,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; ++q) {
+                    for (uint32_t q = 0; q < kTogether; ++q) {
                         if (k + q < s.parts) {
 #pragma unroll
                             for (uint32_t j = 0; j < 4; ++j) {
@@ -766,8 +776,8 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     }
     AclspCountLaunches(1);
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(sms / kCtas * kCtas);
-    config.blockDim = dim3(kThreads);
+    config.gridDim = dim3(sms * kCtasPerSm<kColumns> / kCtas * kCtas);
+    config.blockDim = dim3(kThreads<kColumns>);
     config.dynamicSmemBytes = kBytes;
     config.stream = s;
     cudaLaunchAttribute attributes[2] = {};
