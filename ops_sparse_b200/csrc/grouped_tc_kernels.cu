@@ -1,40 +1,47 @@
 /*
  * Grouped matrix products on the tensor cores (tcgen05), fed by TMA.
  *
- * A tile of the result is 128 lanes x up to kColumns columns of fp32 (int32) sums
- * in tensor memory.  The DENSE matrix lies along the lanes and the ragged rows
+ * A tile of the result is 128 lanes per CTA x up to kColumns columns of fp32 (int32)
+ * sums in tensor memory.  The DENSE matrix lies along the lanes and the ragged rows
  * along the columns: N of tcgen05.mma is any multiple of 16, so a group of 5 rows
  * costs an MMA of 16 columns and not one of 128 rows, and the same kernel serves a
- * decoding batch (all time goes into reading weights) and a training batch.  For
- * the weight gradient both operands are read with their summed index, the rows,
- * along the outer dimension (MN-major), and the last rows of a group, which share
- * a block with the next group's, are cut off in shared memory.
+ * decoding batch, where all time goes into reading weights, and a training batch.
+ * For the weight gradient both operands are read with their summed index, the rows,
+ * along the outer dimension (MN-major), and the last rows of a group, which share a
+ * block with the next group's, are cut off in shared memory.
  *
- * Wide tiles (256 columns) are computed by a pair of CTAs on neighbouring SMs, 256 x 256 results: each holds 128 rows
- * of the dense matrix and half of the ragged rows, and one MMA reads both.  A single CTA would have to load 48 KB for
- * 512 cycles of MMA, more than the 52 bytes per cycle that an SM was measured to get from L2 with all of them
- * loading; the pair loads 32 KB each.
+ * Wide tiles (256 columns) are computed by a pair of CTAs on neighbouring SMs, 256 x
+ * 256 results: each holds 128 rows of the dense matrix and half of the ragged rows,
+ * and one MMA reads both.  A single CTA would have to load 48 KB for 512 cycles of
+ * MMA, more than the 52 bytes per cycle that an SM was measured to get from L2 with
+ * all of them loading; the pair loads 32 KB each (16384 x 4096 x 4096: 1500 TFLOP/s).
  *
- * One CTA per SM, persistent: warp 0 loads blocks of 128 bytes of the summed index
- * into a ring of stages, one lane of warp 1 issues the MMAs, warps 4 to 11 read
- * the finished sums and write results while the next tile computes in the other
- * half of tensor memory.  Warp 3 works out the next tiles ahead of all of them, and
- * warp 2 cuts the ends of groups off; done by the MMA warp itself either left the
- * tensor cores idle for 600 cycles per tile.  Tiles that do not fill a wave are split along the summed
- * index (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and for each
- * piece of the tile, 32 lanes x 16 columns, the warp that arrives last adds them in
- * the CTAs' order, so that the result does not depend on who that is.  CTAs go
- * through the pieces from different ones on: arriving together, each is the last one
- * for some, and the adding is shared (512 x 512 from 16384 rows, 19 CTAs to a tile:
- * 62 us with one CTA adding a whole tile).
+ * CTAs are persistent: warp 0 loads blocks of 128 bytes of the summed index into a
+ * ring of stages, one lane of warp 1 issues the MMAs, warps from 4 on read the
+ * finished sums and write results while the next tile computes in the other half of
+ * tensor memory.  Warp 3 works out the next tiles ahead of all of them, and warp 2
+ * cuts the ends of groups off; done by the MMA warp itself either left the tensor
+ * cores idle for 600 cycles per tile.
  *
- * Operands whose rows do not start on multiples of 16 bytes (odd widths) cannot be loaded by TMA: they are copied to
- * rows that do first (grouped_kernels.cu), in the buffer.  Warps that bring such rows into shared memory themselves,
- * shifting each word into place, were built and measured: 128 x 128 x 64 blocks took 3000 cycles instead of 256.
+ * Tiles that do not fill a wave are split along the summed index
+ * (grouped_schedule.cuh): each CTA leaves its sums in the buffer, and for each piece
+ * of the tile, 32 lanes x 16 columns, the warp that arrives last adds them in the
+ * parts' order, so that the result does not depend on who that is.  Parts go through
+ * the pieces from different ones on: arriving together, each is the last one for some,
+ * and the adding is shared (512 x 512 from 16384 rows: 24 us; 62 us with one CTA adding
+ * a whole tile).
  *
- * Every wait is bounded.  One that runs out makes the CTA leave: the loads in
- * flight are waited for (bounded again), tensor memory is freed, and the buffer's
- * first word counts it.
+ * Operands whose rows do not start on multiples of 16 bytes (odd widths) cannot be
+ * loaded by TMA: they are copied to rows that do first (grouped_kernels.cu), in the
+ * buffer.  Warps that bring such rows into shared memory themselves, shifting each word
+ * into place, were built and measured: 128 x 128 x 64 blocks took 3000 cycles instead of
+ * 256 (2048 x 2049 matrices, 8192 rows: 620 us, with the copy 119 us).
+ *
+ * The set-up of a CTA overlaps the end of the kernel before (programmatic launch); each
+ * warp waits for that one's memory before it touches its own.
+ *
+ * Every wait is bounded.  One that runs out makes the CTA leave: the loads in flight are
+ * given time to land, tensor memory is freed, and the buffer's first word counts it.
  */
 #include <atomic>
 #include <cstdint>
@@ -54,8 +61,8 @@ namespace {
 using namespace aclsp;
 
 // Narrow tiles are for few rows, where reading the dense matrix is all: two CTAs to an SM, with half its shared memory
-// each, so that one loads while the other starts or ends (2048 x 4096 matrices of 64 groups of 4 rows: 172 us with one
-// CTA and all of it).
+// each, so that one loads while the other starts or ends (32 groups of 4 rows, 2048 x 1024 matrices: 26.1 us, with one
+// CTA and all of it 28.6).
 template <uint32_t kColumns>
 constexpr uint32_t kCtasPerSm = kColumns <= 64u ? 2u : 1u;
 // Warps that write results: one or two for each quarter of the lanes of tensor memory.
@@ -789,7 +796,8 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = kCtas > 1u ? 2u : 1u;
-    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn, kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
+    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn,
+                       kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
 }
 
 }  // namespace
@@ -797,8 +805,10 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
 // The width of a tile.  What a choice costs is the number of turns that the workers take for all tiles times what a turn
 // takes: the blocks of the summed index at the rate that an SM gets operands from L2 (a block of a 128 x 32 tile is 20 KB,
 // of a 128 x 64 one 24 KB, of 128 x 128 32 KB; in a pair's 256 x 256 tile each CTA loads 32 KB), or writing the results
-// of the tile before, where that is longer; and the results of the last one.  The host knows the rows of an average group only; larger groups are cut into more tiles, which read the
-// dense matrix again, from L2, smaller ones leave columns unused.
+// of the tile before, where that is longer; and the results of the last one.  The host knows the rows of an average group
+// only; larger groups are cut into more tiles, which read the dense matrix again, from L2, smaller ones leave columns
+// unused.  Measured, us: 1003 rows of 4 groups, 776 x 1001: 10.4 with 128 columns, 14.5 with 256; 5719 rows, 1056 x 1968
+// int8: 23.2 with 128, 24.9 with 256; 512 x 512 from 16384 rows: 24.6 with 128, 36.3 with 256.
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p)
 {
     struct Choice {

@@ -322,7 +322,7 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, offsets: "torch.Tensor | N
 
     x: rows x k, weight: groups x n x k, fp16 or bf16; offsets: groups + 1 ascending int32 values on the same device
     (None with one group).  The result has ``out_dtype``: that type (default) or float32; rows in no group are zero.
-    Differentiable in x and weight; offsets carry no gradient.
+    Differentiable (once) in x and weight, from the result's gradient rounded to their type; offsets carry no gradient.
     """
     _check_grouped(x, weight, offsets, (torch.float16, torch.bfloat16))
     out_dtype = x.dtype if out_dtype is None else out_dtype
