@@ -73,9 +73,11 @@ constexpr uint32_t kThreads = 128u + 32u * kResultWarpsOf<kColumns>;
 constexpr uint32_t kSegments = 4;     // tiles that the schedule may be ahead
 constexpr uint32_t kLeftBytes = kTileLanes * 128u;
 constexpr uint32_t kRightBox = 32;  // rows of one load of a forward product's right operand
-// A warp's 32 lanes x 16 results on their way to rows of C that are not aligned: each lane's one word longer than they
-// are, so that the lanes write to different banks.
-constexpr uint32_t kTurnWarpBytes = 32u * (16u * 4u + 4u);
+// Room for a gradient's results on their way out, per warp: two boxes of 32 rows x 128 bytes for TMA; or, where the rows
+// of C are not aligned, 32 lanes x 16 results, each lane's one word longer than they are, so that the lanes write to
+// different banks.
+constexpr uint32_t kTurnBoxBytes = 32u * 128u;
+constexpr uint32_t kTurnWarpBytes = 2u * kTurnBoxBytes;
 constexpr uint64_t kDrainNs = 10000000ull;
 
 template <uint32_t kColumns, uint32_t kCtas, bool kGradient>
@@ -84,7 +86,7 @@ struct Ring {
     static constexpr uint32_t kStageBytes = kLeftBytes + kRightRows * 128u;
     static constexpr uint32_t kTurnBytes = kGradient ? kResultWarpsOf<kColumns> * kTurnWarpBytes : 0u;
     static constexpr uint32_t kStages = ((kCtasPerSm<kColumns> == 2u ? 111u : 224u) * 1024u - kTurnBytes) / kStageBytes;
-    static constexpr uint32_t kTurn = kStageBytes * kStages;           // behind the stages: StoreGradient's room
+    static constexpr uint32_t kTurn = kStageBytes * kStages;           // behind the stages: results on their way out
     static constexpr uint32_t kBytes = kTurn + kTurnBytes + 1024u;     // stages start on multiples of 1024
 };
 
@@ -274,8 +276,8 @@ __device__ __forceinline__ uint32_t AddSums(uint32_t a, uint32_t b)
 template <bool kInt8, uint32_t kColumns, bool kGradient, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     GroupedTensorKernel(const __grid_constant__ CUtensorMap leftMap, const __grid_constant__ CUtensorMap rightMap,
-                        void* __restrict__ c, uint32_t* __restrict__ buffer, const AclspGroupedParams p,
-                        const uint32_t leftMn, const uint32_t joinBlocks)
+                        const __grid_constant__ CUtensorMap outMap, void* __restrict__ c, uint32_t* __restrict__ buffer,
+                        const AclspGroupedParams p, const uint32_t leftMn, const uint32_t outMapped, const uint32_t joinBlocks)
 {
     using R = Ring<kColumns, kCtas, kGradient>;
     constexpr uint32_t kBlock = kInt8 ? 128u : 64u;         // elements of the summed index in a block
@@ -577,6 +579,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
         const uint32_t turn = ring + R::kTurn + (warp - 4u) * kTurnWarpBytes;
         uint32_t* const counters = buffer + kGroupedHeaderWords;
         uint4* const partials = reinterpret_cast<uint4*>(counters + kGroupedCounters);
+        uint32_t boxes = 0;  // that this warp has sent out
         constexpr uint32_t kSlotVectors = kTileLanes * kColumns / 4u;
         Segment s;
         uint32_t tile = 0;
@@ -606,6 +609,60 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             float laneScale = alpha;
             if (!kGradient && p.colScales != nullptr && row < p.n) {
                 laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + row);
+            }
+            if (kGradient && s.parts == 1u && outMapped != 0u && beta == 0.0f) {
+                if constexpr (kGradient) {
+                    // Through shared memory and TMA, two boxes per warp under way: the stores of a tile take longer than
+                    // its short sums, and the warp that issues them itself waits for each (8192 rows of 16 groups, 4096 x
+                    // 2048: 147 us).
+                    WithOutType(p.outType, [&](auto type) {
+                        using T = decltype(type);
+                        constexpr uint32_t kBoxColumns = 128u / sizeof(T);
+                        constexpr uint32_t kOwn = kColumns / (kResultWarps / 4u);  // columns of this warp
+                        const uint32_t begin = (warp - 4u) / 4u * kOwn;
+                        const uint32_t end = s.columns < begin + kOwn ? s.columns : begin + kOwn;
+                        const uint32_t row0 = row - lane;
+                        for (uint32_t j0 = begin; j0 < end; j0 += kBoxColumns) {
+                            const uint32_t box = turn + (boxes++ & 1u) * kTurnBoxBytes;
+                            if (ElectLane()) {
+                                StoresRead<1>();
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t q = 0; q < kBoxColumns / 16u; ++q) {
+                                uint32_t bits[16];
+                                TmemLoad16(from + j0 + 16u * q, bits);
+                                TmemLoadWait();
+                                alignas(16) T out[16];
+#pragma unroll
+                                for (uint32_t j = 0; j < 16; ++j) {
+                                    out[j] = FromFloat<T>(nothing ? 0.0f : SumToFloat<kInt8>(bits[j]) * laneScale);
+                                }
+                                const uint4* vectors = reinterpret_cast<const uint4*>(out);
+                                constexpr uint32_t kVectors = sizeof(out) / 16u;
+#pragma unroll
+                                for (uint32_t v = 0; v < kVectors; ++v) {
+                                    const uint32_t at = box + lane * 128u + ((q * kVectors + v) ^ (lane & 7u)) * 16u;
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(vectors[v].x),
+                                                 "r"(vectors[v].y), "r"(vectors[v].z), "r"(vectors[v].w)
+                                                 : "memory");
+                                }
+                            }
+                            FenceProxyAsync();
+                            __syncwarp();
+                            if (ElectLane()) {
+                                if (row0 < p.m) {
+                                    TmaStore3(&outMap, box, static_cast<int32_t>(s.right + j0), static_cast<int32_t>(row0),
+                                              static_cast<int32_t>(s.group));
+                                }
+                                StoreGroup();
+                            }
+                            __syncwarp();
+                        }
+                    });
+                }
+                release(half);
+                continue;
             }
             if (s.parts == 1u) {
                 WithOutType(p.outType, [&](auto type) {
@@ -639,6 +696,9 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                 }
             }
             release(half);
+            if (kGradient && ElectLane()) {
+                StoresRead<0>();  // the room may be needed again
+            }
             __threadfence();
             __syncwarp();
             const uint32_t pieces = s.columns > firstChunk ? (s.columns - firstChunk + kChunkStep - 1u) / kChunkStep : 0u;
@@ -705,6 +765,10 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                 });
             }
         }
+        __syncwarp();
+        if (kGradient && ElectLane()) {
+            StoresDone();
+        }
     }
 
     __syncthreads();
@@ -741,11 +805,12 @@ EncodeFn Encoder()
     return fn;
 }
 
-// A map of `rank` dimensions (innermost first) whose boxes are 128 bytes wide and `boxRows` rows high.
-bool Encode(CUtensorMap* map, const AclspGroupedParams& p, const void* base, uint32_t rank, const uint64_t* sizes,
+// A map of `rank` dimensions (innermost first) of elements of a type whose boxes are 128 bytes wide and `boxRows` rows
+// high.
+bool Encode(CUtensorMap* map, uint32_t type, const void* base, uint32_t rank, const uint64_t* sizes,
             const uint64_t* strideElements, uint32_t boxRows)
 {
-    const uint64_t bytes = p.inType == ACLSP_TYPE_I8 ? 1u : 2u;
+    const uint64_t bytes = type == ACLSP_TYPE_I8 ? 1u : type == ACLSP_TYPE_F32 ? 4u : 2u;
     cuuint64_t dims[3];
     cuuint64_t strides[2];
     cuuint32_t box[3] = {static_cast<cuuint32_t>(128u / bytes), boxRows, 1};
@@ -756,17 +821,18 @@ bool Encode(CUtensorMap* map, const AclspGroupedParams& p, const void* base, uin
             strides[i - 1] = strideElements[i - 1] * bytes;
         }
     }
-    const CUtensorMapDataType type = p.inType == ACLSP_TYPE_I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                     : p.inType == ACLSP_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return Encoder()(map, type, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUtensorMapDataType element = type == ACLSP_TYPE_I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                        : type == ACLSP_TYPE_F32  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                        : type == ACLSP_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return Encoder()(map, element, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <bool kInt8, uint32_t kColumns, bool kGradient>
-void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* buffer, const AclspGroupedParams& p,
-            uint32_t leftMn, uint32_t sms, cudaStream_t s)
+void Launch(const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap* out, void* c, void* buffer,
+            const AclspGroupedParams& p, uint32_t leftMn, uint32_t sms, cudaStream_t s)
 {
     constexpr uint32_t kCtas = kColumns == 256u ? 2u : 1u;
     constexpr uint32_t kBytes = Ring<kColumns, kCtas, kGradient>::kBytes;
@@ -796,8 +862,8 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, void* c, void* bu
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = kCtas > 1u ? 2u : 1u;
-    cudaLaunchKernelEx(&config, kernel, left, right, c, static_cast<uint32_t*>(buffer), p, leftMn,
-                       kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
+    cudaLaunchKernelEx(&config, kernel, left, right, out != nullptr ? *out : left, c, static_cast<uint32_t*>(buffer), p, leftMn,
+                       out != nullptr ? 1u : 0u, kColumns >= 256u ? kJoinBlocksWide : kJoinBlocks);
 }
 
 }  // namespace
@@ -904,17 +970,28 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
     const uint64_t rightSizes[2] = {o.right.rowElements, o.right.rows};
     const uint64_t rightStride[1] = {o.right.ld};
     if (p.weightGrad != 0) {
-        if (!Encode(&left, p, bases[0], 2, leftSizes, leftStrides, 64) ||
-            !Encode(&right, p, bases[1], 2, rightSizes, rightStride, 64)) {
+        if (!Encode(&left, p.inType, bases[0], 2, leftSizes, leftStrides, 64) ||
+            !Encode(&right, p.inType, bases[1], 2, rightSizes, rightStride, 64)) {
             return false;
         }
-        (columns == 256u ? Launch<false, 256, true> : Launch<false, 128, true>)(left, right, c, buffer, p, 1u, sms, s);
+        // results through TMA where C allows it
+        CUtensorMap out;
+        const uint64_t outBytes = p.outType == ACLSP_TYPE_F32 ? 4u : 2u;
+        const uint64_t outSizes[3] = {p.n, p.m, p.groups};
+        const uint64_t outStrides[2] = {static_cast<uint64_t>(p.ldc),
+                                        static_cast<uint64_t>(p.groups > 1u ? p.cBatchStride : p.ldc)};
+        const bool outMapped = reinterpret_cast<uintptr_t>(c) % 16u == 0u && outStrides[0] * outBytes % 16u == 0u &&
+                               outStrides[1] * outBytes % 16u == 0u && outStrides[0] * outBytes < kFarthest &&
+                               outStrides[1] * outBytes < kFarthest &&
+                               Encode(&out, p.outType, c, 3, outSizes, outStrides, 32);
+        (columns == 256u ? Launch<false, 256, true> : Launch<false, 128, true>)(left, right, outMapped ? &out : nullptr, c,
+                                                                                buffer, p, 1u, sms, s);
         return true;
     }
     const uint32_t leftMn = p.bInner == 1 ? 0u : 1u;
     const uint32_t leftBox = leftMn != 0 ? static_cast<uint32_t>(128u / bytes) : kTileLanes;
-    if (!Encode(&left, p, bases[0], 3, leftSizes, leftStrides, leftBox) ||
-        !Encode(&right, p, bases[1], 2, rightSizes, rightStride, kRightBox)) {
+    if (!Encode(&left, p.inType, bases[0], 3, leftSizes, leftStrides, leftBox) ||
+        !Encode(&right, p.inType, bases[1], 2, rightSizes, rightStride, kRightBox)) {
         return false;
     }
     const bool int8 = p.inType == ACLSP_TYPE_I8;
@@ -926,6 +1003,6 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
                        : columns == 64u  ? Launch<false, 64, false>
                        : columns == 128u ? Launch<false, 128, false>
                                          : Launch<false, 256, false>);
-    run(left, right, c, buffer, p, leftMn, sms, s);
+    run(left, right, nullptr, c, buffer, p, leftMn, sms, s);
     return true;
 }

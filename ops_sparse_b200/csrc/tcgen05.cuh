@@ -138,6 +138,22 @@ __device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map, u
     }
 }
 
+// A box of shared memory into a batch of matrices; what lies outside them is not written.  The thread's stores form
+// groups: at most kLeft of them may still be reading shared memory after the wait (none under way after StoresDone).
+__device__ __forceinline__ void TmaStore3(const CUtensorMap* map, uint32_t src, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(map), "r"(src), "r"(x),
+                 "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void StoreGroup() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void StoresRead()
+{
+    asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void StoresDone() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
 // A kernel launched with programmatic serialization starts while the one before it in the stream still runs: nothing of
 // that one's may be read, nor anything written, before this wait.  The other call lets the next such kernel start.
 __device__ __forceinline__ void WaitForPreviousKernel() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
