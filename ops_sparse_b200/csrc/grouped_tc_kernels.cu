@@ -361,10 +361,12 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     };
     auto cutRows = [&](uint32_t valid, uint32_t left) {
         const uint32_t vectors = (kStepElements - valid % kStepElements) % kStepElements * 8u;
-        constexpr uint32_t kSmemBlocks = 2u + R::kRightRows / 64u;
-        for (uint32_t i = lane; i < vectors * kSmemBlocks; i += 32u) {
-            const uint32_t address = left + i / vectors * 8192u + valid * 128u + i % vectors * 16u;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(address), "r"(0) : "memory");
+        for (uint32_t i = lane; i < vectors; i += 32u) {
+#pragma unroll
+            for (uint32_t block = 0; block < 2u + R::kRightRows / 64u; ++block) {
+                const uint32_t address = left + block * 8192u + valid * 128u + i * 16u;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(address), "r"(0) : "memory");
+            }
         }
         FenceProxyAsync();
         __syncwarp();
@@ -442,82 +444,98 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             }
         }
     } else if (warp == 1 && rank == 0u) {
-        const bool leftT = kGradient || leftMn != 0u;
-        const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
-        // 32 bytes of the summed index per instruction: inside a 128-byte row, or as many rows as it has elements
-        const uint32_t leftStep = (leftT ? kStepElements * 128u : 32u) >> 4;
-        const uint32_t rightStep = (kGradient ? kStepElements * 128u : 32u) >> 4;
-        Segment s;
-        uint32_t stage = 0;
-        uint32_t parity = 0;
-        uint32_t tile = 0;
-        uint32_t cuts = 0;  // a bit per stage: the parity of its next cut block
-        bool good = true;
-        bool more = nextSegment(&s);
-        while (more) {
-            const uint32_t half = tile & 1u;
-            good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop)) != 0;
-            if (!good) {
-                break;
-            }
-            ++tile;
-            TmemFenceAfter();
-            const uint32_t d = tmem + half * kColumns;
-            const uint32_t instruction = shape | MmaColumns((s.columns + kColumnStep - 1u) / kColumnStep * kColumnStep);
-            const uint32_t length = kGradient ? s.rows : p.k;
-            Segment next;
-            if (s.block0 == s.block1) {
-                more = nextSegment(&next);
-            }
-            for (uint32_t b = s.block0; b < s.block1; ++b) {
-                good = BarWait(SmemAddress(full + stage), parity, stop);
-                good = __all_sync(0xFFFFFFFFu, good) != 0;
+        // One lane does it all: with the warp's votes and an election for each block, a block took 570 cycles to issue, and
+        // the tensor cores need 512 of 256 columns, 384 of 192.
+        if (ElectLane()) {
+            const bool leftT = kGradient || leftMn != 0u;
+            const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
+            // 32 bytes of the summed index per instruction: inside a 128-byte row, or as many rows as it has elements
+            const uint32_t leftStep = (leftT ? kStepElements * 128u : 32u) >> 4;
+            const uint32_t rightStep = (kGradient ? kStepElements * 128u : 32u) >> 4;
+            const uint64_t leftBase = OperandDescriptor(ring, 8192u);
+            const uint64_t rightBase = OperandDescriptor(ring + kLeftBytes, 8192u);
+            uint32_t stage = 0;
+            uint32_t parity = 0;
+            uint32_t tile = 0;
+            uint32_t cuts = 0;  // a bit per stage: the parity of its next cut block
+            bool good = true;
+            struct Work {
+                uint32_t columns, length, block0, block1;
+            };
+            // What this lane needs of the next segment; false at the end.
+            auto take = [&](Work* w) {
+                const uint32_t i = taken % kSegments;
+                if (!BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop)) {
+                    good = false;
+                    return false;
+                }
+                const Segment& s = segments[i];
+                *w = Work{s.columns, kGradient ? s.rows : p.k, s.block0, s.block1};
+                const bool more = s.parts != 0u;
+                BarArrive(SmemAddress(segmentEmpty + i));
+                ++taken;
+                return more;
+            };
+            Work w;
+            bool more = take(&w);
+            while (more) {
+                const uint32_t half = tile & 1u;
+                good = BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop);
                 if (!good) {
                     break;
                 }
-                const uint32_t left = ring + stage * R::kStageBytes;
-                const uint32_t right = left + kLeftBytes;
-                const uint32_t valid = length - b * kBlock < kBlock ? length - b * kBlock : kBlock;
-                const uint32_t steps = (valid + kStepElements - 1u) / kStepElements;
-                if constexpr (kGradient) {
-                    if (valid % kStepElements != 0u) {
-                        good = __all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop)) != 0;
-                        cuts ^= 1u << stage;
-                        if (!good) {
-                            break;
+                ++tile;
+                TmemFenceAfter();
+                const uint32_t d = tmem + half * kColumns;
+                const uint32_t instruction = shape | MmaColumns((w.columns + kColumnStep - 1u) / kColumnStep * kColumnStep);
+                Work next;
+                if (w.block0 == w.block1) {
+                    more = take(&next);
+                }
+                for (uint32_t b = w.block0; b < w.block1; ++b) {
+                    good = BarWait(SmemAddress(full + stage), parity, stop);
+                    if (!good) {
+                        break;
+                    }
+                    const uint32_t valid = w.length - b * kBlock < kBlock ? w.length - b * kBlock : kBlock;
+                    if constexpr (kGradient) {
+                        if (valid % kStepElements != 0u) {
+                            good = BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop);
+                            cuts ^= 1u << stage;
+                            if (!good) {
+                                break;
+                            }
                         }
                     }
-                }
-                if (ElectLane()) {
-                    const uint64_t a = OperandDescriptor(left, 8192u);
-                    const uint64_t w = OperandDescriptor(right, 8192u);
+                    const uint64_t left = leftBase + stage * (R::kStageBytes >> 4);
+                    const uint64_t right = rightBase + stage * (R::kStageBytes >> 4);
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) {
-                        if (i < steps) {
-                            Mma<kInt8, kCtas>(d, a + i * leftStep, w + i * rightStep, instruction,
-                                              b != s.block0 || i != 0u ? 1u : 0u);
+                        if (i * kStepElements < valid) {
+                            Mma<kInt8, kCtas>(d, left + i * leftStep, right + i * rightStep, instruction,
+                                              b != w.block0 || i != 0u ? 1u : 0u);
                         }
                     }
                     MmaCommit<kCtas>(SmemAddress(empty + stage));
+                    if (b == w.block0) {
+                        more = take(&next);  // while this tile computes
+                    }
+                    stage = stage + 1u == R::kStages ? 0u : stage + 1u;
+                    parity ^= stage == 0u ? 1u : 0u;
                 }
-                if (b == s.block0) {
-                    more = nextSegment(&next);  // while this tile computes
+                if (!good) {
+                    break;
                 }
-                stage = stage + 1u == R::kStages ? 0u : stage + 1u;
-                parity ^= stage == 0u ? 1u : 0u;
-            }
-            if (good && ElectLane()) {
                 MmaCommit<kCtas>(SmemAddress(sumsFull + half));
+                w = next;
             }
-            __syncwarp();
-            more = more && good;
-            s = next;
+            if (!good) {  // not under instructions that still read tensor memory
+                uint32_t never = 0;
+                MmaCommit<kCtas>(SmemAddress(&drained));
+                (void)BarWait(SmemAddress(&drained), 0, &never);
+            }
         }
-        if (!good && ElectLane()) {  // not under instructions that still read tensor memory
-            uint32_t never = 0;
-            MmaCommit<kCtas>(SmemAddress(&drained));
-            (void)BarWait(SmemAddress(&drained), 0, &never);
-        }
+        __syncwarp();
     } else if (kGradient && warp == 2) {
         Segment s;
         uint32_t block = 0;  // of all that this CTA loads: the stage is block % kStages
