@@ -14,7 +14,11 @@
  * 256 results: each holds 128 rows of the dense matrix and half of the ragged rows,
  * and one MMA reads both.  A single CTA would have to load 48 KB for 512 cycles of
  * MMA, more than the 52 bytes per cycle that an SM was measured to get from L2 with
- * all of them loading; the pair loads 32 KB each (16384 x 4096 x 4096: 1500 TFLOP/s).
+ * all of them loading; the pair loads 32 KB each.  A block of a pair then takes 0.39 us
+ * (0.28 us of MMAs alone, 0.27 us of loads alone): what bounds it is shared memory, which
+ * the loads write while the MMAs read it.  One group of 18944 rows, 1024 x 8192: 1500
+ * TFLOP/s; 8192 rows of 16 groups, 2048 x 4096, run 200 times without a pause at the clock
+ * that the power limit leaves: 133 us, 1030 TFLOP/s.
  *
  * CTAs are persistent: warp 0 loads blocks of 128 bytes of the summed index into a
  * ring of stages, one lane of warp 1 issues the MMAs, warps from 4 on read the
@@ -169,7 +173,7 @@ __device__ __forceinline__ void StoreForward(const AclspGroupedParams& p, void* 
 // Gradient: the lane is a row of C_g, the sixteen values are neighbours in it.  Called by whole warps.  Where the rows
 // are aligned, each lane writes its own in whole sectors; elsewhere (odd widths, a last column tile) the warp turns the
 // values round in shared memory and writes rows element by element, sixteen lanes to one: a lane at a time to its own row
-// would send every element to the memory by itself (2047 x 2049 from 8192 rows: 306 us).
+// would send every element to the memory by itself (2047 x 2049 from 8192 rows: 306 us, turned round 113 us).
 template <typename T>
 __device__ __forceinline__ void StoreGradient(const AclspGroupedParams& p, void* c, const Segment& s, uint32_t row,
                                               uint32_t j0, const Lane16& sums, float laneScale, float beta, uint32_t turn)
@@ -445,7 +449,8 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
         }
     } else if (warp == 1 && rank == 0u) {
         // One lane does it all: with the warp's votes and an election for each block, a block took 570 cycles to issue, and
-        // the tensor cores need 512 of 256 columns, 384 of 192.
+        // the tensor cores need 512 for 256 columns, 384 for 192 (1024 x 1024 gradients of 2 x 4096 rows: 36.6 us then, 31.0
+        // now).
         if (ElectLane()) {
             const bool leftT = kGradient || leftMn != 0u;
             const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
@@ -631,8 +636,8 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             if (kGradient && s.parts == 1u && outMapped != 0u && beta == 0.0f) {
                 if constexpr (kGradient) {
                     // Through shared memory and TMA, two boxes per warp under way: the stores of a tile take longer than
-                    // its short sums, and the warp that issues them itself waits for each (8192 rows of 16 groups, 4096 x
-                    // 2048: 147 us).
+                    // short sums, and a warp that issues them itself waits for each (2000 rows of 64 groups, 512 x 1024 fp16:
+                    // 25.5 us with its own stores, 18.4 so).
                     WithOutType(p.outType, [&](auto type) {
                         using T = decltype(type);
                         constexpr uint32_t kBoxColumns = 128u / sizeof(T);
@@ -717,8 +722,9 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             if (kGradient && ElectLane()) {
                 StoresRead<0>();  // the room may be needed again
             }
-            __threadfence();
+            // the warp's sums first, then the fence of the lanes that count them
             __syncwarp();
+            __threadfence();
             const uint32_t pieces = s.columns > firstChunk ? (s.columns - firstChunk + kChunkStep - 1u) / kChunkStep : 0u;
             uint32_t lasts = 0;
             uint32_t* const tileCounters = counters + (s.counter * kCtas + rank) * kTileCounters + warp % 4u;
@@ -739,6 +745,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                     lasts = __ballot_sync(0xFFFFFFFFu, last);
                     if (lasts != 0u) {
                         __threadfence();
+                        __syncwarp();
                     }
                 }
                 if ((lasts >> inTwo & 1u) == 0u) {
@@ -992,13 +999,15 @@ bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffe
             !Encode(&right, p.inType, bases[1], 2, rightSizes, rightStride, 64)) {
             return false;
         }
-        // results through TMA where C allows it
+        // Results through TMA where C allows it.  A store that ends behind the last column, between two multiples of 16
+        // bytes, was seen to write on to the next one, so the rows must end on one.
         CUtensorMap out;
         const uint64_t outBytes = p.outType == ACLSP_TYPE_F32 ? 4u : 2u;
         const uint64_t outSizes[3] = {p.n, p.m, p.groups};
         const uint64_t outStrides[2] = {static_cast<uint64_t>(p.ldc),
                                         static_cast<uint64_t>(p.groups > 1u ? p.cBatchStride : p.ldc)};
-        const bool outMapped = reinterpret_cast<uintptr_t>(c) % 16u == 0u && outStrides[0] * outBytes % 16u == 0u &&
+        const bool outMapped = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.n * outBytes % 16u == 0u &&
+                               outStrides[0] * outBytes % 16u == 0u &&
                                outStrides[1] * outBytes % 16u == 0u && outStrides[0] * outBytes < kFarthest &&
                                outStrides[1] * outBytes < kFarthest &&
                                Encode(&out, p.outType, c, 3, outSizes, outStrides, 32);

@@ -699,3 +699,137 @@ def test_training_step_replays_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(77, 301), (300, 1021), (513, 129)])
+def test_gradient_odd_widths_in_aligned_rows(out, m, n):
+    """Rows of C that start on multiples of 16 bytes but end between them: what is behind each stays."""
+    wide = -(-n // 8) * 8
+    Gradient([150, 0, 1, 700, 64, 65], m, n, torch.bfloat16, out, pad=(-m % 8, wide - n, wide - n + 8), first=3, behind=40,
+             seed=m, batch_pad=8).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", [L.ORDER_ROW, L.ORDER_COL])
+@pytest.mark.parametrize("k,n", [(77, 301), (200, 13), (1033, 130)])
+def test_forward_odd_widths_in_aligned_rows(dtype, order, k, n):
+    """What lies between the rows of A and B is in no sum, and what lies between those of C stays."""
+    pad_b = -(k if order == L.ORDER_ROW else n) % 16
+    case = Forward([40, 0, 9, 300], k, n, dtype, order=order, pad=(-k % 16, pad_b, -n % 16), seed=k, batch_pad=-n % 16)
+    a, c = (t.as_strided((t.shape[0], t.stride(0)), (t.stride(0), 1)) for t in (case.a, case.c))
+    every = case.w if order == L.ORDER_ROW else case.w.transpose(1, 2)
+    w = every.as_strided((*every.shape[:2], every.stride(1)), every.stride())
+    poison = 127 if dtype == torch.int8 else float("nan")
+    a[:, k:] = poison
+    w[:, :, every.shape[2]:] = poison
+    c0 = c.clone()
+    case.check()
+    assert torch.equal(c[:, n:], c0[:, n:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_operands_of_odd_widths_in_aligned_rows(dtype):
+    case = Gradient([40, 0, 9, 300], 77, 301, dtype, pad=(3, 3, 3), seed=77)
+    for t in (case.a, case.b):
+        t.as_strided((t.shape[0], t.stride(0)), (t.stride(0), 1))[:, t.shape[1]:] = float("nan")
+    case.check()
+
+
+@pytest.mark.parametrize("groups", [31, 33, 300])
+def test_forward_and_gradient_of_many_groups(groups):
+    sizes = [(7 * g) % 41 if g % 3 else 0 for g in range(groups)]
+    Forward(sizes, 72, 1032, torch.bfloat16, first=1, behind=2, seed=groups).check()
+    Gradient(sizes, 136, 264, torch.bfloat16, first=1, behind=2, seed=groups).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,k,n", [([1], 16400, 264), ([2, 0, 5], 8208, 40), ([300], 12304, 264)])
+def test_forward_long_sums_of_few_tiles(dtype, sizes, k, n):
+    """Tiles split along the summed index into as many parts as there are CTAs for them, the last one short."""
+    Forward(sizes, k, n, dtype, scales=True, seed=k).check()
+
+
+@pytest.mark.parametrize("extra", [0, 1])
+def test_operands_beyond_32_bits(extra):
+    """Rows and matrices whose distance times their number passes 2^32 elements, aligned and not."""
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    rows, k, n, ld = 40, 72, 136, 2 ** 27 + extra
+    far = torch.empty((rows - 1) * ld + 160, dtype=torch.bfloat16, device=DEV)
+    apart = 2 ** 31 + 8 + extra
+    matrices = torch.empty(2 * apart + n * k, dtype=torch.bfloat16, device=DEV)
+    x = torch.as_strided(far, (rows, k), (ld, 1))
+    w = torch.as_strided(matrices, (3, n, k), (apart, k, 1))
+    x0, w0 = randn(rows, k, dtype=torch.bfloat16, gen=gen), randn(3, n, k, dtype=torch.bfloat16, gen=gen)
+    x.copy_(x0)
+    w.copy_(w0)
+    bounds = [0, 11, 11, rows]
+    offsets = torch.tensor(bounds, dtype=torch.int32, device=DEV)
+    want, size = torch.zeros(rows, n, dtype=torch.float64, device=DEV), torch.zeros(rows, n, dtype=torch.float64, device=DEV)
+    for g in range(3):
+        part = slice(bounds[g], bounds[g + 1])
+        want[part] = x0[part].double() @ w0[g].double().T
+        size[part] = x0[part].double().abs() @ w0[g].double().abs().T
+    y = A.grouped_mm(x, w, offsets)
+    close(y, want, sum_bound(k, size, False))
+    # the same rows as the result of a product, and the same matrices as that of a gradient
+    c = torch.as_strided(far, (rows, n), (ld, 1))
+    api.GroupedMM(api.Handle(), api.DnMat(rows, k, k, x0), api.DnMat(n, k, k, w0, L.ORDER_ROW, 3, n * k),
+                  api.DnMat(rows, n, ld, c), offsets, L.OP_T)()
+    close(c, want, sum_bound(k, size, False))
+    dy = randn(rows, n, dtype=torch.bfloat16, gen=gen)
+    api.GroupedMMWeightGrad(api.Handle(), api.DnMat(rows, n, n, dy), api.DnMat(rows, k, k, x0),
+                            api.DnMat(n, k, k, matrices, L.ORDER_ROW, 3, apart), offsets)()
+    for g in range(3):
+        part = slice(bounds[g], bounds[g + 1])
+        close(w[g], dy[part].double().T @ x0[part].double(),
+              sum_bound(rows, dy[part].double().abs().T @ x0[part].double().abs(), False))
+    q, scales = A.quantize_rows(torch.as_strided(far, (rows, n), (ld, 1)))
+    want_q, want_scales = quantized(c)
+    assert torch.equal(q, want_q) and torch.equal(scales, want_scales)
+
+
+def test_products_on_two_streams_at_once():
+    """Each with its own buffer: a long product and many short ones, split and joined, side by side."""
+    long = Forward([3000, 1, 2000], 1024, 2048, torch.bfloat16, seed=1)
+    short = Forward([2], 8208, 264, torch.bfloat16, seed=2)
+    grad = Gradient([900, 0, 300], 256, 264, torch.bfloat16, seed=3)
+    cases = [long, short, grad]
+    wants = []
+    for case in cases:
+        case.op()
+        torch.cuda.synchronize()
+        wants.append(case.c.clone())
+    streams = [torch.cuda.Stream() for _ in cases]
+    for case, stream in zip(cases, streams):
+        case.op.handle = api.Handle(stream)
+        case.c.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for case, times in ((long, 1), (short, 5), (grad, 3)):
+            for _ in range(times):
+                case.op()
+    torch.cuda.synchronize()
+    for case, want in zip(cases, wants):
+        assert torch.equal(case.c, want)
+        assert case.op.wait_failures() == 0
+
+
+def test_eager_and_replayed_products_take_turns_over_one_buffer():
+    case = Forward([5, 0, 70], 4104, 264, torch.bfloat16, seed=4)
+    case.op.preprocess()
+    case.op()
+    want = case.c.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    eager, handle = case.op.handle, api.Handle(side)
+    graph = torch.cuda.CUDAGraph()
+    case.op.handle = handle
+    with torch.cuda.graph(graph, stream=side):
+        case.op()
+        case.op()
+    case.op.handle = eager
+    for turn in range(6):
+        case.c.zero_()
+        graph.replay() if turn % 2 else case.op()
+        assert torch.equal(case.c, want)
