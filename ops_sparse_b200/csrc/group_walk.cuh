@@ -72,25 +72,43 @@ public:
         return true;
     }
 
-    // Number of tiles in all groups; walks to the end.
-    __device__ __forceinline__ uint32_t Count()
+    // Number of tiles in all groups.  Asked for before the first tile, so each lane takes eight groups at a time, whose
+    // loads are under way together (256 rows over 512 groups, 1024 x 1024 matrices: 69 us, 78 with a walk of 32 groups at a
+    // time).
+    __device__ __forceinline__ uint32_t Count() const
     {
-        while (base_ + 32u < groups_) {
-            base_ += 32u;
-            Load();
+        constexpr uint32_t kEach = 8;
+        if (groups_ <= 32u) {
+            return end_;
         }
-        return end_;
-    }
-
-    // Back to the first group; tiles may be asked for from the beginning again.
-    __device__ __forceinline__ void Restart()
-    {
-        if (base_ != 0u) {
-            base_ = 0;
-            end_ = 0;
-            reached_ = 0;
-            Load();
+        uint32_t sum = 0;
+        uint32_t reached = 0;
+        for (uint32_t base = 0; base < groups_; base += 32u * kEach) {
+            const uint32_t g0 = base + threadIdx.x % 32u * kEach;
+            uint32_t bounds[kEach + 1];
+            uint32_t top = 0;
+#pragma unroll
+            for (uint32_t i = 0; i <= kEach; ++i) {
+                bounds[i] = g0 < groups_ && g0 + i <= groups_ ? Clamp(__ldg(offsets_ + g0 + i)) : 0u;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i <= kEach; ++i) {
+                top = bounds[i] > top ? bounds[i] : top;
+            }
+            top = RunningMax(top);
+            uint32_t before = __shfl_up_sync(0xFFFFFFFFu, top, 1);
+            before = threadIdx.x % 32u == 0u || before < reached ? reached : before;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t begin = bounds[i] > before ? bounds[i] : before;
+                const uint32_t size = bounds[i + 1] > begin ? bounds[i + 1] - begin : 0u;  // none behind the last group
+                sum += (size + tileRows_ - 1u) / tileRows_;
+                before = begin > bounds[i + 1] ? begin : bounds[i + 1];
+            }
+            const uint32_t last = __shfl_sync(0xFFFFFFFFu, top, 31);
+            reached = last > reached ? last : reached;
         }
+        return __reduce_add_sync(0xFFFFFFFFu, sum) * across_;
     }
 
 private:
@@ -99,6 +117,16 @@ private:
     __device__ __forceinline__ uint32_t Clamp(int32_t v) const
     {
         return v < 0 ? 0u : (static_cast<uint32_t>(v) > rows_ ? rows_ : static_cast<uint32_t>(v));
+    }
+
+    // The largest value of the lanes up to this one.
+    static __device__ __forceinline__ uint32_t RunningMax(uint32_t v)
+    {
+        for (uint32_t d = 1; d < 32u; d *= 2u) {
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            v = threadIdx.x % 32u >= d && up > v ? up : v;
+        }
+        return v;
     }
 
     __device__ __forceinline__ void Load()
@@ -115,10 +143,7 @@ private:
         }
         // ascending ends: the largest offset up to and including this group's end
         uint32_t top = first > last ? first : last;
-        for (int d = 1; d < 32; d *= 2) {
-            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, top, d);
-            top = static_cast<int>(lane) >= d && up > top ? up : top;
-        }
+        top = RunningMax(top);
         uint32_t before = __shfl_up_sync(0xFFFFFFFFu, top, 1);
         before = lane == 0 ? 0u : before;
         before = before > reached_ ? before : reached_;

@@ -60,7 +60,6 @@ public:
           tileLanes_(tileLanes), blocks_(blocks), length_(blocks)
     {
         tiles_ = walk_.Count();
-        walk_.Restart();
         tile_ = workers.index;
         whole_ = tiles_ / workers.count * workers.count;
         const uint32_t left = tiles_ - whole_;

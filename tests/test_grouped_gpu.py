@@ -190,6 +190,24 @@ def test_forward_bad_offsets_stay_inside(bounds):
     close(case.c, want, sum_bound(case.k, size, False))
 
 
+@pytest.mark.parametrize("groups", [40, 256, 257, 600])
+def test_forward_bad_offsets_of_many_groups(groups):
+    """Both walks over the groups, the one that counts the tiles and the one that finds them, clamp alike."""
+    case = Forward([3] * groups, 40, 264, torch.bfloat16, seed=groups)
+    rows = 3 * groups
+    steps = torch.randint(-40, 61, (groups + 1,), generator=torch.Generator().manual_seed(groups))
+    bounds = (torch.arange(groups + 1) * rows // groups + steps).tolist()
+    case.offsets.copy_(torch.tensor(bounds, dtype=torch.int32))
+    case.op()
+    torch.cuda.synchronize()
+    top, clean = 0, []
+    for b in [min(max(v, 0), rows) for v in bounds]:
+        top = max(top, b)
+        clean.append(top)
+    want, size = case.expected(bounds=clean)
+    close(case.c, want, sum_bound(case.k, size, False))
+
+
 def test_forward_special_values_stay_in_their_rows():
     """Infinities and NaN in one group's rows, and in the rows behind it, do not reach another row."""
     case = Forward([20, 20, 20], 96, 64, torch.bfloat16)
