@@ -113,6 +113,8 @@ aclsparseStatus_t aclsparseB200DnMatSetClosingBarrier(aclsparseDnMatDescr_t mat,
  *   types  A, B fp16 or bf16 with C of that type or fp32: fp32 sums; A, B int8 with C fp32, fp16 or bf16: exact
  *         int32 sums, k <= 131071.  The compute type is ACL_FLOAT.  The result is formed in fp32 and rounded once
  *         to the type of C.  Others, also mirrors and closing barriers on C: NOT_SUPPORTED.
+ * A and B should start on multiples of 16 bytes: rows of any width and leading dimension run on the tensor cores, a
+ * matrix that is merely shifted does not and takes many times as long.
  * Rows of C outside [groupOffsets[0], groupOffsets[groups]) are left as they are; beta == 0 does not read C; an
  * empty group costs nothing; k == 0 gives beta * C.  C must not overlap A or B.  Results do not depend on
  * scheduling.  The buffer holds partial sums of products split along k: 64-byte aligned, one call at a time.

@@ -279,6 +279,16 @@ def _batch_descr(w: torch.Tensor):
     return api.DnMat(rows, cols, ld, w, order, groups, w.stride(0) if groups > 1 else 0)
 
 
+def _loadable(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy where its first element alone keeps its rows from multiples of 16 bytes.
+
+    The tensor-core kernels load from such multiples.  Rows of odd widths are copied by the library, in the buffer, but
+    that has no room for an operand that is merely shifted.
+    """
+    even = all(s == 1 or s * t.element_size() % 16 == 0 for s in t.stride())
+    return t.clone() if even and t.data_ptr() % 16 else t
+
+
 def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=None):
     """x[r] @ op(weight[g]); rows in no group are zero."""
     from . import api
@@ -287,7 +297,7 @@ def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=No
         y = torch.zeros(x.size(0), n, dtype=out_dtype, device=x.device)
         if y.numel():
             with _stream_handle() as handle:
-                api.GroupedMM(handle, _rows_descr(x), _batch_descr(weight), _rows_descr(y),
+                api.GroupedMM(handle, _rows_descr(_loadable(x)), _batch_descr(_loadable(weight)), _rows_descr(y),
                               None if offsets is None else offsets.contiguous(), op_b, row_scales, col_scales)()
     return y
 
@@ -311,7 +321,7 @@ class _GroupedMM(torch.autograd.Function):
                 dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
                 if dw.numel():
                     with _stream_handle() as handle:
-                        api.GroupedMMWeightGrad(handle, _rows_descr(dy), _rows_descr(x), _batch_descr(dw),
+                        api.GroupedMMWeightGrad(handle, _rows_descr(_loadable(dy)), _rows_descr(_loadable(x)), _batch_descr(dw),
                                                 None if offsets is None else offsets.contiguous())()
         return dx, dw, None, None
 

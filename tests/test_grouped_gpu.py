@@ -693,6 +693,27 @@ def test_gradient_of_a_broadcast_result():
     close(x1.grad, want, sum_bound(16, size, False))
 
 
+@pytest.mark.parametrize("shift", [1, 8])
+def test_shifted_operands_give_the_same(shift):
+    """Views that start between two multiples of 16 bytes are computed in the same way as aligned ones."""
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    offsets = torch.tensor([0, 70, 70, 200], dtype=torch.int32, device=DEV)
+
+    def shifted(t):
+        store = torch.empty(t.numel() + shift, dtype=t.dtype, device=DEV)
+        return store[shift:].view(t.shape).copy_(t)
+
+    x, w = randn(200, 1040, dtype=torch.bfloat16, gen=gen), randn(3, 96, 1040, dtype=torch.bfloat16, gen=gen)
+    dy = randn(200, 96, dtype=torch.bfloat16, gen=gen)
+    got = []
+    for put in (lambda t: t, shifted):
+        a, b = put(x).requires_grad_(), put(w).requires_grad_()
+        y = A.grouped_mm(a, b, offsets)
+        got.append((y, *torch.autograd.grad(y, (a, b), put(dy))))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_training_step_replays_in_a_graph():
     gen = torch.Generator(device=DEV).manual_seed(10)
     offsets = torch.tensor([0, 30, 30, 64], dtype=torch.int32, device=DEV)
