@@ -171,73 +171,104 @@ __device__ __forceinline__ uint32_t WordOf(const unsigned char* at, const unsign
 
 constexpr uint32_t kCopyThreads = 256;
 
+// Division of numbers below 2^31 by a divisor known to the host, which makes factor = floor(2^(31 + bits) / divisor) + 1
+// with 2^(bits - 1) < divisor <= 2^bits: the quotient's error, number / 2^(31 + bits) at most, is less than 1 / divisor.
+struct Divisor {
+    uint64_t factor;
+    uint32_t shift;
+    uint32_t divisor;
+    __device__ __forceinline__ uint64_t Quotient(uint64_t v) const
+    {
+        return v >> 31 == 0u ? static_cast<uint32_t>(v) * factor >> shift : v / divisor;
+    }
+};
+
+Divisor DivisorOf(uint32_t d)
+{
+    uint32_t bits = 0;
+    while ((1ull << bits) < d) {
+        ++bits;
+    }
+    return Divisor{(1ull << (31u + bits)) / d + 1u, 31u + bits, d};
+}
+
 // Rows to copy, in bytes.
 struct CopyJob {
     const unsigned char* src;
     unsigned char* dst;
-    uint32_t rows;
+    Divisor rows;
     uint32_t batches;
     int64_t rowBytes;
     int64_t pitch;
     int64_t batchPitch;
-    int64_t dstPitch;
+    Divisor dstVectors;  // of 16 bytes, in a row
     int64_t dstBatchPitch;
 };
 struct CopyJobs {
     CopyJob job[2];
 };
 
-// A thread per 16 bytes of a copied row: it reads the five aligned words that they come from, shifts the bytes into place
-// and writes one vector, the last of a row with what lies behind it.  Bound by HBM: every byte is read and written once
-// (neighbours' common words come from L1).  One launch for both operands: blockIdx.y is the job.  Measured and left: a
-// warp per row (one stretch of it under way at a time: 13 us for 51 rows of 4462 bytes), and a warp per 512 bytes of a
-// row (short last stretches, 11 us for 5005 rows of 1554 bytes).
-__global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const CopyJobs jobs, const int32_t* offsets,
-                                                               uint32_t offsetRows)
+// A thread per 16 bytes of a copied row: it reads the two aligned vectors that they come from, shifts them into place
+// and writes one, the last of a row with what lies behind it.  Every byte is read from memory and written once; the second
+// vector is the next thread's first and comes from L1.  One launch for both operands: blockIdx.y is the job.  Bound by
+// instructions more than by HBM: 52 matrices of 880 x 1137 fp16, 104 MB, 39 us (70 with five words in place of the two
+// vectors, divisions by the hardware's integer code and a grid of eight blocks per SM, which idled where matrices are
+// left out).  Measured and left: two to four vectors of a thread under way together (fewer threads then: 84 to 104 us with
+// the product, 70 so), going down the rows from a fixed place in them, without divisions (105 us), a warp per row
+// (13 us for 51 rows of 4462 bytes), and a warp per 512 bytes of a row (short last stretches, 11 us for 5005 rows of 1554
+// bytes).
+__global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const __grid_constant__ CopyJobs jobs, const int32_t* offsets)
 {
     aclsp::WaitForPreviousKernel();
     aclsp::LetNextKernelStart();
     const CopyJob& c = jobs.job[blockIdx.y];
-    const uint32_t vectors = static_cast<uint32_t>(c.dstPitch / 16);
-    const uint64_t all = static_cast<uint64_t>(c.rows) * c.batches * vectors;
-    const bool fewer = all >> 32 == 0u;  // 32-bit divisions do
-    const unsigned char* const end = c.src + (c.batches - 1) * c.batchPitch + (c.rows - 1) * c.pitch + c.rowBytes;
+    const uint32_t vectors = c.dstVectors.divisor;
+    const uint32_t rows = c.rows.divisor;
+    const uint64_t all = static_cast<uint64_t>(rows) * c.batches * vectors;
+    const unsigned char* const end = c.src + (c.batches - 1) * c.batchPitch + (rows - 1) * c.pitch + c.rowBytes;
     const uint64_t threads = static_cast<uint64_t>(gridDim.x) * kCopyThreads;
 #pragma unroll 2
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < all; i += threads) {
-        uint64_t row = fewer ? static_cast<uint32_t>(i) / vectors : i / vectors;
+        uint64_t row = c.dstVectors.Quotient(i);
         const int64_t byte = static_cast<int64_t>(i - row * vectors) * 16;
         uint32_t batch = 0;
         if (c.batches > 1u) {
-            batch = fewer ? static_cast<uint32_t>(row) / c.rows : static_cast<uint32_t>(row / c.rows);
-            row -= static_cast<uint64_t>(batch) * c.rows;
-            uint32_t first, last;
-            aclsp::GroupRows(offsets, batch, offsetRows, &first, &last);
-            if (first == last) {
+            batch = static_cast<uint32_t>(c.rows.Quotient(row));
+            row -= static_cast<uint64_t>(batch) * rows;
+            if (__ldg(offsets + batch) >= __ldg(offsets + batch + 1)) {
                 continue;  // nobody reads this matrix
             }
         }
         const unsigned char* from = c.src + batch * c.batchPitch + static_cast<int64_t>(row) * c.pitch + byte;
-        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 3u;
+        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
         from -= shift;
-        uint32_t w[5];
-        if (from >= c.src && from + 20 <= end) {
-#pragma unroll
-            for (uint32_t k = 0; k < 5; ++k) {
-                w[k] = __ldg(reinterpret_cast<const uint32_t*>(from) + k);
-            }
+        uint32_t w[8];
+        if (from >= c.src && from + 32 <= end) {
+            const uint4 low = __ldg(reinterpret_cast<const uint4*>(from));
+            const uint4 high = __ldg(reinterpret_cast<const uint4*>(from) + 1);
+            w[0] = low.x, w[1] = low.y, w[2] = low.z, w[3] = low.w;
+            w[4] = high.x, w[5] = high.y, w[6] = high.z, w[7] = high.w;
         } else {  // next to an end of the matrix
 #pragma unroll
-            for (uint32_t k = 0; k < 5; ++k) {
+            for (uint32_t k = 0; k < 8; ++k) {
                 w[k] = WordOf(from + 4 * k, c.src, end);
             }
+        }
+        // by eight bytes, by four, and by what is left of the shift
+#pragma unroll
+        for (uint32_t k = 0; k < 6; ++k) {
+            w[k] = (shift & 8u) != 0u ? w[k + 2] : w[k];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 5; ++k) {
+            w[k] = (shift & 4u) != 0u ? w[k + 1] : w[k];
         }
         uint32_t v[4];
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
-            v[k] = __funnelshift_r(w[k], w[k + 1], 8u * shift);
+            v[k] = __funnelshift_r(w[k], w[k + 1], 8u * (shift & 3u));
         }
-        unsigned char* const to = c.dst + batch * c.dstBatchPitch + static_cast<int64_t>(row) * c.dstPitch + byte;
+        unsigned char* const to = c.dst + batch * c.dstBatchPitch + static_cast<int64_t>(row) * vectors * 16 + byte;
         *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
@@ -260,15 +291,16 @@ void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void
         CopyJob& c = jobs.job[count++];
         c.src = static_cast<const unsigned char*>(*bases[i]);
         c.dst = static_cast<unsigned char*>(buffer) + x->copyOffset;
-        c.rows = static_cast<uint32_t>(x->rows);
+        c.rows = DivisorOf(static_cast<uint32_t>(x->rows));
         c.batches = static_cast<uint32_t>(x->batches);
         c.rowBytes = static_cast<int64_t>(x->rowElements) * bytes;
         c.pitch = static_cast<int64_t>(x->ld) * bytes;
         c.batchPitch = static_cast<int64_t>(x->batchStride) * bytes;
-        c.dstPitch = (c.rowBytes + 15) / 16 * 16;
-        c.dstBatchPitch = c.dstPitch * static_cast<int64_t>(x->rows);
+        const int64_t dstPitch = (c.rowBytes + 15) / 16 * 16;
+        c.dstVectors = DivisorOf(static_cast<uint32_t>(dstPitch / 16));
+        c.dstBatchPitch = dstPitch * static_cast<int64_t>(x->rows);
         *bases[i] = c.dst;
-        x->ld = static_cast<uint64_t>(c.dstPitch / bytes);
+        x->ld = static_cast<uint64_t>(dstPitch / bytes);
         x->batchStride = x->rows * x->ld;
     }
     if (count == 0u) {
@@ -276,7 +308,15 @@ void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void
     }
     AclspCountLaunches(1);
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(148 * 8 / count, count);
+    uint64_t most = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint64_t own = static_cast<uint64_t>(jobs.job[i].rows.divisor) * jobs.job[i].batches * jobs.job[i].dstVectors.divisor;
+        most = own > most ? own : most;
+    }
+    // two vectors to a thread, in large copies more: 24 blocks per SM were measured like 16 and 32
+    constexpr uint64_t kMostBlocks = 148u * 24u;
+    const uint64_t blocks = (most + kCopyThreads * 2u - 1u) / (kCopyThreads * 2u);
+    config.gridDim = dim3(static_cast<uint32_t>(blocks < kMostBlocks ? blocks : kMostBlocks), count);
     config.blockDim = dim3(kCopyThreads);
     config.stream = stream;
     cudaLaunchAttribute early{};
@@ -284,7 +324,7 @@ void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, CopyRowsKernel, jobs, p.offsets, p.rows);
+    cudaLaunchKernelEx(&config, CopyRowsKernel, jobs, p.offsets);
 }
 
 extern "C" uint64_t aclsp_b200_grouped_buffer_bytes(const AclspGroupedParams* params)

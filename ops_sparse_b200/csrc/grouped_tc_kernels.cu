@@ -39,7 +39,7 @@
  * loaded by TMA: they are copied to rows that do first (grouped_kernels.cu), in the
  * buffer.  Warps that bring such rows into shared memory themselves, shifting each word
  * into place, were built and measured: 128 x 128 x 64 blocks took 3000 cycles instead of
- * 256 (2048 x 2049 matrices, 8192 rows: 620 us, with the copy 119 us).
+ * 256 (2048 x 2049 matrices, 8192 rows: 620 us, with the copy 94 us).
  *
  * The set-up of a CTA overlaps the end of the kernel before (programmatic launch); each
  * warp waits for that one's memory before it touches its own.
