@@ -3,13 +3,15 @@
  * and the gradient of those matrices, a sum over a ragged group of rows.
  *
  * The work is done on the tensor cores (grouped_tc_kernels.cu).  Here are the
- * kernels around that: CopyRowsKernel, which brings operands of odd widths to rows
- * that TMA can load, and PlainKernel for what is left: bases that are not 16-byte
+ * kernels around that: FewRowsKernel for a few tokens, CopyRowsKernel, which brings
+ * operands of odd widths to rows that TMA can load, and PlainKernel for what is left:
+ * bases that are not 16-byte
  * aligned, sums over nothing, and sizes beyond 2^28.  It computes 64 x 64 tiles,
  * operands staged through shared memory element by element, products and sums in
  * registers (fp32 FMA; int32 for int8).
  */
 #include <cstdint>
+#include <cstring>
 
 #include <cuda_runtime.h>
 
@@ -154,6 +156,256 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
             }
         }
     }
+}
+
+// ---- products of a few rows ----
+
+constexpr uint32_t kFewThreads = 256;
+constexpr uint32_t kFewDense = 2;  // rows of the dense matrix that a warp reads side by side
+
+// 16 bytes of a row in words, or one element alone in the first; zeros where `in` is false.
+template <uint32_t kBytes>
+struct Words {
+    static constexpr uint32_t kCount = (kBytes + 3u) / 4u;
+    uint32_t w[kCount];
+    __device__ __forceinline__ void Load(const unsigned char* at, bool in)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < kCount; ++i) {
+            w[i] = 0;
+        }
+        if (!in) {
+            return;
+        }
+        if constexpr (kBytes == 16u) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (kBytes == 2u) {
+            w[0] = __ldg(reinterpret_cast<const uint16_t*>(at));
+        } else {
+            w[0] = __ldg(at);
+        }
+    }
+};
+
+// The two 16-bit numbers of a word, exact.
+template <int kIn>
+__device__ __forceinline__ float2 Pair(uint32_t w)
+{
+    if constexpr (kIn == kBF16) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    } else {
+        __half2 h;
+        memcpy(&h, &w, sizeof(h));
+        return __half22float2(h);
+    }
+}
+
+// sum[d][r] += dense[d] . row[r] over the elements of the words.
+template <int kIn, uint32_t kBytes, uint32_t kRows, typename Sum>
+__device__ __forceinline__ void AddProducts(Sum (&sum)[kFewDense][kRows], const Words<kBytes> (&dense)[kFewDense],
+                                            const Words<kBytes> (&row)[kRows])
+{
+#pragma unroll
+    for (uint32_t i = 0; i < Words<kBytes>::kCount; ++i) {
+        if constexpr (kIn == kI8) {
+            // bytes behind a single element are zeros
+#pragma unroll
+            for (uint32_t d = 0; d < kFewDense; ++d) {
+#pragma unroll
+                for (uint32_t r = 0; r < kRows; ++r) {
+                    sum[d][r] = __dp4a(static_cast<int>(dense[d].w[i]), static_cast<int>(row[r].w[i]), sum[d][r]);
+                }
+            }
+        } else {
+            float2 x[kRows];
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                x[r] = Pair<kIn>(row[r].w[i]);
+            }
+#pragma unroll
+            for (uint32_t d = 0; d < kFewDense; ++d) {
+                const float2 w = Pair<kIn>(dense[d].w[i]);
+#pragma unroll
+                for (uint32_t r = 0; r < kRows; ++r) {
+                    sum[d][r] = fmaf(w.x, x[r].x, sum[d][r]);
+                    if constexpr (kBytes == 16u) {
+                        sum[d][r] = fmaf(w.y, x[r].y, sum[d][r]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// The lanes' values v[0 .. kCount), added over the warp: lane 32 / kCount * i gets the sum of v[i].  At each step a lane
+// gives half of its values away and keeps the other half, so that kCount values take little more than one would.
+template <uint32_t kCount, typename Sum>
+__device__ __forceinline__ Sum AddLanes(Sum (&v)[kCount])
+{
+    const uint32_t lane = threadIdx.x % 32u;
+    uint32_t apart = 16;
+#pragma unroll
+    for (uint32_t half = kCount / 2u; half > 0u; half /= 2u) {
+#pragma unroll
+        for (uint32_t i = 0; i < half; ++i) {
+            const bool upper = (lane & apart) != 0u;
+            const Sum keep = upper ? v[i + half] : v[i];
+            const Sum give = upper ? v[i] : v[i + half];
+            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, static_cast<int>(apart));
+        }
+        apart /= 2u;
+    }
+#pragma unroll
+    for (uint32_t d = 16u / kCount; d > 0u; d /= 2u) {
+        v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], static_cast<int>(d));
+    }
+    return v[0];
+}
+
+struct FewOperands {
+    const unsigned char* a;
+    const unsigned char* b;
+    void* c;
+    float alpha;
+    float beta;
+};
+
+// kRows rows of a group from row0 on, of which `count` are its own, times kFewDense rows of its matrix from j0 on.  Called by
+// whole warps.
+template <int kIn, uint32_t kRows>
+__device__ __forceinline__ void FewRows(const AclspGroupedParams& p, const FewOperands& o, uint32_t group, uint32_t row0,
+                                        uint32_t count, uint32_t j0)
+{
+    using Sum = typename Plain<kIn>::Sum;
+    constexpr uint32_t kElement = kIn == kI8 ? 1u : 2u;
+    constexpr uint32_t kPer = 16u / kElement;
+    constexpr uint32_t kTogether = kRows == 4u ? 2u : 4u;  // loads of a row under way
+    const uint32_t lane = threadIdx.x % 32u;
+    const unsigned char* dense[kFewDense];
+    const unsigned char* row[kRows];
+#pragma unroll
+    for (uint32_t d = 0; d < kFewDense; ++d) {  // the last row again where there are no more
+        const uint32_t j = j0 + d < p.n ? j0 + d : p.n - 1u;
+        dense[d] = o.b + (static_cast<int64_t>(group) * p.bBatchStride + static_cast<int64_t>(j) * p.bOuter) * kElement;
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+        row[r] = o.a + static_cast<int64_t>(row0 + (r < count ? r : count - 1u)) * p.aOuter * kElement;
+    }
+    Sum sum[kFewDense][kRows] = {};
+    const uint32_t vectors = p.k / kPer;
+    for (uint32_t v = lane; v < vectors; v += 32u * kTogether) {
+        Words<16> w[kTogether][kFewDense];
+        Words<16> x[kTogether][kRows];
+#pragma unroll
+        for (uint32_t u = 0; u < kTogether; ++u) {
+            const bool in = v + 32u * u < vectors;
+            const int64_t at = static_cast<int64_t>(v + 32u * u) * 16;
+#pragma unroll
+            for (uint32_t d = 0; d < kFewDense; ++d) {
+                w[u][d].Load(dense[d] + at, in);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                x[u][r].Load(row[r] + at, in);
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kTogether; ++u) {
+            AddProducts<kIn, 16, kRows>(sum, w[u], x[u]);
+        }
+    }
+    if (vectors * kPer != p.k) {  // elements behind the last whole vector, fewer than a warp has lanes
+        const uint32_t e = vectors * kPer + lane;
+        Words<kElement> w[kFewDense];
+        Words<kElement> x[kRows];
+#pragma unroll
+        for (uint32_t d = 0; d < kFewDense; ++d) {
+            w[d].Load(dense[d] + static_cast<int64_t>(e) * kElement, e < p.k);
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < kRows; ++r) {
+            x[r].Load(row[r] + static_cast<int64_t>(e) * kElement, e < p.k);
+        }
+        AddProducts<kIn, kElement, kRows>(sum, w, x);
+    }
+    constexpr uint32_t kCount = kFewDense * kRows;
+    Sum all[kCount];
+#pragma unroll
+    for (uint32_t i = 0; i < kCount; ++i) {
+        all[i] = sum[i / kRows][i % kRows];
+    }
+    const float total = static_cast<float>(AddLanes<kCount>(all));
+    const uint32_t mine = lane / (32u / kCount);
+    const uint32_t j = j0 + mine / kRows;
+    if (lane % (32u / kCount) == 0u && j < p.n && mine % kRows < count) {
+        const uint32_t i = row0 + mine % kRows;
+        float scale = o.alpha;
+        if (p.colScales != nullptr) {
+            scale *= __ldg(p.colScales + static_cast<int64_t>(group) * p.n + j);
+        }
+        float s = total * scale;
+        if (p.rowScales != nullptr) {
+            s *= __ldg(p.rowScales + i);
+        }
+        StoreResult(p.outType, o.c, static_cast<int64_t>(i) * p.ldc + j, s, o.beta);
+    }
+}
+
+// A warp takes kFewDense neighbouring rows of a group's matrix and forms their dot products with up to four of the group's
+// rows at a time, fp32 (int32) sums in registers, added over the lanes at the end.  For so few rows reading the matrix is
+// all, and this starts reading as soon as it knows its group: no ring to fill, no tensor memory, no partial sums to
+// join.  Bound by latency, then HBM.  Two tokens, 4 matrices of 1024 x 1024 bf16: 3.4 us (tensor cores: 8.6); one int8
+// token, 4096 x 4096: 3.8 us (8.9); one bf16 token, 4096 x 4096: 7.4 us (11.6).  Only for rows on multiples of 16 bytes:
+// loads of single elements and of shifted vectors were measured, and the tensor cores are faster with the copy (3 rows,
+// 528 x 3823: 18 and 25 us against 12.7).
+template <int kIn>
+__global__ void __launch_bounds__(kFewThreads, 2) FewRowsKernel(const FewOperands operands, const AclspGroupedParams p)
+{
+    aclsp::WaitForPreviousKernel();
+    aclsp::LetNextKernelStart();
+    FewOperands o = operands;
+    o.alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
+    o.beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
+    constexpr uint32_t kWhole = 1u << 30;  // rows of a tile: a group is never cut
+    GroupWalk walk(p.offsets, p.groups, p.rows, kWhole, (p.n + kFewDense - 1u) / kFewDense);
+    const uint32_t warps = gridDim.x * (kFewThreads / 32u);
+    GroupTile tile;
+    for (uint32_t t = blockIdx.x * (kFewThreads / 32u) + threadIdx.x / 32u; walk.Find(t, &tile); t += warps) {
+        const uint32_t j0 = tile.across * kFewDense;
+        for (uint32_t r = 0; r < tile.count; r += 4u) {
+            const uint32_t left = tile.count - r;
+            if (left == 1u) {
+                FewRows<kIn, 1>(p, o, tile.group, tile.row0 + r, 1, j0);
+            } else if (left == 2u) {
+                FewRows<kIn, 2>(p, o, tile.group, tile.row0 + r, 2, j0);
+            } else {
+                FewRows<kIn, 4>(p, o, tile.group, tile.row0 + r, left < 4u ? left : 4u, j0);
+            }
+        }
+    }
+}
+
+template <int kIn>
+void LaunchFewRows(const void* a, const void* b, void* c, const AclspGroupedParams& p, cudaStream_t s)
+{
+    const FewOperands o{static_cast<const unsigned char*>(a), static_cast<const unsigned char*>(b), c, 0.0f, 0.0f};
+    const uint64_t live = p.groups < p.rows ? p.groups : p.rows;
+    const uint64_t units = live * ((p.n + kFewDense - 1u) / kFewDense);
+    const uint64_t blocks = (units + kFewThreads / 32u - 1u) / (kFewThreads / 32u);
+    constexpr uint64_t kMostBlocks = 148u * 8u;
+    AclspCountLaunches(1);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<uint32_t>(blocks < kMostBlocks ? blocks : kMostBlocks));
+    config.blockDim = dim3(kFewThreads);
+    config.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, FewRowsKernel<kIn>, o, p);
 }
 
 // The word at `at`, zeros in place of bytes outside [begin, end).
@@ -343,6 +595,12 @@ extern "C" void aclsp_b200_grouped_mm_kernel_do(const void* a, const void* b, vo
 {
     const AclspGroupedParams& p = *params;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (AclspGroupedFewRows(p) && (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 16u == 0u) {
+        (p.inType == ACLSP_TYPE_F16    ? LaunchFewRows<kF16>
+         : p.inType == ACLSP_TYPE_BF16 ? LaunchFewRows<kBF16>
+                                       : LaunchFewRows<kI8>)(a, b, c, p, s);
+        return;
+    }
     if (AclspGroupedTensorLaunch(a, b, c, buffer, p, s)) {
         return;
     }

@@ -19,6 +19,10 @@ constexpr uint32_t kGroupedCountersEnd = 4u * (kGroupedHeaderWords + aclsp::kGro
 constexpr uint32_t kJoinBlocks = 8;
 constexpr uint32_t kJoinBlocksWide = 48;
 
+// Forward products of so few rows that a kernel without tensor cores (grouped_kernels.cu) is faster, where the bases too
+// are on multiples of 16 bytes.  They need no partial sums.
+bool AclspGroupedFewRows(const AclspGroupedParams& p);
+
 // Columns of a tile: rows of a group that one tile takes (forward), columns of C_g (gradient).
 uint32_t AclspGroupedColumns(const AclspGroupedParams& p);
 

@@ -153,6 +153,49 @@ def test_forward_many_waves_of_tiles(dtype, sizes, k, n):
     Forward(sizes, k, n, dtype, seed=n, first=1, behind=2).check()
 
 
+FEW = [[1], [2], [3], [4], [5], [8], [1, 0, 2, 4, 1], [0, 3, 0, 5, 0], [0] * 40 + [2] + [0] * 30 + [5, 1], [2] * 8, [9, 0, 0, 0, 3]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes", FEW)
+@pytest.mark.parametrize("k,n", [(64, 128), (1040, 97), (16, 1), (2064, 1030)])
+def test_forward_few_rows(dtype, sizes, k, n):
+    Forward(sizes, k, n, dtype, first=1, behind=1, scales=True, seed=k).check(0.5)
+
+
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                       (torch.int8, torch.float32), (torch.int8, torch.float16), (torch.int8, torch.bfloat16)])
+@pytest.mark.parametrize("alpha,beta,scales", [(1.0, 1.0, False), (-0.5, 0.25, True), (0.0, 2.0, False)])
+def test_forward_few_rows_scalars(dtype, out, alpha, beta, scales):
+    case = Forward([3, 0, 1], 160, 145, dtype, out, scales=scales, pad=(16, 16, 3))
+    case.check(alpha * 2.0 ** -12 if dtype == torch.int8 else alpha, beta)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [1, 7, 17, 77, 1033])
+@pytest.mark.parametrize("shift", [(0, 0, 0), (1, 0, 0), (0, 1, 1)])
+def test_forward_few_rows_of_odd_widths(dtype, k, shift):
+    """Rows on multiples of 16 bytes that end between them, with NaN behind; and the same from shifted bases."""
+    case = Forward([2, 0, 5], k, 40, dtype, pad=(-k % 16, -k % 16, 0), shift=shift, seed=k)
+    for t in (case.a, case.w):
+        full = t.as_strided((*t.shape[:-1], t.stride(-2)), t.stride(), t.storage_offset())
+        full[..., k:] = 127 if dtype == torch.int8 else float("nan")
+    case.check()
+
+
+def test_forward_few_rows_bad_offsets_and_special_values():
+    case = Forward([2, 2, 2], 64, 48, torch.bfloat16)
+    case.a[4] = float("inf")
+    case.w[1] = float("nan")
+    case.offsets.copy_(torch.tensor([-5, 4, 2, 2 ** 31 - 1], dtype=torch.int32))
+    case.op()
+    torch.cuda.synchronize()
+    want, size = case.expected(bounds=[0, 4, 4, 6])
+    rows = [0, 1, 2, 3, 5]
+    close(case.c[rows], want[rows], sum_bound(case.k, size[rows], False))
+    assert not torch.isfinite(case.c[4]).any()
+
+
 def test_forward_rows_outside_the_groups_stay():
     Forward([5, 0, 70], 64, 64, torch.bfloat16, first=7, behind=300).check()
 
