@@ -826,7 +826,8 @@ def test_forward_and_gradient_of_many_groups(groups):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("sizes,k,n", [([1], 16400, 264), ([2, 0, 5], 8208, 40), ([300], 12304, 264)])
+@pytest.mark.parametrize("sizes,k,n", [([1], 16400, 264), ([2, 0, 5], 8208, 40), ([20], 16400, 264), ([18, 0, 5, 30], 8208, 40),
+                                       ([300], 12304, 264)])
 def test_forward_long_sums_of_few_tiles(dtype, sizes, k, n):
     """Tiles split along the summed index into as many parts as there are CTAs for them, the last one short."""
     Forward(sizes, k, n, dtype, scales=True, seed=k).check()
@@ -874,9 +875,10 @@ def test_operands_beyond_32_bits(extra):
 def test_products_on_two_streams_at_once():
     """Each with its own buffer: a long product and many short ones, split and joined, side by side."""
     long = Forward([3000, 1, 2000], 1024, 2048, torch.bfloat16, seed=1)
-    short = Forward([2], 8208, 264, torch.bfloat16, seed=2)
+    short = Forward([20], 8208, 264, torch.bfloat16, seed=2)
+    few = Forward([2, 1], 520, 264, torch.bfloat16, seed=5)
     grad = Gradient([900, 0, 300], 256, 264, torch.bfloat16, seed=3)
-    cases = [long, short, grad]
+    cases = [long, short, grad, few]
     wants = []
     for case in cases:
         case.op()
@@ -888,7 +890,7 @@ def test_products_on_two_streams_at_once():
         case.c.zero_()
     torch.cuda.synchronize()
     for _ in range(20):
-        for case, times in ((long, 1), (short, 5), (grad, 3)):
+        for case, times in ((long, 1), (short, 5), (grad, 3), (few, 9)):
             for _ in range(times):
                 case.op()
     torch.cuda.synchronize()
