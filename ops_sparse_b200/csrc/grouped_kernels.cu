@@ -361,11 +361,13 @@ __device__ __forceinline__ void FewRows(const AclspGroupedParams& p, const FewOp
 // loads of single elements and of shifted vectors were measured, and the tensor cores are faster with the copy (3 rows,
 // 528 x 3823: 18 and 25 us against 12.7).
 template <int kIn>
-__global__ void __launch_bounds__(kFewThreads, 2) FewRowsKernel(const FewOperands operands, const AclspGroupedParams p)
+__global__ void __launch_bounds__(kFewThreads, 2) FewRowsKernel(const FewOperands operands,
+                                                                const AclspGroupedParams given)
 {
-    aclsp::WaitForPreviousKernel();
-    aclsp::LetNextKernelStart();
+    AclspGroupedParams p = given;
     FewOperands o = operands;
+    aclsp::WaitForPreviousKernel(o.a, o.b, p.offsets, p.rowScales, p.colScales, p.alphaPtr, p.betaPtr);
+    aclsp::LetNextKernelStart();
     o.alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
     o.beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
     constexpr uint32_t kWhole = 1u << 30;  // rows of a tile: a group is never cut
@@ -471,13 +473,14 @@ struct CopyJobs {
 // bytes).
 __global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const __grid_constant__ CopyJobs jobs, const int32_t* offsets)
 {
-    aclsp::WaitForPreviousKernel();
-    aclsp::LetNextKernelStart();
     const CopyJob& c = jobs.job[blockIdx.y];
+    const unsigned char* src = c.src;
+    aclsp::WaitForPreviousKernel(src, offsets);
+    aclsp::LetNextKernelStart();
     const uint32_t vectors = c.dstVectors.divisor;
     const uint32_t rows = c.rows.divisor;
     const uint64_t all = static_cast<uint64_t>(rows) * c.batches * vectors;
-    const unsigned char* const end = c.src + (c.batches - 1) * c.batchPitch + (rows - 1) * c.pitch + c.rowBytes;
+    const unsigned char* const end = src + (c.batches - 1) * c.batchPitch + (rows - 1) * c.pitch + c.rowBytes;
     const uint64_t threads = static_cast<uint64_t>(gridDim.x) * kCopyThreads;
 #pragma unroll 2
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < all; i += threads) {
@@ -491,11 +494,11 @@ __global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const __grid_cons
                 continue;  // nobody reads this matrix
             }
         }
-        const unsigned char* from = c.src + batch * c.batchPitch + static_cast<int64_t>(row) * c.pitch + byte;
+        const unsigned char* from = src + batch * c.batchPitch + static_cast<int64_t>(row) * c.pitch + byte;
         const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
         from -= shift;
         uint32_t w[8];
-        if (from >= c.src && from + 32 <= end) {
+        if (from >= src && from + 32 <= end) {
             const uint4 low = __ldg(reinterpret_cast<const uint4*>(from));
             const uint4 high = __ldg(reinterpret_cast<const uint4*>(from) + 1);
             w[0] = low.x, w[1] = low.y, w[2] = low.z, w[3] = low.w;
@@ -503,7 +506,7 @@ __global__ void __launch_bounds__(kCopyThreads) CopyRowsKernel(const __grid_cons
         } else {  // next to an end of the matrix
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
-                w[k] = WordOf(from + 4 * k, c.src, end);
+                w[k] = WordOf(from + 4 * k, src, end);
             }
         }
         // by eight bytes, by four, and by what is left of the shift

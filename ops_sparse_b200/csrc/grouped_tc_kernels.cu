@@ -567,14 +567,15 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             block += count;
         }
     } else if (warp == 3) {
+        AclspGroupedParams own = p;
         if (p.offsets != nullptr) {  // without them the schedule needs nothing from memory
-            WaitForPreviousKernel();
+            WaitForPreviousKernel(own.offsets);
         }
         auto schedule = [&]() {
             if constexpr (kGradient) {
-                return GradientSchedule(p, workers, kTileLanes * kCtas, kColumns, kBlock, joinBlocks);
+                return GradientSchedule(own, workers, kTileLanes * kCtas, kColumns, kBlock, joinBlocks);
             } else {
-                return ForwardSchedule(p, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
+                return ForwardSchedule(own, workers, kTileLanes * kCtas, kColumns, (p.k + kBlock - 1u) / kBlock, joinBlocks);
             }
         }();
         bool more = true;
@@ -593,9 +594,10 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             __syncwarp();
         }
     } else if (warp >= 4) {
-        WaitForPreviousKernel();
-        const float alpha = p.alphaPtr != nullptr ? *p.alphaPtr : p.alpha;
-        const float beta = p.betaPtr != nullptr ? *p.betaPtr : p.beta;
+        AclspGroupedParams own = p;
+        WaitForPreviousKernel(own.rowScales, own.colScales, own.alphaPtr, own.betaPtr);
+        const float alpha = p.alphaPtr != nullptr ? *own.alphaPtr : p.alpha;
+        const float beta = p.betaPtr != nullptr ? *own.betaPtr : p.beta;
         const uint32_t tmemLane = threadIdx.x % 128u;
         const uint32_t firstChunk = (warp - 4u) / 4u * 16u;  // of the columns: warps that share lanes take turns
         constexpr uint32_t kChunkStep = kResultWarps / 4u * 16u;
@@ -631,7 +633,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             const bool nothing = s.block0 == s.block1;  // an empty group's gradient: no sums were made
             float laneScale = alpha;
             if (!kGradient && p.colScales != nullptr && row < p.n) {
-                laneScale *= __ldg(p.colScales + static_cast<int64_t>(s.group) * p.n + row);
+                laneScale *= __ldg(own.colScales + static_cast<int64_t>(s.group) * p.n + row);
             }
             if (kGradient && s.parts == 1u && outMapped != 0u && beta == 0.0f) {
                 if constexpr (kGradient) {
@@ -699,7 +701,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                         for (uint32_t j = 0; j < 16; ++j) {
                             sums.v[j] = nothing ? 0.0f : SumToFloat<kInt8>(bits[j]);
                         }
-                        StoreResults<kGradient, decltype(type)>(p, c, s, row, j0, sums, laneScale, beta, turn);
+                        StoreResults<kGradient, decltype(type)>(own, c, s, row, j0, sums, laneScale, beta, turn);
                     }
                 });
                 release(half);
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                     sums.v[j] = SumToFloat<kInt8>(total[j]);
                 }
                 WithOutType(p.outType, [&](auto type) {
-                    StoreResults<kGradient, decltype(type)>(p, c, s, row, j0, sums, laneScale, beta, turn);
+                    StoreResults<kGradient, decltype(type)>(own, c, s, row, j0, sums, laneScale, beta, turn);
                 });
             }
         }

@@ -177,12 +177,12 @@ __device__ __forceinline__ void StoreBytes(signed char* to, const uint32_t (&q)[
 // arithmetic is that of the blocks on an SM: persistent blocks that ask for their next row before they work on the
 // present one need so many registers more that they are slower (16384 x 8192 bf16: 94 us against 86).
 template <int kIn, int kVec, uint32_t kLanes, int kHold, bool kTwice>
-__global__ void __launch_bounds__(kThreads, kVec == 1 ? 8 : 6) QuantizeRowsKernel(const void* __restrict__ x, signed char* __restrict__ q,
+__global__ void __launch_bounds__(kThreads, kVec == 1 ? 8 : 6) QuantizeRowsKernel(const void* x, signed char* __restrict__ q,
                                                                float* __restrict__ scales, uint32_t rows,
                                                                uint32_t cols, int64_t ldx, int64_t ldq)
 {
     __shared__ uint32_t warpTop[kThreads / 32];
-    aclsp::WaitForPreviousKernel();
+    aclsp::WaitForPreviousKernel(x);
     aclsp::LetNextKernelStart();
     constexpr uint32_t kRows = kThreads / kLanes;
     const uint32_t lane = threadIdx.x % kLanes;

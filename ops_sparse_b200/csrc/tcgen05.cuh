@@ -157,6 +157,19 @@ __device__ __forceinline__ void StoresDone() { asm volatile("cp.async.bulk.wait_
 // A kernel launched with programmatic serialization starts while the one before it in the stream still runs: nothing of
 // that one's may be read, nor anything written, before this wait.  The other call lets the next such kernel start.
 __device__ __forceinline__ void WaitForPreviousKernel() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+// The same, for a kernel that reads through these pointers with __ldg: such loads count as loads of memory that never
+// changes, which the compiler may move ahead of the wait, so the pointers are made known only behind it.
+template <typename T>
+__device__ __forceinline__ void KnownFromHere(T*& pointer)
+{
+    asm volatile("" : "+l"(pointer)::"memory");
+}
+template <typename... T>
+__device__ __forceinline__ void WaitForPreviousKernel(T*&... pointers)
+{
+    WaitForPreviousKernel();
+    (KnownFromHere(pointers), ...);
+}
 __device__ __forceinline__ void LetNextKernelStart() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 
 // Writes of this thread to shared memory become visible to the asynchronous proxy (TMA, tcgen05.mma).
