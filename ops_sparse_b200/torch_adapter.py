@@ -294,7 +294,8 @@ def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=No
     from . import api
     n = weight.size(1) if op_b == L.OP_T else weight.size(2)
     with torch.cuda.device(x.device):
-        y = torch.zeros(x.size(0), n, dtype=out_dtype, device=x.device)
+        # without offsets the one group is all rows
+        y = (torch.empty if offsets is None else torch.zeros)(x.size(0), n, dtype=out_dtype, device=x.device)
         if y.numel():
             with _stream_handle() as handle:
                 api.GroupedMM(handle, _rows_descr(_loadable(x)), _batch_descr(_loadable(weight)), _rows_descr(y),

@@ -757,6 +757,17 @@ def test_shifted_operands_give_the_same(shift):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows,k", [(1, 64), (5, 0), (40, 0), (40, 72), (300, 77)])
+def test_one_group_without_offsets(rows, k):
+    """Every element is written, whatever the memory held."""
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    x, w = randn(rows, k, dtype=torch.bfloat16, gen=gen), randn(1, 50, k, dtype=torch.bfloat16, gen=gen)
+    full = torch.full((rows, 50), float("nan"), dtype=torch.bfloat16, device=DEV)
+    del full  # the allocator hands this memory out again
+    y = A.grouped_mm(x, w)
+    close(y, x.double() @ w[0].double().T, sum_bound(k, x.double().abs() @ w[0].double().abs().T, False))
+
+
 def test_training_step_replays_in_a_graph():
     gen = torch.Generator(device=DEV).manual_seed(10)
     offsets = torch.tensor([0, 30, 30, 64], dtype=torch.int32, device=DEV)
