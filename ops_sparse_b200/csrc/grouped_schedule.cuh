@@ -63,7 +63,7 @@ public:
         tile_ = workers.index;
         whole_ = tiles_ / workers.count * workers.count;
         const uint32_t left = tiles_ - whole_;
-        // one part per SM: a second one there would only share its loads (one int8 token, 4096 x 4096: 8.9 us, 9.4 with two)
+        // one part per SM: a second one there would only share its loads (one int8 row, 4096 x 4096: 8.9 us, 9.4 with two)
         const uint32_t most = workers.count < kGroupedMaxCtas ? workers.count : kGroupedMaxCtas;
         if (left != 0u && 2u * left <= most && blocks > kMinSplitBlocks + joinBlocks) {
             const uint32_t parts = most / left;

@@ -14,8 +14,8 @@ constexpr uint32_t kGroupedHeaderWords = 16;
 // Where the partial sums begin; what is before them is what Preprocess clears.
 constexpr uint32_t kGroupedCountersEnd = 4u * (kGroupedHeaderWords + aclsp::kGroupedCounters);
 // What writing and joining partial sums costs, in blocks of the summed index: a tile is split only where more is saved
-// (two tokens through 1024 x 1024 matrices: 8.45 us with 8, 8.8 with 12; 8192 rows through 2048 x 4096 ones, 256 columns:
-// 124 us with 48, 126 with 24, 129 with 8).
+// (4 rows of 4 groups, 1024 x 1024 matrices, tensor cores: 8.45 us with 8, 8.8 with 12; 8192 rows through 2048 x 4096
+// ones, 256 columns: 124 us with 48, 126 with 24, 129 with 8).
 constexpr uint32_t kJoinBlocks = 8;
 constexpr uint32_t kJoinBlocksWide = 48;
 
