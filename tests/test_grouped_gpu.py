@@ -316,6 +316,53 @@ def test_forward_device_scalars():
     close(case.c, want, sum_bound(case.k, size, False))
 
 
+def test_forward_few_rows_device_scalars_and_replayed_with_other_offsets():
+    case = Forward([1, 2, 0, 4], 512, 320, torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    case.op.handle = api.Handle(side)
+    case.op.handle.set_pointer_mode(L.POINTER_MODE_DEVICE)
+    alpha, beta = torch.tensor([0.5], device=DEV), torch.tensor([0.0], device=DEV)
+    case.op.allocate()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        case.op(alpha, beta)
+    for bounds, scale in (([0, 1, 3, 3, 7], 0.5), ([0, 7, 7, 7, 7], -1.0), ([0, 0, 0, 5, 7], 2.0)):
+        case.offsets.copy_(torch.tensor(bounds, dtype=torch.int32))
+        alpha.fill_(scale)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, size = case.expected(scale, bounds=bounds)
+        close(case.c, want, sum_bound(case.k, size, False))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_each_product_sees_the_rows_quantised_just_before_it(rows):
+    """Kernels that start while the one before them ends, back to back, over the same few buffers."""
+    gen = torch.Generator(device=DEV).manual_seed(15)
+    x = torch.randn(30, rows, 1024, generator=gen, device=DEV).bfloat16()
+    w, w_scales = A.quantize_rows(torch.randn(512, 1024, generator=gen, device=DEV).bfloat16())
+    q, scales = torch.empty(rows, 1024, dtype=torch.int8, device=DEV), torch.empty(rows, device=DEV)
+    y = torch.empty(30, rows, 512, device=DEV)
+    handle, buffer = api.Handle(), None
+    steps = []
+    for i in range(30):
+        product = api.GroupedMM(handle, api.DnMat(rows, 1024, 1024, q), api.DnMat(512, 1024, 1024, w),
+                                api.DnMat(rows, 512, 512, y[i]), None, L.OP_T, scales, w_scales)
+        product.buffer = buffer = product.allocate() if buffer is None else buffer
+        steps.append((api.QuantizeRows(handle, api.DnMat(rows, 1024, 1024, x[i]), api.DnMat(rows, 1024, 1024, q), scales),
+                      product))
+    torch.cuda.synchronize()
+    for quantise, product in steps:
+        quantise()
+        product()
+    torch.cuda.synchronize()
+    for i in range(30):
+        qi, si = A.quantize_rows(x[i])
+        assert torch.equal(y[i], A.int8_mm(qi, w, si, w_scales, out_dtype=torch.float32))
+
+
 def test_forward_on_another_stream_and_in_a_graph():
     case = Forward([3, 0, 40, 1], 512, 320, torch.bfloat16)
     side = torch.cuda.Stream()
