@@ -242,6 +242,7 @@ typedef struct AclspGroupedParams {
     const int32_t* offsets;   /* groups + 1 values, or NULL: one group of all rows */
     const float* rowScales;
     const float* colScales;
+    uint64_t waitLimitNs;     /* longest wait of the tensor-core kernel before its CTA gives up; 0: four seconds */
 } AclspGroupedParams;
 
 /* Bytes of buffer that the launcher below wants for these parameters (a host computation). */

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
-from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libops_sparse.so")
@@ -95,7 +95,7 @@ class GroupedParams(ctypes.Structure):
                 ("aOuter", c_int64), ("aInner", c_int64), ("bOuter", c_int64), ("bInner", c_int64),
                 ("bBatchStride", c_int64), ("ldc", c_int64), ("cBatchStride", c_int64),
                 ("alpha", c_float), ("beta", c_float), ("alphaPtr", c_void_p), ("betaPtr", c_void_p),
-                ("offsets", c_void_p), ("rowScales", c_void_p), ("colScales", c_void_p)]
+                ("offsets", c_void_p), ("rowScales", c_void_p), ("colScales", c_void_p), ("waitLimitNs", c_uint64)]
 
 
 _P = c_void_p

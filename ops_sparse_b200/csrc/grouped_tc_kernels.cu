@@ -44,8 +44,9 @@
  * The set-up of a CTA overlaps the end of the kernel before (programmatic launch); each
  * warp waits for that one's memory before it touches its own.
  *
- * Every wait is bounded.  One that runs out makes the CTA leave: the loads in flight are
- * given time to land, tensor memory is freed, and the buffer's first word counts it.
+ * Every wait is bounded.  One that runs out makes the CTA leave, and the other of its pair:
+ * loads and MMAs in flight are given time to land, tensor memory is freed, and the
+ * buffer's first word counts it.
  */
 #include <atomic>
 #include <cstdint>
@@ -341,12 +342,13 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     const uint32_t tmem = tmemAddress;
     LetNextKernelStart();  // each warp waits for the previous one itself, before it touches global memory
     volatile uint32_t* const stop = &gaveUp;
+    const uint64_t limit = p.waitLimitNs;
 
     // The next segment of the schedule, for one of the warps that follow it; parts == 0 ends it.
     uint32_t taken = 0;
     auto nextSegment = [&](Segment* s) {
         const uint32_t i = taken % kSegments;
-        if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop))) {
+        if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop, limit))) {
             return false;
         }
         *s = segments[i];
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             const uint32_t rightAt = (kGradient ? s.right : s.row0) + rank * share;
             if (ElectLane()) {
                 for (uint32_t b = s.block0; b < s.block1; ++b) {
-                    if (!BarWait(SmemAddress(empty + stage), parity ^ 1u, stop)) {
+                    if (!BarWait(SmemAddress(empty + stage), parity ^ 1u, stop, limit)) {
                         good = false;
                         break;
                     }
@@ -441,12 +443,6 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             __syncwarp();
             good = __all_sync(0xFFFFFFFFu, good) != 0;
         }
-        // A CTA that gives up must not end under its copies: they have this long to land.
-        if (!good) {
-            const uint64_t began = Nanoseconds();
-            while (Nanoseconds() - began < kDrainNs) {
-            }
-        }
     } else if (warp == 1 && rank == 0u) {
         // One lane does it all: with the warp's votes and an election for each block, a block took 570 cycles to issue, and
         // the tensor cores need 512 for 256 columns, 384 for 192 (1024 x 1024 gradients of 2 x 4096 rows: 36.6 us then, 31.0
@@ -470,7 +466,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             // What this lane needs of the next segment; false at the end.
             auto take = [&](Work* w) {
                 const uint32_t i = taken % kSegments;
-                if (!BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop)) {
+                if (!BarWait(SmemAddress(segmentFull + i), taken / kSegments & 1u, stop, limit)) {
                     good = false;
                     return false;
                 }
@@ -485,7 +481,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             bool more = take(&w);
             while (more) {
                 const uint32_t half = tile & 1u;
-                good = BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop);
+                good = BarWait(SmemAddress(sumsEmpty + half), (tile >> 1 & 1u) ^ 1u, stop, limit);
                 if (!good) {
                     break;
                 }
@@ -498,14 +494,14 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
                     more = take(&next);
                 }
                 for (uint32_t b = w.block0; b < w.block1; ++b) {
-                    good = BarWait(SmemAddress(full + stage), parity, stop);
+                    good = BarWait(SmemAddress(full + stage), parity, stop, limit);
                     if (!good) {
                         break;
                     }
                     const uint32_t valid = w.length - b * kBlock < kBlock ? w.length - b * kBlock : kBlock;
                     if constexpr (kGradient) {
                         if (valid % kStepElements != 0u) {
-                            good = BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop);
+                            good = BarWait(SmemAddress(cutDone + stage), cuts >> stage & 1u, stop, limit);
                             cuts ^= 1u << stage;
                             if (!good) {
                                 break;
@@ -537,7 +533,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             if (!good) {  // not under instructions that still read tensor memory
                 uint32_t never = 0;
                 MmaCommit<kCtas>(SmemAddress(&drained));
-                (void)BarWait(SmemAddress(&drained), 0, &never);
+                (void)BarWait(SmemAddress(&drained), 0, &never, kWaitLimitNs);
             }
         }
         __syncwarp();
@@ -550,7 +546,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             const uint32_t valid = count != 0u ? validRows(s, s.block1 - 1u) : 0u;
             if (valid % kStepElements != 0u) {
                 const uint32_t stage = (block + count - 1u) % R::kStages;
-                if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutFull + stage), cuts >> stage & 1u, stop))) {
+                if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(cutFull + stage), cuts >> stage & 1u, stop, limit))) {
                     break;
                 }
                 cuts ^= 1u << stage;
@@ -584,7 +580,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             more = schedule.Next(&s);
             s.parts = more ? s.parts : 0u;
             const uint32_t i = given % kSegments;
-            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentEmpty + i), (given / kSegments & 1u) ^ 1u, stop))) {
+            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentEmpty + i), (given / kSegments & 1u) ^ 1u, stop, limit))) {
                 break;
             }
             if (lane == 0) {
@@ -623,7 +619,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
         };
         while (nextSegment(&s)) {
             const uint32_t half = tile & 1u;
-            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsFull + half), tile >> 1 & 1u, stop))) {
+            if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(sumsFull + half), tile >> 1 & 1u, stop, limit))) {
                 break;
             }
             ++tile;
@@ -799,11 +795,23 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     }
 
     __syncthreads();
-    if (threadIdx.x == 0 && gaveUp != 0u) {
-        atomicAdd(buffer, 1u);
-    }
     if constexpr (kCtas == 2) {
+        if (threadIdx.x == 0 && *stop != 0u) {
+            StorePeer(PeerAddress(SmemAddress(&gaveUp), rank ^ 1u), 1u);
+        }
         ClusterSync();  // neither CTA leaves while the other may still reach its shared memory
+    }
+    // Where a wait ran out, in any warp of this CTA or of the pair's other one, loads and MMAs may still be under way, also
+    // those of warps that ended as they should: neither CTA may free its tensor memory or leave its shared memory under
+    // them, so both give them time to land.
+    if (*stop != 0u) {
+        if (threadIdx.x == 0) {
+            atomicAdd(buffer, 1u);
+            const uint64_t began = Nanoseconds();
+            while (Nanoseconds() - began < kDrainNs) {
+            }
+        }
+        __syncthreads();
     }
     if (warp == 2) {
         TmemFenceAfter();
@@ -986,9 +994,11 @@ AclspGroupedOperands AclspGroupedDescribe(const AclspGroupedParams& p)
     return o;
 }
 
-bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
+bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& given,
                               cudaStream_t s)
 {
+    AclspGroupedParams p = given;
+    p.waitLimitNs = p.waitLimitNs != 0u ? p.waitLimitNs : kWaitLimitNs;
     constexpr uint32_t kLongest = 1u << 28;  // block and tile numbers stay far inside 32 bits
     constexpr uint64_t kFarthest = 1ull << 40;  // strides that a tensor map takes, in bytes
     const uint32_t columns = AclspGroupedColumns(p);

@@ -50,6 +50,11 @@ __device__ __forceinline__ void BarArrivePeer(uint32_t peerBar)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(peerBar) : "memory");
 }
 
+__device__ __forceinline__ void StorePeer(uint32_t peerAddress, uint32_t value)
+{
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(peerAddress), "r"(value) : "memory");
+}
+
 __device__ __forceinline__ void ClusterSync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
@@ -80,11 +85,11 @@ __device__ __forceinline__ uint64_t Nanoseconds()
     return t;
 }
 
-constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint64_t kWaitLimitNs = 4000000000ull;  // where nothing else is asked for
 
-// Waits for the phase of `parity` to end, four seconds at most.  `*gaveUp` is shared by the CTA: a wait that runs out
-// sets it, and every other wait then gives up too, so that the CTA leaves in bounded time.
-__device__ __forceinline__ bool BarWait(uint32_t bar, uint32_t parity, volatile uint32_t* gaveUp)
+// Waits for the phase of `parity` to end, `limit` nanoseconds at most.  `*gaveUp` is shared by the CTA: a wait that runs
+// out sets it, and every other wait then gives up too, so that the CTA leaves in bounded time.
+__device__ __forceinline__ bool BarWait(uint32_t bar, uint32_t parity, volatile uint32_t* gaveUp, uint64_t limit)
 {
     // The clock is looked at rarely: reading it takes longer than most waits.
     uint64_t began = 0;
@@ -95,7 +100,7 @@ __device__ __forceinline__ bool BarWait(uint32_t bar, uint32_t parity, volatile 
         if (spin % 256u == 255u) {
             const uint64_t now = Nanoseconds();
             began = began == 0u ? now : began;
-            if (*gaveUp != 0u || now - began > kWaitLimitNs) {
+            if (*gaveUp != 0u || now - began > limit) {
                 *gaveUp = 1u;
                 return false;
             }
