@@ -41,8 +41,9 @@
  * into place, were built and measured: 128 x 128 x 64 blocks took 3000 cycles instead of
  * 256 (2048 x 2049 matrices, 8192 rows: 620 us, with the copy 94 us).
  *
- * The set-up of a CTA overlaps the end of the kernel before (programmatic launch); each
- * warp waits for that one's memory before it touches its own.
+ * The set-up of a CTA overlaps the end of the kernel before (programmatic launch).  Each
+ * warp waits for that one before it touches memory, and before its first bounded wait: the
+ * kernel before may take as long as it likes.
  *
  * Every wait is bounded.  One that runs out makes the CTA leave, and the other of its pair:
  * loads and MMAs in flight are given time to land, tensor memory is freed, and the
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     }
     TmemFenceAfter();
     const uint32_t tmem = tmemAddress;
-    LetNextKernelStart();  // each warp waits for the previous one itself, before it touches global memory
+    LetNextKernelStart();  // each warp waits for the previous one itself, before it touches global memory or waits for another warp
     volatile uint32_t* const stop = &gaveUp;
     const uint64_t limit = p.waitLimitNs;
 
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
         // One lane does it all: with the warp's votes and an election for each block, a block took 570 cycles to issue, and
         // the tensor cores need 512 for 256 columns, 384 for 192 (1024 x 1024 gradients of 2 x 4096 rows: 36.6 us then, 31.0
         // now).
+        WaitForPreviousKernel();
         if (ElectLane()) {
             const bool leftT = kGradient || leftMn != 0u;
             const uint32_t shape = MmaShape(kCtas, kInt8, p.inType == ACLSP_TYPE_BF16, leftT, kGradient);
@@ -538,6 +540,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
         }
         __syncwarp();
     } else if (kGradient && warp == 2) {
+        WaitForPreviousKernel();
         Segment s;
         uint32_t block = 0;  // of all that this CTA loads: the stage is block % kStages
         uint32_t cuts = 0;   // a bit per stage: the parity of its next cut block
@@ -580,6 +583,9 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
             more = schedule.Next(&s);
             s.parts = more ? s.parts : 0u;
             const uint32_t i = given % kSegments;
+            if (given == kSegments) {
+                WaitForPreviousKernel();  // the first wait that others have to end
+            }
             if (!__all_sync(0xFFFFFFFFu, BarWait(SmemAddress(segmentEmpty + i), (given / kSegments & 1u) ^ 1u, stop, limit))) {
                 break;
             }

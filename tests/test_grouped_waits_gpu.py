@@ -80,3 +80,65 @@ def test_a_wait_that_runs_out_ends_the_product_and_is_counted(form):
     case.run(0)
     torch.cuda.synchronize()
     assert case.failures() == 0 and torch.equal(case.c, want)
+
+
+SLOW = """
+#include <cuda_runtime.h>
+// Lets the next kernel of the stream start at once, and ends after `ns` nanoseconds.
+__global__ void Slow(unsigned long long ns)
+{
+    asm volatile("griddepcontrol.launch_dependents;");
+    unsigned long long began, now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(began));
+    do {
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    } while (now - began < ns);
+}
+extern "C" int slow(unsigned long long ns, void* stream)
+{
+    Slow<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(ns);
+    return static_cast<int>(cudaGetLastError());
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def slow(tmp_path_factory):
+    """A kernel as other libraries may have them: its dependents start early, and it takes its time."""
+    import os
+    import subprocess
+    nvcc = "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no CUDA compiler")
+    where = tmp_path_factory.mktemp("slow")
+    (where / "slow.cu").write_text(SLOW)
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompiler", "-fPIC", str(where / "slow.cu"),
+                    "-o", str(where / "slow.so")], check=True)
+    fn = ctypes.CDLL(str(where / "slow.so")).slow
+    fn.argtypes, fn.restype = [ctypes.c_uint64, ctypes.c_void_p], ctypes.c_int
+    return fn
+
+
+BEHIND = {"narrow": dict(rows=20, n=600, k=1000), "wide": dict(rows=2000, n=1000, k=512),
+          "many tiles": dict(rows=2500, n=5000, k=128), "gradient, cut": dict(rows=1003, n=520, m=264),
+          "gradient, many tiles": dict(rows=1003, n=4000, m=4000)}
+
+
+@pytest.mark.parametrize("offsets", [False, True])
+@pytest.mark.parametrize("form", list(BEHIND))
+def test_the_limit_of_a_wait_does_not_count_the_kernel_before(slow, form, offsets):
+    """A product that starts 200 ms before the kernel in front of it ends, and may wait for 20 ms."""
+    case = Long(**BEHIND[form])
+    rows = torch.tensor([0, case.p.rows], dtype=torch.int32, device=DEV)
+    case.p.offsets = rows.data_ptr() if offsets else None
+    case.clear()
+    case.run(0)
+    torch.cuda.synchronize()
+    want = case.c.clone()
+    case.c[:-GUARD] = 0
+    case.clear()
+    torch.cuda.synchronize()
+    assert slow(200_000_000, case.stream) == 0
+    case.run(20_000_000)
+    assert case.failures() == 0
+    assert torch.equal(case.c, want) and not (want[:-GUARD] == 0).all()
