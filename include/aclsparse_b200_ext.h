@@ -159,11 +159,19 @@ aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t handle, con
                                                    aclsparseDnMatDescr_t matC, aclDataType computeType,
                                                    void* externalBuffer);
 
-/* How many CTAs of grouped products over `externalBuffer` gave up a wait since its counters were last cleared.  Every
- * wait of those kernels is bounded, at four seconds; a CTA whose wait runs out leaves its tiles unfinished and counts
- * itself here.  Anything but 0 means that results since then are not to be used; the call then clears the counters, so
- * that the next product can use the buffer again.  Synchronises `stream`.  No counterpart in the reference. */
+/* How many CTAs of grouped products over `externalBuffer` gave up a wait since its counters were last cleared: by
+ * Preprocess, by this call, or by a product that found no current Preprocess (every one in a capture) and cleared them
+ * itself, so that without Preprocess it speaks of the last product alone.  Every wait of those kernels is bounded, at four
+ * seconds from the end of the kernel before; a CTA whose wait runs out leaves its tiles unfinished and counts itself here,
+ * the other one of its pair too.  Anything but 0 means that results since then are not to be used; the call then clears
+ * the counters, so that the next product can use the buffer again.  The buffer has been through a Preprocess or a product
+ * with results to write.  Synchronises `stream`; in a capture: NOT_SUPPORTED.  No counterpart in the reference. */
 aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stream, void* externalBuffer, unsigned* count);
+
+/* The same count over every grouped product of this process on the current device, whatever its buffer and whether that
+ * still exists.  Nothing clears it: a reading that is larger than the one before means that a product which ended
+ * between them is incomplete.  Synchronises `stream`, and counts what has ended by then; in a capture: NOT_SUPPORTED. */
+aclsparseStatus_t aclsparseB200GroupedMMTotalWaitFailures(aclrtStream stream, unsigned* count);
 
 /* Rows of a matrix in 8 bits with one scale each, the operand of the int8 product above:
  *     scales[r] = max_k |X[r, k]| * (1 / 127)   (in fp32, 1 / 127 being its nearest fp32 number),

@@ -201,6 +201,7 @@ SIGNATURES = {
     "aclsparseB200GroupedMMWeightGradPreprocess": [_P, _P, _P, _P, _P, _P, _P, c_int, _P],
     "aclsparseB200GroupedMMWeightGrad": [_P, _P, _P, _P, _P, _P, _P, c_int, _P],
     "aclsparseB200GroupedMMWaitFailures": [_P, _P, POINTER(c_uint32)],
+    "aclsparseB200GroupedMMTotalWaitFailures": [_P, POINTER(c_uint32)],
     "aclsparseB200QuantizeRows": [_P, _P, _P, _P],
     # include/aclsparse_b200_kernels.h
     "spmv_b200_preprocess_kernel_do": [_P, _P, c_uint32, c_uint32, c_uint32, c_int32, c_int64, _P],

@@ -360,12 +360,23 @@ class _Grouped:
 
     def wait_failures(self) -> int:
         """CTAs that gave up a wait since the buffer's counters were last cleared (0 after healthy products); waits for
-        the handle's stream."""
+        the handle's stream.  Without ``preprocess`` every product clears them first: ``grouped_wait_failures`` counts
+        all products."""
         count, stream = ctypes.c_uint32(0), c_void_p(None)
         check("aclsparseGetStream", L.lib().aclsparseGetStream(self.handle.raw, byref(stream)))
         check("aclsparseB200GroupedMMWaitFailures",
               L.lib().aclsparseB200GroupedMMWaitFailures(stream, _ptr(self.buffer), byref(count)))
         return int(count.value)
+
+
+def grouped_wait_failures(stream: "torch.cuda.Stream | None" = None) -> int:
+    """CTAs of all grouped products of this process on the current device that gave up a wait; waits for ``stream`` (the
+    current one by default).  Nothing clears the count: a larger reading than before means incomplete results."""
+    count = ctypes.c_uint32(0)
+    s = (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+    check("aclsparseB200GroupedMMTotalWaitFailures",
+          L.lib().aclsparseB200GroupedMMTotalWaitFailures(c_void_p(s), byref(count)))
+    return int(count.value)
 
 
 class GroupedMM(_Grouped):

@@ -11,6 +11,7 @@
 
 #include "aclsparse_b200_ext.h"
 #include "aclsparse_b200_kernels.h"
+#include "grouped_tc.h"
 #include "internal.h"
 #include "plan_layout.h"
 
@@ -416,6 +417,9 @@ extern "C" aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stre
     if (externalBuffer == nullptr || count == nullptr) {
         return ACL_SPARSE_STATUS_INVALID_VALUE;
     }
+    if (IsCapturing(stream)) {
+        return ACL_SPARSE_STATUS_NOT_SUPPORTED;  // nothing has run yet, and a wait would end the capture
+    }
     auto s = static_cast<cudaStream_t>(stream);
     uint32_t value = 0;  // the buffer's first word
     if (cudaMemcpyAsync(&value, externalBuffer, sizeof(value), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
@@ -428,6 +432,23 @@ extern "C" aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stre
         aclsp_b200_grouped_preprocess_kernel_do(externalBuffer, stream);
         return Enqueued("aclsparseB200GroupedMMWaitFailures");
     }
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+extern "C" aclsparseStatus_t aclsparseB200GroupedMMTotalWaitFailures(aclrtStream stream, unsigned* count)
+{
+    if (count == nullptr) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    if (IsCapturing(stream)) {
+        return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    }
+    uint32_t value = 0;
+    if (AclspGroupedTotalWaitFailures(static_cast<cudaStream_t>(stream), &value) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return ACL_SPARSE_STATUS_EXECUTION_FAILED;
+    }
+    *count = value;
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 

@@ -55,6 +55,9 @@ void AclspGroupedCopyRows(AclspGroupedOperands* o, const void** left, const void
 bool AclspGroupedTensorLaunch(const void* a, const void* b, void* c, void* buffer, const AclspGroupedParams& p,
                               cudaStream_t stream);
 
+// CTAs on the current device that gave up a wait since the program began; waits for the stream.
+cudaError_t AclspGroupedTotalWaitFailures(cudaStream_t stream, uint32_t* count);
+
 // SMs of the current device, 0 when none can be queried (handle.cpp).
 uint32_t AclspSmCount();
 

@@ -47,7 +47,7 @@
  *
  * Every wait is bounded.  One that runs out makes the CTA leave, and the other of its pair:
  * loads and MMAs in flight are given time to land, tensor memory is freed, and the
- * buffer's first word counts it.
+ * buffer's first word and a word of the device's count it.
  */
 #include <atomic>
 #include <cstdint>
@@ -65,6 +65,10 @@
 namespace {
 
 using namespace aclsp;
+
+// CTAs on this device that gave up a wait since the program began.  The count in the buffer lives no longer than the buffer
+// or until its counters are cleared, which products do themselves; nothing clears this one.
+__device__ uint32_t gWaitFailures;
 
 // Narrow tiles are for few rows, where reading the dense matrix is all: two CTAs to an SM, with half its shared memory
 // each, so that one loads while the other starts or ends (32 groups of 4 rows, 2048 x 1024 matrices: 26.1 us, with one
@@ -813,6 +817,7 @@ __global__ void __launch_bounds__(kThreads<kColumns>, kCtasPerSm<kColumns>)
     if (*stop != 0u) {
         if (threadIdx.x == 0) {
             atomicAdd(buffer, 1u);
+            atomicAdd(&gWaitFailures, 1u);
             const uint64_t began = Nanoseconds();
             while (Nanoseconds() - began < kDrainNs) {
             }
@@ -908,6 +913,12 @@ void Launch(const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap
 }
 
 }  // namespace
+
+cudaError_t AclspGroupedTotalWaitFailures(cudaStream_t s, uint32_t* count)
+{
+    const cudaError_t err = cudaMemcpyFromSymbolAsync(count, gWaitFailures, sizeof(*count), 0, cudaMemcpyDeviceToHost, s);
+    return err != cudaSuccess ? err : cudaStreamSynchronize(s);
+}
 
 // The width of a tile.  What a choice costs is the number of turns that the workers take for all tiles times what a turn
 // takes: the blocks of the summed index at the rate that an SM gets operands from L2 (a block of a 128 x 32 tile is 20 KB,

@@ -15,6 +15,7 @@ The products between the sparse steps of a mixture-of-experts layer have no coun
     grouped_mm(x, weight, offsets)                        y[r] = x[r] @ weight[g].T for the rows r of group g, with gradients
     int8_mm(x, weight, x_scales, w_scales, offsets)       the same on int8 with one scale per row and per output column
     quantize_rows(x)                                      int8 rows and their scales
+    wait_failures(device)                                 whether products have ended without their results: 0 if none
 
 Argument errors are raised as ``ValueError`` / ``TypeError`` before anything is launched, in the order the reference
 checks them; the product itself runs through the C API on the current CUDA stream.  Like the reference's adapter,
@@ -381,6 +382,17 @@ def quantize_rows(x: torch.Tensor) -> "tuple[torch.Tensor, torch.Tensor]":
     return q, scales
 
 
+def wait_failures(device=None) -> int:
+    """CTAs of ``grouped_mm`` and ``int8_mm``, gradients among them, that gave up a (four seconds' bounded) wait on
+    ``device`` since the program began; waits for its current stream.
+
+    0 in healthy programs.  A reading larger than the one before means that results between them are incomplete.
+    """
+    from . import api
+    with torch.cuda.device(device):
+        return api.grouped_wait_failures()
+
+
 _installed = []
 
 
@@ -393,4 +405,5 @@ def install() -> None:
     _installed.append(lib)  # the registration lives as long as the Library object
 
 
-__all__ = ["mv", "mm", "addmm", "spmv_csr", "spmv_workspace", "grouped_mm", "int8_mm", "quantize_rows", "install"]
+__all__ = ["mv", "mm", "addmm", "spmv_csr", "spmv_workspace", "grouped_mm", "int8_mm", "quantize_rows", "wait_failures",
+           "install"]

@@ -142,3 +142,43 @@ def test_the_limit_of_a_wait_does_not_count_the_kernel_before(slow, form, offset
     case.run(20_000_000)
     assert case.failures() == 0
     assert torch.equal(case.c, want) and not (want[:-GUARD] == 0).all()
+
+
+def test_failures_outlive_the_buffer_and_the_next_product():
+    """What the adapter's user can ask: its buffers are gone after each call, and cleared before each."""
+    from ops_sparse_b200 import torch_adapter as A
+    case = Long(**LONG["several tiles"])
+    case.clear()
+    before = A.wait_failures()
+    case.run(1)
+    after = A.wait_failures()
+    assert 1 <= after - before <= 148
+    case.clear()                        # as a product does that finds no Preprocess
+    case.run(0)
+    assert case.failures() == 0         # the buffer's own count speaks of that product alone
+    del case
+    x, w = torch.randn(40, 64, device=DEV).bfloat16(), torch.randn(1, 48, 64, device=DEV).bfloat16()
+    y = A.grouped_mm(x, w)
+    assert torch.isfinite(y).all() and A.wait_failures(DEV) == after == api.grouped_wait_failures()
+
+
+def test_counts_are_refused_in_a_capture_and_leave_it_alone():
+    x, w = torch.randn(300, 512, device=DEV).bfloat16(), torch.randn(1, 256, 512, device=DEV).bfloat16()
+    c = torch.zeros(300, 256, device=DEV)
+    side = torch.cuda.Stream()
+    op = api.GroupedMM(api.Handle(side), api.DnMat(300, 512, 512, x), api.DnMat(256, 512, 512, w), api.DnMat(300, 256, 256, c),
+                       op_b=L.OP_T)
+    op.allocate()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        op()
+        for ask in (op.wait_failures, api.grouped_wait_failures):
+            with pytest.raises(api.AclsparseError) as refused:
+                ask()
+            assert refused.value.status == L.NOT_SUPPORTED
+    graph.replay()
+    torch.cuda.synchronize()
+    assert op.wait_failures() == 0
+    want = x.double() @ w[0].double().T
+    assert ((c.double() - want).abs() <= 520 * 2.0 ** -23 * (x.double().abs() @ w[0].double().abs().T)).all()
