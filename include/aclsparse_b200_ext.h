@@ -108,7 +108,8 @@ aclsparseStatus_t aclsparseB200DnMatSetClosingBarrier(aclsparseDnMatDescr_t mat,
  *   matA  rows x k, row-major.  matC  rows x n, row-major.  matB  one batch entry per group
  *         (aclsparseDnMatSetStridedBatch), op(B_g) is k x n, row- or column-major, op N / T (H is T).
  *   groupOffsets  DEVICE array of groups + 1 int32, ascending; NULL with a single group: all rows.  Its content is
- *         never trusted with an address: values are clamped to [0, rows], and to the largest one before them.
+ *         never trusted with an address: values are clamped to [0, rows], and to the largest one before them, so that
+ *         every row is in one group at most.
  *   rowScales (rows floats) and colScales (groups x n floats), DEVICE arrays, may be NULL: ones.
  *   types  A, B fp16 or bf16 with C of that type or fp32: fp32 sums; A, B int8 with C fp32, fp16 or bf16: exact
  *         int32 sums, k <= 131071.  The compute type is ACL_FLOAT.  The result is formed in fp32 and rounded once

@@ -17,6 +17,48 @@
 
 namespace aclsp {
 
+// An offset inside the matrix.
+__device__ __forceinline__ uint32_t ClampOffset(int32_t v, uint32_t rows)
+{
+    return v < 0 ? 0u : (static_cast<uint32_t>(v) > rows ? rows : static_cast<uint32_t>(v));
+}
+
+// The largest value of the lanes up to this one.
+__device__ __forceinline__ uint32_t RunningMax(uint32_t v)
+{
+    for (uint32_t d = 1; d < 32u; d *= 2u) {
+        const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        v = threadIdx.x % 32u >= d && up > v ? up : v;
+    }
+    return v;
+}
+
+// The rows of 32 groups from `base` on, one per lane.  Ends ascend whatever the array holds: none is below the largest
+// offset before it, of which *reached is the one before these groups, and then behind them.  Called by a whole warp.
+__device__ __forceinline__ void RowsOfGroups(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t base,
+                                             uint32_t* reached, uint32_t* begin, uint32_t* size)
+{
+    const uint32_t lane = threadIdx.x % 32u;
+    const uint32_t g = base + lane;
+    uint32_t first = 0;
+    uint32_t last = 0;
+    if (offsets == nullptr) {
+        last = g == 0 ? rows : 0u;
+    } else if (g < groups) {
+        first = ClampOffset(__ldg(offsets + g), rows);
+        last = ClampOffset(__ldg(offsets + g + 1), rows);
+    }
+    const uint32_t top = RunningMax(first > last ? first : last);
+    uint32_t before = __shfl_up_sync(0xFFFFFFFFu, top, 1);
+    before = lane == 0 ? 0u : before;
+    before = before > *reached ? before : *reached;
+    *begin = first > before ? first : before;
+    const uint32_t until = last > *begin ? last : *begin;
+    *size = g < groups ? until - *begin : 0u;
+    const uint32_t all = __shfl_sync(0xFFFFFFFFu, top, 31);
+    *reached = all > *reached ? all : *reached;
+}
+
 // One tile: `count` rows from row `row0` on, of group `group`; `across` is its place along the other dimension.
 struct GroupTile {
     uint32_t group;
@@ -89,7 +131,7 @@ public:
             uint32_t top = 0;
 #pragma unroll
             for (uint32_t i = 0; i <= kEach; ++i) {
-                bounds[i] = g0 < groups_ && g0 + i <= groups_ ? Clamp(__ldg(offsets_ + g0 + i)) : 0u;
+                bounds[i] = g0 < groups_ && g0 + i <= groups_ ? ClampOffset(__ldg(offsets_ + g0 + i), rows_) : 0u;
             }
 #pragma unroll
             for (uint32_t i = 0; i <= kEach; ++i) {
@@ -114,42 +156,10 @@ public:
 private:
     static constexpr uint32_t kBand = 8;
 
-    __device__ __forceinline__ uint32_t Clamp(int32_t v) const
-    {
-        return v < 0 ? 0u : (static_cast<uint32_t>(v) > rows_ ? rows_ : static_cast<uint32_t>(v));
-    }
-
-    // The largest value of the lanes up to this one.
-    static __device__ __forceinline__ uint32_t RunningMax(uint32_t v)
-    {
-        for (uint32_t d = 1; d < 32u; d *= 2u) {
-            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            v = threadIdx.x % 32u >= d && up > v ? up : v;
-        }
-        return v;
-    }
-
     __device__ __forceinline__ void Load()
     {
         const uint32_t lane = threadIdx.x % 32u;
-        const uint32_t g = base_ + lane;
-        uint32_t first = 0;
-        uint32_t last = 0;
-        if (offsets_ == nullptr) {
-            last = g == 0 ? rows_ : 0u;
-        } else if (g < groups_) {
-            first = Clamp(__ldg(offsets_ + g));
-            last = Clamp(__ldg(offsets_ + g + 1));
-        }
-        // ascending ends: the largest offset up to and including this group's end
-        uint32_t top = first > last ? first : last;
-        top = RunningMax(top);
-        uint32_t before = __shfl_up_sync(0xFFFFFFFFu, top, 1);
-        before = lane == 0 ? 0u : before;
-        before = before > reached_ ? before : reached_;
-        begin_ = first > before ? first : before;
-        const uint32_t until = last > begin_ ? last : begin_;
-        size_ = g < groups_ ? until - begin_ : 0u;
+        RowsOfGroups(offsets_, groups_, rows_, base_, &reached_, &begin_, &size_);
         uint32_t sum = (size_ + tileRows_ - 1u) / tileRows_ * across_;
         for (int d = 1; d < 32; d *= 2) {
             const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
@@ -157,8 +167,6 @@ private:
         }
         inclusive_ = sum + end_;
         end_ = __shfl_sync(0xFFFFFFFFu, inclusive_, 31);
-        const uint32_t chunkTop = __shfl_sync(0xFFFFFFFFu, top, 31);
-        reached_ = chunkTop > reached_ ? chunkTop : reached_;
     }
 
     const int32_t* offsets_;
@@ -174,23 +182,38 @@ private:
     uint32_t inclusive_ = 0;
 };
 
-// Rows of group g for a kernel that looks at one group only: clamped, never negative in number.
-__device__ __forceinline__ void GroupRows(const int32_t* offsets, uint32_t g, uint32_t rows, uint32_t* first,
-                                          uint32_t* last)
-{
-    if (offsets == nullptr) {
-        *first = 0;
-        *last = rows;
-        return;
+// The rows of one group after another, for a kernel whose warps all ask for the same groups in ascending order; the same
+// rows as above.
+class GroupRows {
+public:
+    __device__ __forceinline__ GroupRows(const int32_t* offsets, uint32_t rows) : offsets_(offsets), rows_(rows) {}
+
+    __device__ __forceinline__ void Find(uint32_t g, uint32_t* first, uint32_t* last)
+    {
+        if (offsets_ == nullptr) {
+            *first = 0;
+            *last = rows_;
+            return;
+        }
+        uint32_t top = 0;
+        for (uint32_t i = seen_ + threadIdx.x % 32u; i <= g; i += 32u) {
+            const uint32_t v = ClampOffset(__ldg(offsets_ + i), rows_);
+            top = v > top ? v : top;
+        }
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+        reached_ = top > reached_ ? top : reached_;
+        seen_ = g + 1u;
+        const uint32_t end = ClampOffset(__ldg(offsets_ + g + 1), rows_);
+        *first = reached_;
+        *last = end > reached_ ? end : reached_;
     }
-    const int64_t a = __ldg(offsets + g);
-    const int64_t b = __ldg(offsets + g + 1);
-    const int64_t top = rows;
-    const int64_t lo = a < 0 ? 0 : (a > top ? top : a);
-    const int64_t hi = b < lo ? lo : (b > top ? top : b);
-    *first = static_cast<uint32_t>(lo);
-    *last = static_cast<uint32_t>(hi);
-}
+
+private:
+    const int32_t* offsets_;
+    uint32_t rows_;
+    uint32_t seen_ = 0;     // offsets that have been looked at
+    uint32_t reached_ = 0;  // the largest of them
+};
 
 }  // namespace aclsp
 

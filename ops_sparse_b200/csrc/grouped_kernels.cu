@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
     const uint32_t across = (p.n + kPlainTile - 1u) / kPlainTile;
     const uint32_t down = (p.m + kPlainTile - 1u) / kPlainTile;
     GroupWalk walk(p.offsets, p.weightGrad != 0 ? 0u : p.groups, p.rows, kPlainTile, across);
+    aclsp::GroupRows groupRows(p.offsets, p.rows);
     const int tid = static_cast<int>(threadIdx.x);
     const int ti = tid / 16 * 4;
     const int tj = tid % 16;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kPlainThreads) PlainKernel(const void* __restr
             i0 = t / across % down * kPlainTile;
             iCount = p.m - i0;
             j0 = t % across * kPlainTile;
-            aclsp::GroupRows(p.offsets, group, p.rows, &k0, &k1);
+            groupRows.Find(group, &k0, &k1);
         } else {
             GroupTile tile;
             if (!walk.Find(t, &tile)) {

@@ -194,22 +194,16 @@ private:
         return (blocks + even - 1u) / even;
     }
 
-    __device__ __forceinline__ uint32_t Blocks(uint32_t g, uint32_t* first, uint32_t* size) const
-    {
-        uint32_t last;
-        GroupRows(offsets_, g, rows_, first, &last);
-        *size = last - *first;
-        return (*size + blockRows_ - 1u) / blockRows_;
-    }
-
     // The blocks of all tiles, and the longest tile's.
     __device__ __forceinline__ void Sum(uint32_t* blocks, uint32_t* longest) const
     {
         uint32_t sum = 0;
         uint32_t top = 0;
-        for (uint32_t g = threadIdx.x % 32u; g < groups_; g += 32u) {
-            uint32_t first, size;
-            const uint32_t own = Blocks(g, &first, &size);
+        uint32_t reached = 0;
+        for (uint32_t base = 0; base < groups_; base += 32u) {
+            uint32_t begin, size;
+            RowsOfGroups(offsets_, groups_, rows_, base, &reached, &begin, &size);
+            const uint32_t own = (size + blockRows_ - 1u) / blockRows_;
             sum += perGroup_ * own;
             top = own > top ? own : top;
         }
@@ -221,13 +215,8 @@ private:
     __device__ __forceinline__ void Load()
     {
         const uint32_t lane = threadIdx.x % 32u;
-        const uint32_t g = base_ + lane;
-        begin_ = 0;
-        size_ = 0;
-        uint32_t sum = 0;
-        if (g < groups_) {
-            sum = perGroup_ * Parts(Blocks(g, &begin_, &size_), length_);
-        }
+        RowsOfGroups(offsets_, groups_, rows_, base_, &reached_, &begin_, &size_);
+        uint32_t sum = base_ + lane < groups_ ? perGroup_ * Parts((size_ + blockRows_ - 1u) / blockRows_, length_) : 0u;
         for (int d = 1; d < 32; d *= 2) {
             const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
             sum += static_cast<int>(lane) >= d ? up : 0u;
@@ -250,6 +239,7 @@ private:
     uint32_t next_;                  // number of the next part
     uint32_t base_ = 0;
     uint32_t end_ = 0;
+    uint32_t reached_ = 0;  // largest offset before the groups that the lanes hold
     uint32_t begin_ = 0;
     uint32_t size_ = 0;
     uint32_t inclusive_ = 0;

@@ -1,0 +1,63 @@
+"""Calls of the grouped products that their documentation allows and that went wrong, or could: offsets that do not
+ascend, buffers whose memory had another use, products side by side that share nothing but the GPU."""
+import pytest
+import torch
+
+from ops_sparse_b200 import _lib as L
+from ops_sparse_b200 import api
+from ops_sparse_b200 import torch_adapter as A
+from tests.test_grouped_gpu import DEV, Forward, Gradient, close, randn, sum_bound
+
+pytestmark = pytest.mark.gpu
+
+
+def ascending(bounds, rows):
+    """Each offset inside the matrix, and none below one before it."""
+    top, out = 0, []
+    for b in bounds:
+        top = max(top, min(max(b, 0), rows))
+        out.append(top)
+    return out
+
+
+def check_gradient(case, bounds):
+    case.offsets.copy_(torch.tensor(bounds, dtype=torch.int32))
+    case.bounds = ascending(bounds, case.a.shape[0])
+    case.check()
+
+
+@pytest.mark.parametrize("shift", [(0, 0, 0), (1, 0, 0)], ids=["tensor cores", "plain"])
+@pytest.mark.parametrize("bounds", [[-5, 40, 20, 2 ** 31 - 1], [0, 50, 20, 80], [90, 60, 30, 0], [-7, 10, 10 ** 9, 90],
+                                    [2 ** 31 - 1, -2 ** 31, 5, 6], [30, 10, 60, 40]])
+def test_gradient_of_bad_offsets_has_every_row_once_at_most(bounds, shift):
+    """The groups are those of the forward product, so that the gradient stays its derivative."""
+    check_gradient(Gradient([30, 30, 30], 64, 48, torch.bfloat16, pad=(8, 8, 0), shift=shift), bounds)
+
+
+@pytest.mark.parametrize("shift", [(0, 0, 0), (0, 1, 0)], ids=["tensor cores", "plain"])
+@pytest.mark.parametrize("groups", [31, 32, 33, 64, 300])
+def test_gradient_of_bad_offsets_of_many_groups(groups, shift):
+    case = Gradient([3] * groups, 136, 72, torch.bfloat16, pad=(8, 8, 0), shift=shift, seed=groups)
+    rows = 3 * groups
+    steps = torch.randint(-40, 61, (groups + 1,), generator=torch.Generator().manual_seed(groups))
+    check_gradient(case, (torch.arange(groups + 1) * rows // groups + steps).tolist())
+
+
+@pytest.mark.parametrize("bounds", [[0, 9000, 3000, 12000], [4000, 100, 11000, 11999], [0, 12000, 5000, 12000]])
+def test_gradient_of_bad_offsets_split_along_the_rows(bounds):
+    check_gradient(Gradient([4000, 4000, 4000], 136, 264, torch.bfloat16, seed=4), bounds)
+
+
+def test_gradient_of_bad_offsets_is_the_derivative_of_the_product():
+    """Through the adapter: what autograd gets is the formula's gradient for the rows that the product used."""
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    x, w = randn(90, 64, dtype=torch.bfloat16, gen=gen), randn(3, 48, 64, dtype=torch.bfloat16, gen=gen)
+    dy = randn(90, 48, dtype=torch.bfloat16, gen=gen)
+    offsets = torch.tensor([0, 50, 20, 80], dtype=torch.int32, device=DEV)
+    w1 = w.clone().requires_grad_()
+    y = A.grouped_mm(x, w1, offsets, out_dtype=torch.float32)
+    gw, = torch.autograd.grad(y, w1, dy.float())
+    for g, (first, last) in enumerate([(0, 50), (50, 50), (50, 80)]):
+        r = slice(first, last)
+        close(y[r].detach(), x[r].double() @ w[g].double().T, sum_bound(64, x[r].double().abs() @ w[g].double().abs().T, False))
+        close(gw[g], dy[r].double().T @ x[r].double(), sum_bound(50, dy[r].double().abs().T @ x[r].double().abs(), False))
