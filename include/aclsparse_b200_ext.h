@@ -120,7 +120,10 @@ aclsparseStatus_t aclsparseB200DnMatSetClosingBarrier(aclsparseDnMatDescr_t mat,
  * empty group costs nothing; k == 0 gives beta * C.  C must not overlap A or B.  Results do not depend on
  * scheduling.  The buffer holds partial sums of products split along k: 64-byte aligned, one call at a time.
  * Preprocess clears its counters; it is optional: a product that finds no Preprocess of its matC for this buffer
- * on this stream clears them itself, with one more launch.  Asynchronous on the handle's stream.
+ * on this stream clears them itself, with one more launch.  A Preprocess holds until another one or another operator is
+ * given the buffer, or GetBufferSize is asked for this matC again; until then nothing else may write to the buffer, so
+ * memory that has had another use in between, or comes from another allocation at the same address, needs one of the two
+ * first.  Asynchronous on the handle's stream.
  * No counterpart in the reference. */
 aclsparseStatus_t aclsparseB200GroupedMMGetBufferSize(aclsparseHandle_t handle, aclsparseOperation_t opB,
                                                       const void* alpha, aclsparseConstDnMatDescr_t matA,

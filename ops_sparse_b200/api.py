@@ -328,9 +328,19 @@ class _Grouped:
     not made anew."""
 
     name = ""
+    _buffer = None
+    _unknown = False  # the buffer is new to this operator: what a Preprocess of C left at its address is not in it
 
     def _args(self, pa, pb):
         raise NotImplementedError
+
+    @property
+    def buffer(self):
+        return self._buffer
+
+    @buffer.setter
+    def buffer(self, buffer) -> None:
+        self._buffer, self._unknown = buffer, True
 
     def _call(self, phase: str, alpha, beta, last) -> None:
         pa, pb, _keep = _scalars(alpha, beta) if isinstance(alpha, torch.Tensor) else _float_scalars(alpha, beta)
@@ -346,17 +356,22 @@ class _Grouped:
     def allocate(self, alpha=1.0, beta=0.0):
         n = self.buffer_size(alpha, beta)
         self.buffer = torch.empty(max(n, 64), dtype=torch.uint8, device=self.c.values.device)
+        self._unknown = False  # asking for the size has forgotten it
         return self.buffer
 
     def preprocess(self, alpha=1.0, beta=0.0) -> None:
-        if self.buffer is None:
+        if self._buffer is None:
             self.allocate(alpha, beta)
-        self._call("Preprocess", alpha, beta, self.buffer.data_ptr())
+        self._call("Preprocess", alpha, beta, self._buffer.data_ptr())
+        self._unknown = False
 
     def __call__(self, alpha=1.0, beta=0.0) -> None:
-        if self.buffer is None:
+        if self._buffer is None:
             self.allocate(alpha, beta)
-        self._call("", alpha, beta, self.buffer.data_ptr())
+        if self._unknown:
+            self.buffer_size(alpha, beta)  # forgets the Preprocess
+            self._unknown = False
+        self._call("", alpha, beta, self._buffer.data_ptr())
 
     def wait_failures(self) -> int:
         """CTAs that gave up a wait since the buffer's counters were last cleared (0 after healthy products); waits for
@@ -396,7 +411,6 @@ class GroupedMM(_Grouped):
         _device_array("col_scales", col_scales, torch.float32, b.batch_count * c.cols)
         self.handle, self.a, self.b, self.c, self.op_b = handle, a, b, c, op_b
         self.offsets, self.row_scales, self.col_scales = offsets, row_scales, col_scales
-        self.buffer = None
 
     def _args(self, pa, pb):
         return (self.handle.raw, self.op_b, pa, self.a.raw, _address(self.offsets), self.b.raw, _address(self.row_scales),
@@ -411,7 +425,6 @@ class GroupedMMWeightGrad(_Grouped):
     def __init__(self, handle: Handle, a: DnMat, b: DnMat, c: DnMat, offsets=None):
         _device_array("offsets", offsets, torch.int32, c.batch_count + 1)
         self.handle, self.a, self.b, self.c, self.offsets = handle, a, b, c, offsets
-        self.buffer = None
 
     def _args(self, pa, pb):
         return (self.handle.raw, pa, self.a.raw, self.b.raw, _address(self.offsets), pb, self.c.raw, L.ACL_FLOAT)

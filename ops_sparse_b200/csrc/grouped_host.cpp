@@ -303,6 +303,8 @@ extern "C" aclsparseStatus_t aclsparseB200GroupedMMGetBufferSize(
     st = DescribeForward(kMm, matA, matB, matC, opB, groupOffsets, rowScales, colScales, computeType, &p);
     if (st == ACL_SPARSE_STATUS_SUCCESS) {
         *bufferSize = static_cast<size_t>(aclsp_b200_grouped_buffer_bytes(&p));
+        // The caller is about to bring a buffer.  It may lie where the last one did, with anything in it.
+        matC->grouped = GroupedPlanRecord{};
     }
     return st;
 }
@@ -364,6 +366,8 @@ extern "C" aclsparseStatus_t aclsparseB200GroupedMMWeightGradGetBufferSize(
     st = DescribeGradient(kGrad, matA, matB, matC, groupOffsets, computeType, &p, &swap);
     if (st == ACL_SPARSE_STATUS_SUCCESS) {
         *bufferSize = static_cast<size_t>(aclsp_b200_grouped_buffer_bytes(&p));
+        // The caller is about to bring a buffer.  It may lie where the last one did, with anything in it.
+        matC->grouped = GroupedPlanRecord{};
     }
     return st;
 }

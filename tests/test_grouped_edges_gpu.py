@@ -61,3 +61,76 @@ def test_gradient_of_bad_offsets_is_the_derivative_of_the_product():
         r = slice(first, last)
         close(y[r].detach(), x[r].double() @ w[g].double().T, sum_bound(64, x[r].double().abs() @ w[g].double().abs().T, False))
         close(gw[g], dy[r].double().T @ x[r].double(), sum_bound(50, dy[r].double().abs().T @ x[r].double().abs(), False))
+
+
+# ---- buffers ----
+
+def split_product():
+    """A product whose tiles are split, so that it lives by the counters in its buffer, and its result."""
+    case = Forward([20], 16400, 264, torch.bfloat16)
+    case.op.preprocess()
+    case.op()
+    torch.cuda.synchronize()
+    want, size = case.expected()
+    close(case.c, want, sum_bound(case.k, size, False))
+    return case, case.c.clone()
+
+
+def again(case):
+    return api.GroupedMM(case.op.handle, case.op.a, case.op.b, case.op.c, case.op.offsets, case.op.op_b)
+
+
+def test_a_buffer_at_the_address_of_an_earlier_one_is_cleared():
+    """The result's descriptor remembers a Preprocess by the buffer's address; the memory has had another use since."""
+    case, want = split_product()
+    address, size, op = case.op.buffer.data_ptr(), case.op.buffer.numel(), again(case)
+    case.op = None
+    other = torch.empty(size, dtype=torch.uint8, device=DEV).fill_(0xAB)
+    assert other.data_ptr() == address
+    del other
+    case.c.zero_()
+    op()
+    assert op.buffer.data_ptr() == address and torch.equal(case.c, want)
+
+
+def test_a_buffer_that_is_handed_over_is_cleared():
+    case, want = split_product()
+    buffer, op = case.op.buffer, again(case)
+    for fresh in (op, case.op):  # another operator's, and the same one's again
+        buffer.fill_(0xCD)
+        fresh.buffer = buffer
+        case.c.zero_()
+        fresh()
+        assert torch.equal(case.c, want)
+    case.op.preprocess()
+    case.c.zero_()
+    case.op()
+    assert torch.equal(case.c, want)
+
+
+def test_asking_for_the_size_ends_a_preprocess():
+    """As a program in C does that frees its buffer, asks for the size again and goes on without a Preprocess."""
+    case, want = split_product()
+    case.op.buffer.fill_(0xEF)
+    case.op.buffer_size()
+    case.c.zero_()
+    case.op()
+    assert torch.equal(case.c, want)
+
+
+def test_gradient_buffer_at_the_address_of_an_earlier_one_is_cleared():
+    case = Gradient([9000], 136, 264, torch.bfloat16)
+    case.op.preprocess()
+    case.op()
+    want, (handle, a, b, c, offsets) = case.c.clone(), (case.op.handle, case.op.a, case.op.b, case.op.c, case.op.offsets)
+    address, size = case.op.buffer.data_ptr(), case.op.buffer.numel()
+    case.op = None
+    other = torch.empty(size, dtype=torch.uint8, device=DEV).fill_(0xAB)
+    assert other.data_ptr() == address
+    del other
+    case.c.zero_()
+    op = api.GroupedMMWeightGrad(handle, a, b, c, offsets)
+    op()
+    assert op.buffer.data_ptr() == address and torch.equal(case.c, want)
+    want64, size64, most = case.expected()
+    close(case.c, want64, sum_bound(most, size64, False))
