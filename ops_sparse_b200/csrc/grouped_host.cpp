@@ -276,7 +276,7 @@ aclsparseStatus_t Execute(const char* api, aclsparseContext* h, const void* a, c
                        AclspPlanIsCurrent(buffer, r.serial) && !IsCapturing(h->stream);
     if (!clear) {
         aclsp_b200_grouped_preprocess_kernel_do(buffer, h->stream);
-        (void)AclspPublishPlan(buffer);  // whatever plan the buffer held is gone
+        AclspForgetPlan(buffer);  // whatever plan the buffer held is gone
     }
     aclsp_b200_grouped_mm_kernel_do(a, b, c->values, buffer, &p, h->stream);
     return Enqueued(api);

@@ -176,8 +176,10 @@ uint64_t AclspNextWorkspaceOwnerId();
 
 // Plan ownership of workspace buffers (plan_registry.cpp).  AclspPublishPlan records that `buffer` now
 // holds a freshly built plan and returns its serial number; AclspPlanIsCurrent says whether the plan
-// with that serial is still the last one built in `buffer`.
+// with that serial is still the last one built in `buffer`.  AclspForgetPlan: the buffer was written to and holds
+// no plan any more.
 uint64_t AclspPublishPlan(const void* buffer);
+void AclspForgetPlan(const void* buffer);
 bool AclspPlanIsCurrent(const void* buffer, uint64_t serial);
 void AclspResetSpmvPlan(aclsparseSpMatDescr* descr);
 

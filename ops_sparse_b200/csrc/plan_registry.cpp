@@ -6,7 +6,9 @@
  * So every plan build takes a fresh serial number, writes it next to the
  * descriptor's record and publishes (buffer -> serial) here; a product reuses
  * the plan in a buffer only while the buffer's published serial is still its
- * own.  The reference keeps such a registry for SpMM, keyed by the workspace
+ * own.  An operator that writes to a buffer without leaving a plan in it takes
+ * the entry out and adds none, so that its buffers, of which there may be many,
+ * push no plan out.  The reference keeps such a registry for SpMM, keyed by the workspace
  * address (sparse/spmm/arch35/host/spmm_host.cpp:99-228, an LRU of 1024
  * entries, sparse/spmm/arch35/host/spmm_host_internal.h:56-112); its SpMV
  * records a plan only in Preprocess (sparse/spmv/arch35/spmv_host.cpp:578).
@@ -65,6 +67,17 @@ uint64_t AclspPublishPlan(const void* buffer)
         r.order.pop_back();
     }
     return serial;
+}
+
+void AclspForgetPlan(const void* buffer)
+{
+    Registry& r = TheRegistry();
+    std::lock_guard<std::mutex> lock(r.mutex);
+    const auto it = r.entries.find(buffer);
+    if (it != r.entries.end()) {
+        r.order.erase(it->second.where);
+        r.entries.erase(it);
+    }
 }
 
 bool AclspPlanIsCurrent(const void* buffer, uint64_t serial)

@@ -1,5 +1,6 @@
 """Calls of the grouped products that their documentation allows and that went wrong, or could: offsets that do not
 ascend, buffers whose memory had another use, products side by side that share nothing but the GPU."""
+import numpy as np
 import pytest
 import torch
 
@@ -134,3 +135,25 @@ def test_gradient_buffer_at_the_address_of_an_earlier_one_is_cleared():
     assert op.buffer.data_ptr() == address and torch.equal(case.c, want)
     want64, size64, most = case.expected()
     close(case.c, want64, sum_bound(most, size64, False))
+
+
+def test_plans_of_sparse_products_outlive_any_number_of_grouped_products():
+    """A grouped product without Preprocess keeps no plan in its buffer: a thousand buffers push no SpMV plan out."""
+    from tests.gpu_util import SpmvCase, random_csr
+    row_ptr, col_ind = random_csr(np.random.default_rng(3), [8] * 300, 200)
+    sparse = SpmvCase(row_ptr, col_ind, np.ones(2400), np.ones(200), np.zeros(300))
+    sparse.run()
+    before = api.kernel_launches()
+    sparse.run(preprocess=False)
+    each = api.kernel_launches() - before
+    x, w = torch.randn(2, 64, device=DEV).bfloat16(), torch.randn(1, 32, 64, device=DEV).bfloat16()
+    c = torch.empty(2, 32, device=DEV)
+    op = api.GroupedMM(api.Handle(), api.DnMat(2, 64, 64, x), api.DnMat(32, 64, 64, w), api.DnMat(2, 32, 32, c), op_b=L.OP_T)
+    size = -(-op.buffer_size() // 64) * 64
+    many = torch.empty(1100 * size, dtype=torch.uint8, device=DEV)
+    for i in range(1100):
+        op.buffer = many[i * size:(i + 1) * size]
+        op()
+    before = api.kernel_launches()
+    sparse.run(preprocess=False)
+    assert api.kernel_launches() - before == each
