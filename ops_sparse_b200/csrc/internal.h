@@ -177,10 +177,10 @@ uint64_t AclspNextWorkspaceOwnerId();
 // Plan ownership of workspace buffers (plan_registry.cpp).  AclspPublishPlan records that `buffer` now
 // holds a freshly built plan and returns its serial number; AclspPlanIsCurrent says whether the plan
 // with that serial is still the last one built in `buffer`.  AclspForgetPlan: the buffer was written to and holds
-// no plan any more.
-uint64_t AclspPublishPlan(const void* buffer);
-void AclspForgetPlan(const void* buffer);
-bool AclspPlanIsCurrent(const void* buffer, uint64_t serial);
+// no plan any more.  A serial of 0 (no memory to record it) is never current.
+uint64_t AclspPublishPlan(const void* buffer) noexcept;
+void AclspForgetPlan(const void* buffer) noexcept;
+bool AclspPlanIsCurrent(const void* buffer, uint64_t serial) noexcept;
 void AclspResetSpmvPlan(aclsparseSpMatDescr* descr);
 
 // Logging: ACLSPARSE_LOG_LEVEL=0 (off, default) / 1 (errors) / 2 (info) / 3 (debug) -> stderr.

@@ -8,7 +8,8 @@
  * the plan in a buffer only while the buffer's published serial is still its
  * own.  An operator that writes to a buffer without leaving a plan in it takes
  * the entry out and adds none, so that its buffers, of which there may be many,
- * push no plan out.  The reference keeps such a registry for SpMM, keyed by the workspace
+ * push no plan out.  Nothing here throws: the callers are C functions.
+ * The reference keeps such a registry for SpMM, keyed by the workspace
  * address (sparse/spmm/arch35/host/spmm_host.cpp:99-228, an LRU of 1024
  * entries, sparse/spmm/arch35/host/spmm_host_internal.h:56-112); its SpMV
  * records a plan only in Preprocess (sparse/spmv/arch35/spmv_host.cpp:578).
@@ -47,48 +48,61 @@ std::atomic<uint64_t> gNextSerial{1};
 
 }  // namespace
 
-uint64_t AclspPublishPlan(const void* buffer)
+uint64_t AclspPublishPlan(const void* buffer) noexcept
 {
     const uint64_t serial = gNextSerial.fetch_add(1, std::memory_order_relaxed);
     if (buffer == nullptr) {
         return serial;
     }
-    Registry& r = TheRegistry();
-    std::lock_guard<std::mutex> lock(r.mutex);
-    auto it = r.entries.find(buffer);
-    if (it != r.entries.end()) {
-        r.order.erase(it->second.where);
-        r.entries.erase(it);
+    try {
+        Registry& r = TheRegistry();
+        std::lock_guard<std::mutex> lock(r.mutex);
+        const auto it = r.entries.find(buffer);
+        if (it != r.entries.end()) {  // no memory is needed
+            it->second.serial = serial;
+            r.order.splice(r.order.begin(), r.order, it->second.where);
+            return serial;
+        }
+        std::list<const void*> added{buffer};
+        r.entries.emplace(buffer, Registry::Entry{serial, added.begin()});
+        r.order.splice(r.order.begin(), added);  // its iterators stay valid
+        while (r.entries.size() > kMaxEntries) {  // the oldest buffer is forgotten: its plan will be rebuilt
+            r.entries.erase(r.order.back());
+            r.order.pop_back();
+        }
+        return serial;
+    } catch (...) {
+        return 0;  // no memory for the entry: the buffer counts as one without a plan
     }
-    r.order.push_front(buffer);
-    r.entries.emplace(buffer, Registry::Entry{serial, r.order.begin()});
-    while (r.entries.size() > kMaxEntries) {  // the oldest buffer is forgotten: its plan will be rebuilt
-        r.entries.erase(r.order.back());
-        r.order.pop_back();
-    }
-    return serial;
 }
 
-void AclspForgetPlan(const void* buffer)
+void AclspForgetPlan(const void* buffer) noexcept
 {
-    Registry& r = TheRegistry();
-    std::lock_guard<std::mutex> lock(r.mutex);
-    const auto it = r.entries.find(buffer);
-    if (it != r.entries.end()) {
-        r.order.erase(it->second.where);
-        r.entries.erase(it);
+    try {
+        Registry& r = TheRegistry();
+        std::lock_guard<std::mutex> lock(r.mutex);
+        const auto it = r.entries.find(buffer);
+        if (it != r.entries.end()) {
+            r.order.erase(it->second.where);
+            r.entries.erase(it);
+        }
+    } catch (...) {  // no memory for the registry itself: there is nothing to forget
     }
 }
 
-bool AclspPlanIsCurrent(const void* buffer, uint64_t serial)
+bool AclspPlanIsCurrent(const void* buffer, uint64_t serial) noexcept
 {
     if (buffer == nullptr || serial == 0) {
         return false;
     }
-    Registry& r = TheRegistry();
-    std::lock_guard<std::mutex> lock(r.mutex);
-    const auto it = r.entries.find(buffer);
-    return it != r.entries.end() && it->second.serial == serial;
+    try {
+        Registry& r = TheRegistry();
+        std::lock_guard<std::mutex> lock(r.mutex);
+        const auto it = r.entries.find(buffer);
+        return it != r.entries.end() && it->second.serial == serial;
+    } catch (...) {
+        return false;
+    }
 }
 
 namespace {
