@@ -343,7 +343,10 @@ class _Grouped:
         self._buffer, self._unknown = buffer, True
 
     def _call(self, phase: str, alpha, beta, last) -> None:
-        pa, pb, _keep = _scalars(alpha, beta) if isinstance(alpha, torch.Tensor) else _float_scalars(alpha, beta)
+        if isinstance(alpha, torch.Tensor):
+            pa, pb, _keep = _scalars(alpha, beta)
+        else:  # looked up by value: an object that stands for a number may stand for another one by the next call
+            pa, pb, _keep = _float_scalars(float(alpha), float(beta))
         status = getattr(L.lib(), self.name + phase)(*self._args(pa, pb), last)
         if status != L.SUCCESS:
             raise AclsparseError(self.name + phase, status)
