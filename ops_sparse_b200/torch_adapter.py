@@ -280,14 +280,17 @@ def _batch_descr(w: torch.Tensor):
     return api.DnMat(rows, cols, ld, w, order, groups, w.stride(0) if groups > 1 else 0)
 
 
-def _loadable(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy where its first element alone keeps its rows from multiples of 16 bytes.
+def _loadable(describe, t: torch.Tensor):
+    """``describe(t)``, of a copy where its first element alone keeps its rows from multiples of 16 bytes.
 
     The tensor-core kernels load from such multiples.  Rows of odd widths are copied by the library, in the buffer, but
-    that has no room for an operand that is merely shifted.
+    that has no room for an operand that is merely shifted.  The strides that count are the descriptor's: a tensor's own
+    say nothing where a dimension has one element (a row cut out of a matrix of odd width keeps that width as its stride).
     """
-    even = all(s == 1 or s * t.element_size() % 16 == 0 for s in t.stride())
-    return t.clone() if even and t.data_ptr() % 16 else t
+    d = describe(t)
+    unit = d.values.element_size()
+    even = d.ld * unit % 16 == 0 and d.batch_stride * unit % 16 == 0
+    return describe(d.values.clone()) if even and d.values.data_ptr() % 16 else d
 
 
 def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=None):
@@ -299,7 +302,7 @@ def _forward(x, weight, offsets, out_dtype, op_b, row_scales=None, col_scales=No
         y = (torch.empty if offsets is None else torch.zeros)(x.size(0), n, dtype=out_dtype, device=x.device)
         if y.numel():
             with _stream_handle() as handle:
-                api.GroupedMM(handle, _rows_descr(_loadable(x)), _batch_descr(_loadable(weight)), _rows_descr(y),
+                api.GroupedMM(handle, _loadable(_rows_descr, x), _loadable(_batch_descr, weight), _rows_descr(y),
                               None if offsets is None else offsets.contiguous(), op_b, row_scales, col_scales)()
     return y
 
@@ -323,7 +326,7 @@ class _GroupedMM(torch.autograd.Function):
                 dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
                 if dw.numel():
                     with _stream_handle() as handle:
-                        api.GroupedMMWeightGrad(handle, _rows_descr(_loadable(dy)), _rows_descr(_loadable(x)), _batch_descr(dw),
+                        api.GroupedMMWeightGrad(handle, _loadable(_rows_descr, dy), _loadable(_rows_descr, x), _batch_descr(dw),
                                                 None if offsets is None else offsets.contiguous())()
         return dx, dw, None, None
 

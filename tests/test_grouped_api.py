@@ -42,3 +42,33 @@ def test_a_scalar_that_changes_its_value_is_read_at_every_call(monkeypatch, make
     op(2, np.float32(0.25))
     op(True, 1)
     assert op.seen[-4:] == [(1.0, 0.5), (1.0, 2.0), (2.0, 0.25), (1.0, 1.0)]
+
+
+def shifted(shape, stride, shift, dtype=torch.float16):
+    store = torch.zeros(shift + 1 + sum((n - 1) * s for n, s in zip(shape, stride)), dtype=dtype)
+    assert store.data_ptr() % 16 == 0
+    return store[shift:].as_strided(shape, stride, store.storage_offset() + shift)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.int8])
+def test_adapter_copies_operands_that_are_merely_shifted(dtype):
+    """One row, one matrix, one column: the strides of what there is only one of do not make an operand odd."""
+    from ops_sparse_b200 import torch_adapter as A
+    rows, batch = A._rows_descr, A._batch_descr
+    for describe, shape, stride in ((rows, (1, 784), (777, 1)), (rows, (3, 784), (784, 1)), (rows, (1, 784), (1, 1)),
+                                    (rows, (5, 16), (800, 1)), (batch, (1, 9, 784), (6993, 784, 1)),
+                                    (batch, (1, 1, 784), (6993, 777, 1)), (batch, (3, 1, 784), (784, 777, 1)),
+                                    (batch, (1, 784, 9), (7001, 1, 784))):
+        for shift in (1, 3, 15):
+            t = shifted(shape, stride, shift, dtype)
+            t.copy_(torch.arange(t.numel()).reshape(shape) % 100)
+            d = A._loadable(describe, t)
+            assert d.values.data_ptr() % 16 == 0 and torch.equal(d.values, t)
+            assert d.ld == {3: lambda: d.ld, 2: lambda: d.values.stride(0) if shape[0] > 1 else shape[1]}[len(shape)]()
+        d = A._loadable(describe, shifted(shape, stride, 0, dtype))
+        assert d.values.data_ptr() % 16 == 0
+    # rows that the library copies anyway are described as they are, wherever they start
+    for describe, shape, stride in ((rows, (1, 777), (784, 1)), (rows, (3, 777), (777, 1)), (batch, (2, 5, 48), (777, 48, 1)),
+                                    (batch, (1, 784, 1), (7001, 1, 777))):  # the last: rows of one element, one apart
+        t = shifted(shape, stride, 1, dtype)
+        assert A._loadable(describe, t).values.data_ptr() == t.data_ptr()

@@ -157,3 +157,31 @@ def test_plans_of_sparse_products_outlive_any_number_of_grouped_products():
     before = api.kernel_launches()
     sparse.run(preprocess=False)
     assert api.kernel_launches() - before == each
+
+
+# ---- operands cut out of larger ones ----
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_rows_cut_out_of_a_matrix_of_odd_width_are_computed_as_others(dtype, rows):
+    """The same kernel, and so the same bits; one row's stride is that of the matrix it was cut out of."""
+    gen = torch.Generator(device=DEV).manual_seed(23)
+    big = randn(40, 777, dtype=dtype, gen=gen)
+    x = big[3:3 + rows, :776]
+    w = randn(1, 520, 776, dtype=dtype, gen=gen)
+    got = A.grouped_mm(x, w, out_dtype=torch.float32)
+    close(got, x.double() @ w[0].double().T, sum_bound(776, x.double().abs() @ w[0].double().abs().T, False))
+    if rows == 1:  # more rows of an odd pitch go through the library's own copy
+        assert x.stride(0) == 777 and x.data_ptr() % 16 != 0
+    assert torch.equal(got, A.grouped_mm(x.contiguous().clone(), w, out_dtype=torch.float32))
+    odd = randn(2, 521, 777, dtype=dtype, gen=gen)[1:2, 1:2, :776]  # one row of one matrix, as weights
+    assert torch.equal(A.grouped_mm(x, odd, out_dtype=torch.float32),
+                       A.grouped_mm(x.contiguous().clone(), odd.contiguous().clone(), out_dtype=torch.float32))
+
+
+def test_one_int8_row_cut_out_of_a_matrix_of_odd_width():
+    gen = torch.Generator(device=DEV).manual_seed(24)
+    x, w = randn(5, 777, dtype=torch.int8, gen=gen)[2:3, :768], randn(264, 768, dtype=torch.int8, gen=gen)
+    one, scales = torch.ones(1, device=DEV), torch.ones(264, device=DEV)
+    assert x.data_ptr() % 16 != 0
+    assert torch.equal(A.int8_mm(x, w, one, scales, out_dtype=torch.float32).double(), x.double() @ w.double().T)
