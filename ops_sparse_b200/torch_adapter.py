@@ -255,8 +255,10 @@ def _check_offsets(offsets, groups: int, device) -> None:
 
 
 def _rows_descr(t: torch.Tensor):
-    """Row-major descriptor of a 2-D tensor; a copy is made where a row is not contiguous or rows overlap."""
+    """Row-major descriptor of a 2-D tensor; a copy is made where a row is not contiguous or rows overlap, and of a view
+    that stands for the negative of its memory."""
     from . import api
+    t = t.resolve_neg()
     if t.size(1) > 1 and t.stride(1) != 1 or t.size(0) > 1 and t.stride(0) < t.size(1):
         t = t.contiguous()
     return api.DnMat(t.size(0), t.size(1), t.stride(0) if t.size(0) > 1 else t.size(1), t)
@@ -265,6 +267,7 @@ def _rows_descr(t: torch.Tensor):
 def _batch_descr(w: torch.Tensor):
     """Descriptor of a 3-D tensor, one matrix per group, rows or columns contiguous; else a copy is described."""
     from . import api
+    w = w.resolve_neg()
     groups, rows, cols = w.shape
 
     def fits(outer, outer_stride, inner, inner_stride):

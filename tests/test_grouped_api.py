@@ -72,3 +72,16 @@ def test_adapter_copies_operands_that_are_merely_shifted(dtype):
                                     (batch, (1, 784, 1), (7001, 1, 777))):  # the last: rows of one element, one apart
         t = shifted(shape, stride, 1, dtype)
         assert A._loadable(describe, t).values.data_ptr() == t.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [torch.complex32, torch.complex64])
+def test_adapter_resolves_views_that_stand_for_a_negative(dtype):
+    """The imaginary part of a conjugate is the memory's negative, not the memory."""
+    from ops_sparse_b200 import torch_adapter as A
+    z = torch.arange(48, dtype=torch.float32).to(dtype) * 1j
+    for describe, shape in ((A._rows_descr, (48, 1)), (A._rows_descr, (6, 8)), (A._batch_descr, (2, 3, 8)), (A._batch_descr, (2, 24, 1))):
+        t = z.reshape(shape).conj().imag
+        assert t.is_neg()
+        d = describe(t)
+        assert not d.values.is_neg()
+        assert torch.equal(d.values.float().flatten(), -torch.arange(48, dtype=torch.float32))
