@@ -185,3 +185,37 @@ def test_one_int8_row_cut_out_of_a_matrix_of_odd_width():
     one, scales = torch.ones(1, device=DEV), torch.ones(264, device=DEV)
     assert x.data_ptr() % 16 != 0
     assert torch.equal(A.int8_mm(x, w, one, scales, out_dtype=torch.float32).double(), x.double() @ w.double().T)
+
+
+# ---- side by side ----
+
+def test_prepared_products_side_by_side_reuse_their_counters():
+    """Four streams, each with a buffer that is cleared once: split tiles leave their counters at zero for the next product,
+    with others' tiles on the same SMs, and no wait runs out in any of them."""
+    long = Forward([3000, 1, 2000], 1024, 2048, torch.bfloat16, seed=1)
+    split = Forward([20], 16400, 264, torch.bfloat16, seed=2)
+    int8 = Forward([40, 9], 8208, 264, torch.int8, seed=5)
+    grad = Gradient([9000, 0, 3000], 256, 264, torch.bfloat16, seed=3)
+    turns = ((long, 1), (split, 5), (grad, 3), (int8, 9))
+    wants = []
+    for case, _ in turns:
+        case.check()
+        wants.append(case.c.clone())
+    for case, _ in turns:
+        case.op.handle = api.Handle(torch.cuda.Stream())
+        case.c.zero_()
+    torch.cuda.synchronize()
+    before = api.grouped_wait_failures()
+    for case, _ in turns:
+        case.op.preprocess()
+    launches = api.kernel_launches()
+    for _ in range(20):
+        for case, times in turns:
+            for _ in range(times):
+                case.op()
+    assert api.kernel_launches() - launches == 20 * sum(times for _, times in turns)  # nobody cleared anything again
+    torch.cuda.synchronize()
+    for (case, _), want in zip(turns, wants):
+        assert torch.equal(case.c, want)
+        assert case.op.wait_failures() == 0
+    assert api.grouped_wait_failures() == before
