@@ -117,7 +117,8 @@ aclsparseStatus_t aclsparseB200DnMatSetClosingBarrier(aclsparseDnMatDescr_t mat,
  * A and B should start on multiples of 16 bytes: rows of any width and leading dimension run on the tensor cores, a
  * matrix that is merely shifted does not and takes many times as long.
  * Rows of C outside [groupOffsets[0], groupOffsets[groups]) are left as they are; beta == 0 does not read C; an
- * empty group costs nothing; k == 0 gives beta * C.  C must not overlap A or B.  Results do not depend on
+ * empty group costs nothing; k == 0 gives beta * C; alpha == 0 multiplies the sums like any other alpha (an infinity or a
+ * NaN in them gives NaN).  C must not overlap A or B.  Results do not depend on
  * scheduling.  The buffer holds partial sums of products split along k: 64-byte aligned, one call at a time.
  * Preprocess clears its counters; it is optional: a product that finds no Preprocess of its matC for this buffer
  * on this stream clears them itself, with one more launch.  A Preprocess holds until another one or another operator is

@@ -5,9 +5,8 @@
  * The work is done on the tensor cores (grouped_tc_kernels.cu).  Here are the
  * kernels around that: FewRowsKernel for a few tokens, CopyRowsKernel, which brings
  * operands of odd widths to rows that TMA can load, and PlainKernel for what is left:
- * bases that are not 16-byte
- * aligned, sums over nothing, and sizes beyond 2^28.  It computes 64 x 64 tiles,
- * operands staged through shared memory element by element, products and sums in
+ * bases that are not 16-byte aligned, sums over nothing, and sizes beyond 2^28.  It
+ * computes 64 x 64 tiles, operands staged through shared memory element by element, products and sums in
  * registers (fp32 FMA; int32 for int8).
  */
 #include <cstdint>

@@ -13,12 +13,12 @@
  * Wide tiles (256 columns) are computed by a pair of CTAs on neighbouring SMs, 256 x
  * 256 results: each holds 128 rows of the dense matrix and half of the ragged rows,
  * and one MMA reads both.  A single CTA would have to load 48 KB for 512 cycles of
- * MMA, more than the 52 bytes per cycle that an SM was measured to get from L2 with
- * all of them loading; the pair loads 32 KB each.  A block of a pair then takes 0.39 us
- * (0.28 us of MMAs alone, 0.27 us of loads alone): what bounds it is shared memory, which
- * the loads write while the MMAs read it.  One group of 18944 rows, 1024 x 8192: 1500
- * TFLOP/s; 8192 rows of 16 groups, 2048 x 4096, run 200 times without a pause at the clock
- * that the power limit leaves: 133 us, 1030 TFLOP/s.
+ * MMA, more than the 49 to 63 bytes per cycle that an SM was measured to get with all
+ * of them loading; the pair loads 32 KB each.  A block of a pair then takes 572 cycles, 560
+ * with the loads left out and 523 with the MMAs left out: what bounds it are the MMAs, at
+ * the clock that the power limit leaves (1.1 GHz without a pause, 1.65 without the loads).
+ * One group of 18944 rows, 1024 x 8192: 217 us in a short run, 1470 TFLOP/s, and 264 us,
+ * 1200 TFLOP/s, without a pause; 8192 rows of 16 groups, 2048 x 4096, without a pause: 146 us.
  *
  * CTAs are persistent: warp 0 loads blocks of 128 bytes of the summed index into a
  * ring of stages, one lane of warp 1 issues the MMAs, warps from 4 on read the

@@ -13,10 +13,12 @@
  * A division per element would cost more than reading and writing the element.
  *
  * Bound by HBM: the row is read once, kept in registers between its maximum and its
- * quotients, and written (16384 x 8192 bf16: 73.5 us, 5.5 TB/s; 64 x 4096: 2.6 us).  A row
- * is a warp's where rows are short and many, a block's otherwise; rows too long for the
- * registers are read twice, the second time from L2.  Rows that do not start on 16-byte
- * boundaries are read element by element (16384 x 8001 fp16: 152 us).
+ * quotients, and written (16384 x 8192 bf16: 74.5 us, 5.4 TB/s, 78 without a pause; 64 x 4096:
+ * 2.6 us).  A row is a warp's where rows are short and many, a block's otherwise.  Rows of
+ * more than 8192 16-bit or 4096 32-bit elements take a form that spills 80 bytes a thread,
+ * and what passes twice that length is read twice, the second time from L2 (8192 x 14336 bf16:
+ * 81 us, 4.4 TB/s; 4096 x 28672: 85).  Rows that do not start on 16-byte boundaries are read
+ * element by element (16384 x 8001 fp16: 147 us).
  */
 #include <cstdint>
 
