@@ -351,14 +351,24 @@ class _Grouped:
         if status != L.SUCCESS:
             raise AclsparseError(self.name + phase, status)
 
+    def _stream(self) -> int:
+        """The handle's stream as PyTorch names it: 0 is the default one."""
+        stream = c_void_p(None)
+        check("aclsparseGetStream", L.lib().aclsparseGetStream(self.handle.raw, byref(stream)))
+        return 0 if stream.value in (None, 0x1) else stream.value
+
     def buffer_size(self, alpha=1.0, beta=0.0) -> int:
         size = c_size_t(0)
         self._call("GetBufferSize", alpha, beta, byref(size))
         return int(size.value)
 
     def allocate(self, alpha=1.0, beta=0.0):
-        n = self.buffer_size(alpha, beta)
-        self.buffer = torch.empty(max(n, 64), dtype=torch.uint8, device=self.c.values.device)
+        n, device = self.buffer_size(alpha, beta), self.c.values.device
+        stream = self._stream()
+        # memory of the stream that uses it: what is freed there is given out again behind the products
+        other = stream if stream != torch.cuda.current_stream(device).cuda_stream else None
+        with torch.cuda.stream(None if other is None else torch.cuda.ExternalStream(other, device=device)):
+            self.buffer = torch.empty(max(n, 64), dtype=torch.uint8, device=device)
         self._unknown = False  # asking for the size has forgotten it
         return self.buffer
 

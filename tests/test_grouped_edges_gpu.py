@@ -219,3 +219,23 @@ def test_prepared_products_side_by_side_reuse_their_counters():
         assert torch.equal(case.c, want)
         assert case.op.wait_failures() == 0
     assert api.grouped_wait_failures() == before
+
+
+def test_a_buffer_stays_its_streams_own_until_the_product_has_run():
+    """An operator on a stream of its own, dropped while its product waits there: nobody else gets the buffer before."""
+    case, want = split_product()
+    side = torch.cuda.Stream()
+    handle = api.Handle(side)
+    op = api.GroupedMM(handle, case.op.a, case.op.b, case.op.c, case.op.offsets, case.op.op_b)
+    case.c.zero_()
+    torch.cuda.synchronize()
+    op.preprocess()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+    op()
+    size = op.buffer.numel()
+    del op  # the handle lives on: destroying it would wait for the stream
+    others = [torch.full((size,), 0xAB, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(case.c, want)
+    del others, handle
