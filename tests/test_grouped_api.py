@@ -85,3 +85,7 @@ def test_adapter_resolves_views_that_stand_for_a_negative(dtype):
         d = describe(t)
         assert not d.values.is_neg()
         assert torch.equal(d.values.float().flatten(), -torch.arange(48, dtype=torch.float32))
+
+
+def test_count_of_wait_failures_refuses_no_result(lib):
+    assert lib.aclsparseB200GroupedMMTotalWaitFailures(None, None) == L.INVALID_VALUE
