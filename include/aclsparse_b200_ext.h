@@ -169,8 +169,8 @@ aclsparseStatus_t aclsparseB200GroupedMMWeightGrad(aclsparseHandle_t handle, con
  * itself, so that without Preprocess it speaks of the last product alone.  Every wait of those kernels is bounded, at four
  * seconds from the end of the kernel before; a CTA whose wait runs out leaves its tiles unfinished and counts itself here,
  * the other one of its pair too.  Anything but 0 means that results since then are not to be used; the call then clears
- * the counters, so that the next product can use the buffer again.  The buffer has been through a Preprocess or a product
- * with results to write.  Synchronises `stream`; in a capture: NOT_SUPPORTED.  No counterpart in the reference. */
+ * the counters, so that the next product can use the buffer again.  The buffer has been through a Preprocess or a
+ * product.  Synchronises `stream`; in a capture: NOT_SUPPORTED.  No counterpart in the reference. */
 aclsparseStatus_t aclsparseB200GroupedMMWaitFailures(aclrtStream stream, void* externalBuffer, unsigned* count);
 
 /* The same count over every grouped product of this process on the current device, whatever its buffer and whether that

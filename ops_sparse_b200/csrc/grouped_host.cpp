@@ -267,9 +267,6 @@ aclsparseStatus_t Preprocess(const char* api, aclsparseContext* h, aclsparseDnMa
 aclsparseStatus_t Execute(const char* api, aclsparseContext* h, const void* a, const void* b, aclsparseDnMatDescr* c,
                           void* buffer, const AclspGroupedParams& p)
 {
-    if ((p.weightGrad == 0 && p.rows == 0) || p.n == 0 || (p.weightGrad != 0 && p.m == 0)) {
-        return ACL_SPARSE_STATUS_SUCCESS;  // nothing to write
-    }
     (void)cudaGetLastError();
     const GroupedPlanRecord& r = c->grouped;
     const bool clear = r.buffer == buffer && r.stream == h->stream && r.streamEpoch == h->streamEpoch &&
@@ -277,6 +274,10 @@ aclsparseStatus_t Execute(const char* api, aclsparseContext* h, const void* a, c
     if (!clear) {
         aclsp_b200_grouped_preprocess_kernel_do(buffer, h->stream);
         AclspForgetPlan(buffer);  // whatever plan the buffer held is gone
+    }
+    if ((p.weightGrad == 0 && p.rows == 0) || p.n == 0 || (p.weightGrad != 0 && p.m == 0)) {
+        (void)cudaGetLastError();
+        return ACL_SPARSE_STATUS_SUCCESS;  // nothing to write, which needs no GPU either; the buffer counts no failures
     }
     aclsp_b200_grouped_mm_kernel_do(a, b, c->values, buffer, &p, h->stream);
     return Enqueued(api);

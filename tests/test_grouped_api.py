@@ -89,3 +89,19 @@ def test_adapter_resolves_views_that_stand_for_a_negative(dtype):
 
 def test_count_of_wait_failures_refuses_no_result(lib):
     assert lib.aclsparseB200GroupedMMTotalWaitFailures(None, None) == L.INVALID_VALUE
+
+
+def test_a_product_without_results_needs_no_gpu(lib):
+    h, one, made = ctypes.c_void_p(None), ctypes.byref(ctypes.c_float(1.0)), []
+    assert lib.aclsparseCreate(ctypes.byref(h)) == L.SUCCESS
+    for rows, cols in ((0, 16), (24, 16), (0, 24)):
+        d = ctypes.c_void_p(None)
+        assert lib.aclsparseCreateDnMat(ctypes.byref(d), rows, cols, cols, 0x10000, L.ACL_BF16, L.ORDER_ROW) == L.SUCCESS
+        made.append(d)
+    buffer = np.zeros(1 << 17, np.uint8)  # what stands for the device's memory where there is none
+    if not torch.cuda.is_available():
+        at = buffer.ctypes.data + -buffer.ctypes.data % 64
+        assert lib.aclsparseB200GroupedMM(h, L.OP_T, one, made[0], None, made[1], None, None, one, made[2], L.ACL_FLOAT, at) == L.SUCCESS
+    for d in made:
+        assert lib.aclsparseDestroyDnMat(d) == L.SUCCESS
+    assert lib.aclsparseDestroy(h) == L.SUCCESS

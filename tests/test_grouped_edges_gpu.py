@@ -239,3 +239,11 @@ def test_a_buffer_stays_its_streams_own_until_the_product_has_run():
     torch.cuda.synchronize()
     assert torch.equal(case.c, want)
     del others, handle
+
+
+def test_a_product_without_results_leaves_no_count_of_failures():
+    """Nothing is launched for it, and whatever its buffer's memory held is no count."""
+    for case in (Forward([0, 0], 64, 48, torch.bfloat16), Gradient([5], 64, 0, torch.bfloat16)):
+        case.op.allocate().fill_(0xAB)
+        case.op()
+        assert case.op.wait_failures() == 0
